@@ -549,6 +549,61 @@ int dsa_sparse_decode_heads_bf16(const void* q_nope, int64_t qn_stride_t, int64_
                                  int32_t num_tokens, int32_t num_heads, float scale, void* out, int64_t out_stride_t,
                                  int64_t out_stride_h, float* lse_out /* fp32 [T,N] or NULL */, mlahip_stream_t stream);
 
+/* ---- layers with ordinary key and value heads ------------------------------------------------
+ * No counterpart on the latent path above: what a layer with query heads and fewer (or as many) key and value heads runs around a
+ * paged cache [pages, page, heads, dim] of its own, keys and values apart (attention/backends/attention.py:216-281 is the
+ * reference's backend for such layers).  Type codes: 0 = bf16, 1 = fp32, 2 = fp16, 3 = fp8-e4m3.
+ *
+ * The step in front, one launch: RMSNorm of every query and key head over its dim values (q_gamma / k_gamma [dim] of the inputs'
+ * type, NULL: none; y = x * rsqrt(mean(x^2) + eps) * gamma), rotary positions on the first rotary_dim values (tables cos / sin
+ * [table_rows, rotary_dim / 2], fp32 or bf16, rows cs_stride elements apart, the row of positions[t]; interleaved = 0: pairs
+ * (i, i + rotary_dim / 2), 1: (2i, 2i + 1); the result is laid out as the input), all in fp32 and rounded once; queries to q_out
+ * (may be q), keys and values to the cache row slot_mapping[t] (negative or past the cache: not written), rotated keys to k_out too
+ * where it is not NULL (may be k).  Caches of the inputs' type, or e4m3 (code 3): x / k_scale[head], x / v_scale[head] (NULL: 1),
+ * values beyond +-448 become +-448.  A token whose position is not in the tables is not written anywhere.  kv_heads = 0: queries
+ * alone; without caches (all three pointers NULL) v is not read.  dim and rotary_dim: multiples of 16 up to 256. */
+int mlahip_qk_norm_rope_cache(
+    const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t, int64_t k_stride_h, const void* v,
+    int64_t v_stride_t, int64_t v_stride_h, int64_t num_tokens, int32_t q_heads, int32_t kv_heads, int32_t dim, int32_t dtype,
+    const void* q_gamma, const void* k_gamma, float eps, const void* cos, const void* sin, int64_t cs_stride, int64_t table_rows,
+    int32_t table_dtype, int32_t rotary_dim, int32_t interleaved, const int64_t* positions, const int64_t* slot_mapping,
+    void* k_cache, int64_t kc_page_stride, int64_t kc_row_stride, int64_t kc_head_stride, void* v_cache, int64_t vc_page_stride,
+    int64_t vc_row_stride, int64_t vc_head_stride, int32_t page_size, int64_t num_pages, int32_t cache_dtype, const float* k_scale,
+    const float* v_scale, void* q_out, int64_t qo_stride_t, int64_t qo_stride_h, void* k_out, int64_t ko_stride_t,
+    int64_t ko_stride_h, mlahip_stream_t stream);
+
+/* Attention of each request's newest tokens over that cache: token i of a request's s tokens (rows [b * max_q_len, ..) of q, or
+ * [query_start_loc[b], query_start_loc[b + 1])) sees keys j <= seq_lens[b] - s + i, and with window > 0 only j > that - window.
+ * q [num_tokens, q_heads, dim] (bf16 or fp16), caches of its type or e4m3 (times k_scale / v_scale [kv_heads] fp32, NULL: 1), query
+ * head h with key head h / (q_heads / kv_heads), dim 64, 128 or 256, pages of a multiple of 16 tokens.  out as q through its
+ * strides; lse_out fp32 [num_tokens, q_heads] or NULL: log of the sum of exp(scores).  A row that sees no key gives zeros and -inf.
+ * seq_lens beyond the block table's room count as that room; page numbers outside the cache are read as its first or last page.
+ * num_chunks > 0: the keys of all requests, end to end, are cut into that many equal pieces, a workgroup each (times groups of
+ * heads and rows), and a second launch joins the pieces of a request, with mlahip_gqa_decode_workspace_bytes of workspace;
+ * 0: one launch, a request to a workgroup, no workspace. */
+size_t mlahip_gqa_decode_workspace_bytes(int32_t batch, int32_t max_q_len, int32_t q_heads, int32_t dim, int32_t num_chunks);
+int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t num_tokens, const void* k_cache,
+                      int64_t kc_page_stride, int64_t kc_row_stride, int64_t kc_head_stride, const void* v_cache,
+                      int64_t vc_page_stride, int64_t vc_row_stride, int64_t vc_head_stride, int64_t num_pages, int32_t page_size,
+                      const int32_t* block_table, int64_t bt_stride, int32_t max_blocks, const int32_t* seq_lens,
+                      const int32_t* query_start_loc /* may be NULL */, int32_t batch, int32_t max_q_len, int32_t q_heads,
+                      int32_t kv_heads, int32_t dim, int32_t dtype, int32_t cache_dtype, const float* k_scale, const float* v_scale,
+                      float scale, int32_t window, void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse_out,
+                      void* workspace, size_t workspace_bytes, int32_t num_chunks, mlahip_stream_t stream);
+
+/* ---- pages of a cache, any cache -------------------------------------------------------------
+ * cache[dst[i], r] = cache[src[i], r] for r < rows[i] (rows = NULL: whole pages) in every cache of the list, in as few launches as
+ * hold their arguments.  caches, src, dst and rows are HOST arrays, read before the call returns (a captured graph keeps the pairs of its
+ * capture).  A destination named twice, or one that is a source too, is refused: the copies have no order.
+ * block_table (device, int32, may be NULL; not beside rows): entries that name a source name its destination afterwards. */
+typedef struct {
+  void* base;                     /* page 0, row 0 */
+  int64_t page_stride_bytes, row_stride_bytes, row_bytes;
+} mlahip_page_cache;
+int mlahip_copy_pages(const mlahip_page_cache* caches, int32_t num_caches, const int32_t* src, const int32_t* dst,
+                      const int32_t* rows /* may be NULL */, int32_t num_pairs, int64_t num_pages, int32_t page_size,
+                      int32_t* block_table, int64_t bt_stride, int32_t bt_rows, int32_t bt_cols, mlahip_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

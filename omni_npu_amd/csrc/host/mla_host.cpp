@@ -60,7 +60,7 @@ Stream stream_of(const Tensor& t) { return (Stream)c10::hip::getCurrentHIPStream
 PyObject* g_workspace = nullptr;
 auto& g_scratch = *new std::map<std::tuple<int, Stream, int>, Tensor>;      // (guarded by the GIL, as the Python side is)
 Tensor& scratch(const Tensor& like, Stream stream, int64_t bytes, int tag) {
-  static const char* const names[] = {"decode", "topk", "absorb"};
+  static const char* const names[] = {"decode", "topk", "absorb", "gqa"};
   Tensor& t = g_scratch[{like.get_device(), stream, tag}];
   if (!t.defined() || t.numel() < bytes) t = py::cast<Tensor>(py::handle(g_workspace)(like.device(), bytes, names[tag]));
   return t;
@@ -563,6 +563,139 @@ bool dsa_select_prompts(const Tensor& q, const Tensor& k, const Tensor& weights,
   return true;
 }
 
+// A call that the library refuses (nothing is launched) is the general path's to explain.
+bool done(int rc, const char* what) {
+  if (rc < 0 && rc > -100) return false;
+  check(rc, what);
+  return true;
+}
+// kernels.qk_norm_rope_cache
+int type_code(at::ScalarType t) { return t == at::kBFloat16 ? 0 : t == at::kFloat ? 1 : t == at::kHalf ? 2 : t == at::kFloat8_e4m3fn ? 3 : -1; }
+bool heads_of(const Tensor& x, int64_t t, int64_t h, int64_t d, at::ScalarType dt, const at::Device& dev) {
+  return x.dim() == 3 && x.scalar_type() == dt && x.device() == dev && x.size(0) == t && x.size(1) == h && x.size(2) == d && x.stride(2) == 1;
+}
+bool head_cache(const Tensor& c, int64_t h, int64_t d, at::ScalarType dt, const at::Device& dev) {
+  return c.dim() == 4 && c.device() == dev && (c.scalar_type() == dt || c.scalar_type() == at::kFloat8_e4m3fn) && c.size(0) >= 1 &&
+         c.size(2) == h && c.size(3) == d && c.stride(3) == 1;
+}
+bool head_scale(const OptTensor& s, bool fp8, int64_t h, const at::Device& dev) {
+  return !s || (fp8 && s->scalar_type() == at::kFloat && s->dim() == 1 && s->size(0) == h && s->is_contiguous() && s->device() == dev);
+}
+bool longs(const Tensor& x, int64_t t, const at::Device& dev) {
+  return x.scalar_type() == at::kLong && x.dim() == 1 && x.numel() >= t && (t <= 1 || x.stride(0) == 1) && x.device() == dev;
+}
+bool wants_grad(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t && t->requires_grad()) return true;
+  return false;
+}
+const Tensor* ptr_of(const OptTensor& t) { return t ? &*t : nullptr; }
+void* data_of(const OptTensor& t) { return t ? t->data_ptr() : nullptr; }
+
+bool qk_norm_rope_cache(const Tensor& q, const OptTensor& k, const OptTensor& v, const Tensor& cos, const Tensor& sin, const Tensor& positions,
+                        const OptTensor& slots, const OptTensor& k_cache, const OptTensor& v_cache, const OptTensor& q_gamma,
+                        const OptTensor& k_gamma, double eps, bool interleaved, const OptTensor& q_out, const OptTensor& k_out,
+                        const OptTensor& k_scale, const OptTensor& v_scale) {
+  if (!current_gpu(q) || q.dim() != 3) return false;
+  const at::Device dev = q.device();
+  const at::ScalarType dt = q.scalar_type();
+  const int64_t t = q.size(0), hq = q.size(1), d = q.size(2);
+  if ((dt != at::kBFloat16 && dt != at::kHalf) || q.stride(2) != 1 || !k || k->dim() != 3) return false;
+  const int64_t hk = k->size(1);
+  const bool cached = slots.has_value();
+  if (cached != k_cache.has_value() || cached != v_cache.has_value() || (cached && !v) || !heads_of(*k, t, hk, d, dt, dev) ||
+      (cached && !heads_of(*v, t, hk, d, dt, dev)) || (q_out && !heads_of(*q_out, t, hq, d, dt, dev)) ||
+      (k_out && !heads_of(*k_out, t, hk, d, dt, dev)) || !longs(positions, t, dev) || (cached && !longs(*slots, t, dev)))
+    return false;
+  for (const OptTensor* g : {&q_gamma, &k_gamma})
+    if (*g && ((*g)->scalar_type() != dt || (*g)->dim() != 1 || (*g)->size(0) != d || !(*g)->is_contiguous() || (*g)->device() != dev)) return false;
+  const int table = type_code(cos.scalar_type());
+  if (cos.dim() != 2 || sin.dim() != 2 || cos.sizes() != sin.sizes() || cos.strides() != sin.strides() || cos.scalar_type() != sin.scalar_type() ||
+      (table != 0 && table != 1) || cos.stride(1) != 1 || cos.size(0) < 1 || cos.device() != dev || sin.device() != dev)
+    return false;
+  bool fp8 = false;
+  if (cached) {
+    if (!head_cache(*k_cache, hk, d, dt, dev) || !head_cache(*v_cache, hk, d, dt, dev) || k_cache->sizes() != v_cache->sizes() ||
+        k_cache->scalar_type() != v_cache->scalar_type())
+      return false;
+    fp8 = k_cache->scalar_type() == at::kFloat8_e4m3fn;
+  }
+  if (!head_scale(k_scale, fp8, hk, dev) || !head_scale(v_scale, fp8, hk, dev) || wants_grad({&q, &*k, ptr_of(v), ptr_of(q_gamma), ptr_of(k_gamma)}))
+    return false;
+  const Tensor& qo = q_out ? *q_out : q;
+  const Tensor* ko = k_out ? &*k_out : cached ? nullptr : &*k;
+  const Tensor *kc = cached ? &*k_cache : nullptr, *vc = cached ? &*v_cache : nullptr;
+  return done(mlahip_qk_norm_rope_cache(
+            q.data_ptr(), q.stride(0), q.stride(1), k->data_ptr(), k->stride(0), k->stride(1), cached ? v->data_ptr() : nullptr,
+            cached ? v->stride(0) : 0, cached ? v->stride(1) : 0, t, (int)hq, (int)hk, (int)d, type_code(dt), data_of(q_gamma), data_of(k_gamma),
+            (float)eps, cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.size(0), table, (int)(2 * cos.size(1)), interleaved,
+            (const int64_t*)positions.data_ptr(), (const int64_t*)data_of(slots), kc ? kc->data_ptr() : nullptr, kc ? kc->stride(0) : 0,
+            kc ? kc->stride(1) : 0, kc ? kc->stride(2) : 0, vc ? vc->data_ptr() : nullptr, vc ? vc->stride(0) : 0, vc ? vc->stride(1) : 0,
+            vc ? vc->stride(2) : 0, kc ? (int)kc->size(1) : 1, kc ? kc->size(0) : 1, kc ? type_code(kc->scalar_type()) : 0,
+            (const float*)data_of(k_scale), (const float*)data_of(v_scale), qo.data_ptr(), qo.stride(0), qo.stride(1),
+            ko ? ko->data_ptr() : nullptr, ko ? ko->stride(0) : 0, ko ? ko->stride(1) : 0, stream_of(q)), "mlahip_qk_norm_rope_cache");
+}
+
+// kernels.gqa_chunks
+int gqa_chunks(int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads, int64_t dim, bool fp8, int64_t max_seq_len) {
+  const int64_t rows = q_len * q_heads / kv_heads, waves = dim == 256 && !fp8 ? 4 : 8;
+  int64_t heads = 1;
+  while (heads * 2 <= waves && kv_heads % (heads * 2) == 0) heads *= 2;
+  const int64_t groups = kv_heads / heads * div_up(rows, rows <= 16 ? 16 : 32), units = batch * div_up(max_seq_len, 64);
+  return (int)std::max<int64_t>(1, std::min(256 / groups, units));
+}
+
+// kernels.gqa_decode
+bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& seq_lens, double scale,
+                const Tensor& out, int64_t q_len, const OptTensor& qsl, int64_t window, const OptTensor& k_scale, const OptTensor& v_scale,
+                const OptTensor& lse, int64_t num_chunks, int64_t max_seq_len, const OptTensor& workspace) {
+  if (!current_gpu(q) || q.dim() != 3 || workspace || k_cache.dim() != 4 || num_chunks > (1 << 16)) return false;
+  const at::Device dev = q.device();
+  const at::ScalarType dt = q.scalar_type();
+  const int64_t t = q.size(0), hq = q.size(1), d = q.size(2), hk = k_cache.size(2), b = seq_lens.numel();
+  if ((dt != at::kBFloat16 && dt != at::kHalf) || q.stride(2) != 1 || !heads_of(out, t, hq, d, dt, dev) || hk < 1 || hq < 1 || hq % hk ||
+      !head_cache(k_cache, hk, d, dt, dev) || !head_cache(v_cache, hk, d, dt, dev) || k_cache.sizes() != v_cache.sizes() ||
+      k_cache.scalar_type() != v_cache.scalar_type() || q_len < 1 || window < 0 || !is_i32(seq_lens, 1, dev) || !seq_lens.is_contiguous() ||
+      !is_i32(block_table, 2, dev) || block_table.size(0) < b || block_table.size(1) < 1 || b < 1 ||
+      (qsl ? !(is_i32(*qsl, 1, dev) && qsl->is_contiguous() && qsl->numel() == b + 1) : t != b * q_len) ||
+      (lse && !(lse->scalar_type() == at::kFloat && lse->dim() == 2 && lse->size(0) == t && lse->size(1) == hq && lse->is_contiguous() && lse->device() == dev)))
+    return false;
+  const bool fp8 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
+  if (!head_scale(k_scale, fp8, hk, dev) || !head_scale(v_scale, fp8, hk, dev) || wants_grad({&q, &k_cache, &v_cache})) return false;
+  int64_t longest = block_table.size(1) * k_cache.size(1);
+  if (max_seq_len > 0 && c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) longest = std::min(longest, max_seq_len);
+  if (window > 0) longest = std::min(longest, window + q_len + 62);
+  const int chunks = num_chunks >= 0 ? (int)num_chunks : gqa_chunks(b, q_len, hq, hk, d, fp8, longest);
+  Stream st = stream_of(q);
+  const int64_t need = (int64_t)mlahip_gqa_decode_workspace_bytes((int)b, (int)q_len, (int)hq, (int)d, chunks);
+  Tensor* ws = need ? &scratch(q, st, need, 3) : nullptr;
+  return done(mlahip_gqa_decode(q.data_ptr(), q.stride(0), q.stride(1), t, k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
+                          v_cache.data_ptr(), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2), k_cache.size(0), (int)k_cache.size(1),
+                          (const int32_t*)block_table.data_ptr(), block_table.stride(0), (int)block_table.size(1),
+                          (const int32_t*)seq_lens.data_ptr(), (const int32_t*)data_of(qsl), (int)b, (int)q_len, (int)hq, (int)hk, (int)d,
+                          type_code(dt), type_code(k_cache.scalar_type()), (const float*)data_of(k_scale), (const float*)data_of(v_scale),
+                          (float)scale, (int)window, out.data_ptr(), out.stride(0), out.stride(1), (float*)data_of(lse),
+                          ws ? ws->data_ptr() : nullptr, ws ? (size_t)ws->numel() : 0, chunks, st), "mlahip_gqa_decode");
+}
+
+// The launch of kernels.copy_pages, which has checked the tensors and the pairs: the library's code.
+int copy_pages(const std::vector<Tensor>& caches, const std::vector<int32_t>& src, const std::vector<int32_t>& dst,
+                const std::optional<std::vector<int32_t>>& rows, const OptTensor& table) {
+  std::vector<mlahip_page_cache> list;
+  list.reserve(caches.size());
+  for (const Tensor& c : caches) {
+    const int64_t es = c.element_size(), row = c.numel() / (c.size(0) * c.size(1)) * es;
+    // (the stride of a dim of one entry says nothing)
+    const int64_t row_stride = c.size(1) > 1 ? c.stride(1) * es : row, page_stride = c.size(0) > 1 ? c.stride(0) * es : row_stride * c.size(1);
+    list.push_back({c.data_ptr(), page_stride, row_stride, row});
+  }
+  return mlahip_copy_pages(list.data(), (int)list.size(), src.data(), dst.data(), rows ? rows->data() : nullptr, (int)src.size(), caches[0].size(0),
+                          (int)caches[0].size(1), table ? (int32_t*)table->data_ptr() : nullptr,
+                          table ? (table->size(0) > 1 ? table->stride(0) : table->size(1)) : 0, table ? (int)table->size(0) : 0,
+                          table ? (int)table->size(1) : 0, stream_of(caches[0]));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -575,8 +708,12 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("norm_rope_cache", &norm_rope_cache);
   m.def("prefill", &prefill);
   m.def("dsa_select_prompts", &dsa_select_prompts);
+  m.def("qk_norm_rope_cache", &qk_norm_rope_cache);
+  m.def("gqa_decode", &gqa_decode);
+  m.def("copy_pages", &copy_pages);
   // (what this file has a copy of, for a test to hold against kernels.py)
   m.def("launch_splits", &launch_splits, py::arg("batch"), py::arg("q_len"), py::arg("heads"), py::arg("max_seq_len"), py::arg("full") = false);
+  m.def("gqa_chunks", &gqa_chunks);
   m.def("prefill_long_rows", &prefill_long_rows);
   m.def("prefill_blocks", &prefill_blocks);
   m.def("prefill_pieces", &prefill_pieces);

@@ -1374,3 +1374,240 @@ def quant_rows_fp8(x: torch.Tensor, out8: torch.Tensor, out_scale: torch.Tensor,
         rc = lib.dsa_quant_rows_fp8(x2.data_ptr(), x2.stride(0), n, slot_mapping.data_ptr(), out8.data_ptr(), out8.stride(0),
                                     out8.stride(1), sc.data_ptr(), sc.stride(0), out8.shape[1], out8.shape[0], _stream(x))
     _lib.check(rc, "dsa_quant_rows_fp8")
+
+
+# ------------------------------------------------------------------------------------------------
+# Layers with ordinary key and value heads: the step in front of the attention, the attention over the paged cache, and the pages
+# of any cache.
+
+_HEAD_DT = {torch.bfloat16: 0, torch.float16: 2}
+_E4M3 = 3
+
+
+def _one_device(what: str, *ts) -> torch.device:
+    _need_cuda(*ts)
+    dev = next(t.device for t in ts if t is not None)
+    if any(t is not None and t.device != dev for t in ts):
+        raise ValueError(f"{what}: tensors on different devices: {sorted({str(t.device) for t in ts if t is not None})}")
+    return dev
+
+
+def _no_grad(what: str, *ts) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() or with detached tensors")
+
+
+def _head_cache(what: str, name: str, c: torch.Tensor, kv_heads: int, dim: int, dtype: torch.dtype) -> int:
+    """The type code of a cache [pages, page, kv_heads, dim] of ``dtype`` or e4m3."""
+    if c.dim() != 4 or c.shape[2:] != (kv_heads, dim) or c.stride(3) != 1 or c.shape[0] < 1:
+        raise ValueError(f"{what}: {name} must be [pages, page, {kv_heads}, {dim}] with a contiguous last dim, got {tuple(c.shape)}")
+    if c.dtype == torch.float8_e4m3fn:
+        return _E4M3
+    if c.dtype != dtype:
+        raise TypeError(f"{what}: {name} must be {dtype} like the queries, or float8_e4m3fn, got {c.dtype}")
+    return _HEAD_DT[dtype]
+
+
+def _head_scales(what: str, fp8: bool, kv_heads: int, **scales) -> list:
+    for name, s in scales.items():
+        if s is not None and not fp8:
+            raise ValueError(f"{what}: {name} goes with a float8_e4m3fn cache")
+        if s is not None and (s.dtype != torch.float32 or s.shape != (kv_heads,) or not s.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be a contiguous fp32 [{kv_heads}] vector")
+    return [s.data_ptr() if s is not None else None for s in scales.values()]
+
+
+def qk_norm_rope_cache(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor,
+                       positions: torch.Tensor, slot_mapping: Optional[torch.Tensor] = None,
+                       k_cache: Optional[torch.Tensor] = None, v_cache: Optional[torch.Tensor] = None, *,
+                       q_gamma: Optional[torch.Tensor] = None, k_gamma: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                       interleaved: bool = False, q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None,
+                       k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None) -> None:
+    """Per-head RMSNorm, rotary positions and the cache write of a layer with ordinary key and value heads, in one launch.
+
+    q [T,Hq,D], k and v [T,Hk,D] bf16 or fp16 (any token / head strides of 16-byte multiples, so views of the projection's
+    result; D and the rotated width multiples of 16 up to 256); ``cos`` / ``sin`` fp32 or bf16 [positions, R/2], R <= D the
+    rotated width, indexed by ``positions`` int64 [T]; pairs (i, i+R/2), or with ``interleaved`` (2i, 2i+1), results laid out as
+    the inputs.  ``q_gamma`` / ``k_gamma`` [D]: RMSNorm of every query / key head in front of the rotation.  Everything in fp32,
+    rounded once.  Queries go to ``q_out`` (default: in place).  With ``slot_mapping`` int64 [T] keys and values go to row
+    slot_mapping[t] of ``k_cache`` / ``v_cache`` [pages, page, Hk, D] of the inputs' type or float8_e4m3fn (x / k_scale[h],
+    x / v_scale[h], fp32 [Hk], saturated); negative slots and slots past the cache are skipped.  Rotated keys go to ``k_out`` too
+    where it is given (default without a cache: in place); ``k=None`` rotates queries alone.  A token whose position is not in
+    the tables is not written anywhere."""
+    what = "qk_norm_rope_cache"
+    if _host.load().qk_norm_rope_cache(q, k, v, cos, sin, positions, slot_mapping, k_cache, v_cache, q_gamma, k_gamma, eps, interleaved,
+                                       q_out, k_out, k_scale, v_scale):
+        return
+    dev = _one_device(what, q, k, v, cos, sin, positions, slot_mapping, k_cache, v_cache, q_gamma, k_gamma, q_out, k_out, k_scale, v_scale)
+    _no_grad(what, q, k, v, q_gamma, k_gamma)
+    cached = slot_mapping is not None
+    if cached != (k_cache is not None) or cached != (v_cache is not None) or cached and (k is None or v is None):
+        raise ValueError(f"{what}: a cache write takes k, v, slot_mapping, k_cache and v_cache together")
+    if q.dim() != 3 or q.dtype not in _HEAD_DT or q.stride(2) != 1:
+        raise ValueError(f"{what}: q must be bf16 or fp16 [T, Hq, D] with a contiguous last dim, got {q.dtype} {tuple(q.shape)}")
+    t, hq, d = q.shape
+    hk = 0 if k is None else k.shape[1]
+    q_out = q if q_out is None else q_out
+    if k_out is None and k is not None and not cached:
+        k_out = k
+    if k is None and (k_out is not None or k_gamma is not None):
+        raise ValueError(f"{what}: k_out and k_gamma go with k")
+    for name, x, h in (("k", k, hk), ("v", v if cached else None, hk), ("q_out", q_out, hq), ("k_out", k_out, hk)):
+        if x is not None and (x.shape != (t, h, d) or x.dtype != q.dtype or x.stride(2) != 1):
+            raise ValueError(f"{what}: {name} must be {q.dtype} [{t}, {h}, {d}] with a contiguous last dim, got {x.dtype} {tuple(x.shape)}")
+    for name, x in (("q_gamma", q_gamma), ("k_gamma", k_gamma)):
+        if x is not None and (x.shape != (d,) or x.dtype != q.dtype or not x.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be a contiguous {q.dtype} [{d}] vector")
+    if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.dtype not in _DT or cos.stride() != sin.stride() or \
+            cos.stride(1) != 1 or cos.shape[0] < 1:
+        raise ValueError(f"{what}: cos / sin must be fp32 or bf16 [positions, R/2] rows with equal strides, got {tuple(cos.shape)} {cos.dtype}")
+    for name, x in (("positions", positions), ("slot_mapping", slot_mapping)):
+        if x is not None and (x.dtype != torch.int64 or x.dim() != 1 or x.numel() < t or x.stride(0) != 1 and t > 1):
+            raise ValueError(f"{what}: {name} must be contiguous int64 [{t}]")
+    cache_args, cache_code, scales = (None, 0, 0, 0, None, 0, 0, 0, 1, 1), 0, (None, None)
+    if cached:
+        cache_code = _head_cache(what, "k_cache", k_cache, hk, d, q.dtype)
+        if _head_cache(what, "v_cache", v_cache, hk, d, q.dtype) != cache_code or k_cache.shape != v_cache.shape:
+            raise ValueError(f"{what}: k_cache and v_cache must agree in shape and type")
+        scales = _head_scales(what, cache_code == _E4M3, hk, k_scale=k_scale, v_scale=v_scale)
+        cache_args = (k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(), *v_cache.stride()[:3], k_cache.shape[1], k_cache.shape[0])
+    elif k_scale is not None or v_scale is not None:
+        raise ValueError(f"{what}: scales go with a float8_e4m3fn cache")
+    row = lambda x: (x.data_ptr(), x.stride(0), x.stride(1)) if x is not None else (None, 0, 0)
+    ptr = lambda x: x.data_ptr() if x is not None else None
+    with torch.cuda.device(dev):
+        rc = _lib.load().mlahip_qk_norm_rope_cache(
+            *row(q), *row(k), *row(v if cached else None), t, hq, hk, d, _HEAD_DT[q.dtype], ptr(q_gamma), ptr(k_gamma), float(eps),
+            cos.data_ptr(), sin.data_ptr(), cos.stride(0), cos.shape[0], _DT[cos.dtype], 2 * cos.shape[1], int(interleaved),
+            positions.data_ptr(), ptr(slot_mapping), *cache_args, cache_code, *scales, *row(q_out), *row(k_out), _stream(q))
+    _lib.check(rc, "mlahip_qk_norm_rope_cache")
+
+
+def gqa_chunks(batch: int, q_len: int, q_heads: int, kv_heads: int, dim: int, fp8: bool, max_seq_len: int, num_cus: int = 256) -> int:
+    """Pieces that gqa_decode cuts the cached keys of a step into (0: a request to a workgroup, one launch)."""
+    rows = q_len * q_heads // kv_heads
+    waves = 4 if dim == 256 and not fp8 else 8
+    heads = 1
+    while heads * 2 <= waves and kv_heads % (heads * 2) == 0:
+        heads *= 2
+    groups = kv_heads // heads * math.ceil(rows / (16 if rows <= 16 else 32))
+    units = batch * math.ceil(max_seq_len / 64)
+    return max(1, min(num_cus // groups, units))
+
+
+def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+               scale: float, out: torch.Tensor, q_len: int = 1, query_start_loc: Optional[torch.Tensor] = None,
+               window: Optional[int] = None, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+               lse_out: Optional[torch.Tensor] = None, num_chunks: Optional[int] = None, max_seq_len: Optional[int] = None,
+               workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of each request's newest tokens over a paged cache of ordinary key and value heads.
+
+    q [T,Hq,D] bf16 or fp16, D 64, 128 or 256; caches [pages, page, Hk, D] of its type or float8_e4m3fn (times ``k_scale`` /
+    ``v_scale`` fp32 [Hk]), page a multiple of 16, any page / row / head strides of 16-byte multiples; query head h reads key head
+    h // (Hq // Hk).  block_table int32 [B,maxblk], seq_lens int32 [B] on the device, the newest tokens included.  Sequence b owns
+    query tokens [b*q_len, (b+1)*q_len), or with query_start_loc (int32 [B+1], device) those, at most q_len of them; token i of s
+    sees keys [0, L - s + i], with ``window`` only the newest ``window`` of these.  ``out`` [T,Hq,D] like q; ``lse_out`` fp32
+    [T,Hq].  A row without keys gives zeros and -inf.  ``max_seq_len``: no request is longer (it shapes the launch; results are right
+    without); under capture the table's room counts, as a graph is replayed over others."""
+    what = "gqa_decode"
+    if _host.load().gqa_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out, q_len, query_start_loc,
+                               0 if window is None else window or -1, k_scale, v_scale, lse_out,
+                               -1 if num_chunks is None else num_chunks, max_seq_len or 0, workspace):
+        return out
+    dev = _one_device(what, q, k_cache, v_cache, block_table, seq_lens, out, query_start_loc, k_scale, v_scale, lse_out, workspace)
+    _no_grad(what, q, k_cache, v_cache)
+    if q.dim() != 3 or q.dtype not in _HEAD_DT or q.stride(2) != 1 or out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
+        raise ValueError(f"{what}: q and out must be bf16 or fp16 [T, Hq, D] with contiguous last dims, got {q.dtype} {tuple(q.shape)}, "
+                         f"{out.dtype} {tuple(out.shape)}")
+    t, hq, d = q.shape
+    if k_cache.dim() != 4:
+        raise ValueError(f"{what}: k_cache must be [pages, page, Hk, {d}], got {tuple(k_cache.shape)}")
+    hk = k_cache.shape[2]
+    code = _head_cache(what, "k_cache", k_cache, hk, d, q.dtype)
+    if _head_cache(what, "v_cache", v_cache, hk, d, q.dtype) != code or k_cache.shape != v_cache.shape:
+        raise ValueError(f"{what}: k_cache and v_cache must agree in shape and type")
+    if hk < 1 or hq % hk:
+        raise ValueError(f"{what}: {hq} query heads over {hk} key heads")
+    if window is not None and window < 1:
+        raise ValueError(f"{what}: a window of {window} keys")
+    if q_len < 1:
+        raise ValueError(f"{what}: q_len {q_len}")
+    b = seq_lens.numel()
+    if seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous() or block_table.dtype != torch.int32 or block_table.dim() != 2 or \
+            block_table.shape[0] < b or block_table.shape[1] < 1 or block_table.stride(1) != 1 and block_table.shape[1] > 1:
+        raise ValueError(f"{what}: seq_lens must be contiguous int32 [B] and block_table int32 [>= B, blocks] with contiguous rows")
+    if query_start_loc is None:
+        if t != b * q_len:
+            raise ValueError(f"{what}: {t} query tokens for {b} requests of {q_len}")
+    elif query_start_loc.dtype != torch.int32 or query_start_loc.numel() != b + 1 or not query_start_loc.is_contiguous():
+        raise ValueError(f"{what}: query_start_loc must be contiguous int32 [{b + 1}]")
+    if lse_out is not None and (lse_out.dtype != torch.float32 or lse_out.shape != (t, hq) or not lse_out.is_contiguous()):
+        raise ValueError(f"{what}: lse_out must be contiguous fp32 [{t}, {hq}]")
+    scales = _head_scales(what, code == _E4M3, hk, k_scale=k_scale, v_scale=v_scale)
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        longest = block_table.shape[1] * k_cache.shape[1]
+        if max_seq_len and not torch.cuda.is_current_stream_capturing():
+            longest = min(longest, max_seq_len)
+        if window is not None:
+            longest = min(longest, window + q_len + 62)
+        if num_chunks is None:
+            num_chunks = gqa_chunks(b, q_len, hq, hk, d, code == _E4M3, longest)
+        need = lib.mlahip_gqa_decode_workspace_bytes(b, q_len, hq, d, num_chunks)
+        ws = workspace
+        if ws is None and need:
+            ws = _workspace(dev, need, "gqa")
+        rc = lib.mlahip_gqa_decode(
+            q.data_ptr(), q.stride(0), q.stride(1), t, k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(), *v_cache.stride()[:3],
+            k_cache.shape[0], k_cache.shape[1], block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
+            query_start_loc.data_ptr() if query_start_loc is not None else None, b, q_len, hq, hk, d, _HEAD_DT[q.dtype], code, *scales,
+            float(scale), window or 0, out.data_ptr(), out.stride(0), out.stride(1), lse_out.data_ptr() if lse_out is not None else None,
+            ws.data_ptr() if ws is not None else None, ws.numel() * ws.element_size() if ws is not None else 0, num_chunks, _stream(q))
+    _lib.check(rc, "mlahip_gqa_decode")
+    return out
+
+
+def copy_pages(caches, src, dst, rows=None, block_table: Optional[torch.Tensor] = None) -> None:
+    """cache[dst[i], :n] = cache[src[i], :n] for every pair i and every cache of the list (all layers', of any kind: [pages, page, ...]
+    with contiguous rows of any type), n = rows[i] or the whole page: copies, and forks with the filled rows of a last page.
+
+    ``src``, ``dst`` and ``rows`` are host values (lists, or CPU tensors): the scheduler has them there, and they are checked
+    before anything is launched.  A destination may be named once and not be a source of the same call.  With ``block_table`` (int32
+    [requests, blocks] on the device) the pages move: entries that name a source name its destination afterwards.  In a captured graph
+    the pairs are those of the capture."""
+    what = "copy_pages"
+    as_list = lambda x: x.tolist() if torch.is_tensor(x) else list(x)
+    if any(torch.is_tensor(x) and x.is_cuda for x in (src, dst, rows)):
+        raise ValueError(f"{what}: src, dst and rows are read on the host: lists or CPU tensors")
+    caches = [caches] if torch.is_tensor(caches) else list(caches)
+    src, dst, rows = as_list(src), as_list(dst), None if rows is None else as_list(rows)
+    if any(isinstance(i, bool) or not isinstance(i, int) for x in (src, dst, rows or ()) for i in x):
+        raise TypeError(f"{what}: page numbers and rows are whole numbers")
+    if not caches or len(src) != len(dst) or rows is not None and len(rows) != len(src):
+        raise ValueError(f"{what}: {len(caches)} caches, {len(src)} sources, {len(dst)} destinations"
+                         + (f", {len(rows)} row counts" if rows is not None else ""))
+    dev = _one_device(what, *caches, block_table)
+    _no_grad(what, *caches)
+    pages, page = caches[0].shape[:2] if caches[0].dim() >= 2 else (0, 0)
+    for c in caches:
+        if c.dim() < 2 or c.shape[:2] != (pages, page) or pages < 1 or page < 1 or c[0, 0].numel() < 1 or not c[0, 0].is_contiguous():
+            raise ValueError(f"{what}: caches must be [pages, page, ...] of the same pages with contiguous rows, got {tuple(c.shape)}")
+        if c.stride(0) < 1 and pages > 1 or c.stride(1) < 1 and page > 1:
+            raise ValueError(f"{what}: a cache whose pages or rows share memory")
+    for i, (a, z) in enumerate(zip(src, dst)):
+        if not (0 <= a < pages and 0 <= z < pages):
+            raise ValueError(f"{what}: pair {i} copies page {a} to {z} of {pages}")
+        if rows is not None and not 0 <= rows[i] <= page:
+            raise ValueError(f"{what}: pair {i} copies {rows[i]} rows of {page}")
+    if len(set(dst)) != len(dst) or set(src) & set(dst):
+        raise ValueError(f"{what}: a page is the destination of two pairs, or a source and a destination")
+    if block_table is not None:
+        if rows is not None:
+            raise ValueError(f"{what}: a moved page is moved whole: no rows beside a block table")
+        if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 and block_table.shape[1] > 1 or \
+                block_table.stride(0) < block_table.shape[1] and block_table.shape[0] > 1:
+            raise ValueError(f"{what}: block_table must be int32 [requests, blocks] with contiguous rows")
+    if not src:
+        return
+    with torch.cuda.device(dev):
+        _lib.check(_host.load().copy_pages(caches, src, dst, rows, block_table), "mlahip_copy_pages")
