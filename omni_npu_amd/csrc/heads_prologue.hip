@@ -8,9 +8,11 @@
 // in fp32 from the 16-bit inputs, rounded once: to the inputs' type, or for an 8-bit cache x / scale[head] to e4m3 (values beyond
 // +-448 become +-448, NaN stays NaN).
 //
-// A group of 8, 16 or 32 lanes holds a head, eight values a lane; the norm's sum and a half pair's other element come by lane moves.
-// A group takes several heads of one token, so that the token's table entries are read once (a lane's entries are four times its
-// values' bytes).  What bounds it is memory: every value is read and written once.
+// A group of 8, 16 or 32 lanes holds a head, four pairs a lane (of half pairs its values are four in either half, so that both of a pair
+// are the lane's own); the norm's sum goes by lane moves.  A group takes several heads of one token, so that the token's table entries
+// and the gains are read once.  What bounds it is memory: every value is read and written once.
+#include <type_traits>
+
 #include "cache_rows.hpp"
 
 namespace mlahip {
@@ -30,138 +32,144 @@ struct PrologueParams {
   float eps;
 };
 
-template <typename T> struct Vec8 { typedef T type __attribute__((ext_vector_type(8))); };
+template <typename T> struct Vec4 { typedef T type __attribute__((ext_vector_type(4))); };
 
-// eight entries of a table from entry i on
-__device__ __forceinline__ void entries(const char* row, int i, bool f32, float* e) {
-  if (f32) {
-    const f32x4 a = *(const f32x4*)(row + i * 4), b = *(const f32x4*)(row + i * 4 + 16);
-#pragma unroll
-    for (int j = 0; j < 4; j++) { e[j] = a[j]; e[4 + j] = b[j]; }
-  } else {
-    const bf16x8 a = *(const bf16x8*)(row + i * 2);
-#pragma unroll
-    for (int j = 0; j < 8; j++) e[j] = (float)a[j];
-  }
+// four entries of a table from entry i on
+__device__ __forceinline__ f32x4 entries(const char* row, int i, bool f32) {
+  if (f32) return *(const f32x4*)(row + i * 4);
+  const bf16x4 a = *(const bf16x4*)(row + i * 2);
+  return f32x4{(float)a[0], (float)a[1], (float)a[2], (float)a[3]};
 }
-__device__ __forceinline__ void entries4(const char* row, int i, bool f32, float* e) {
-  if (f32) {
-    const f32x4 a = *(const f32x4*)(row + i * 4);
-#pragma unroll
-    for (int j = 0; j < 4; j++) e[j] = a[j];
-  } else {
-    const bf16x4 a = *(const bf16x4*)(row + i * 2);
-#pragma unroll
-    for (int j = 0; j < 4; j++) e[j] = (float)a[j];
-  }
+
+// Sum over the 8, 16 or 32 lanes of a head: within rows of 16 by data-parallel-primitive moves.
+template <int kLanes> __device__ __forceinline__ float lanes_sum(float x) {
+  auto add = [&](auto ctrl) { x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(ctrl)::value, 0xf, 0xf, true)); };
+  add(std::integral_constant<int, 0xB1>{});                  // the neighbour, the pair beside, the other half row mirrored,
+  add(std::integral_constant<int, 0x4E>{});
+  add(std::integral_constant<int, 0x141>{});
+  if constexpr (kLanes >= 16) add(std::integral_constant<int, 0x140>{});   // the row mirrored
+  if constexpr (kLanes >= 32) x += __shfl_xor(x, 16, 64);
+  return x;
 }
 
 // x / s to e4m3, saturated: the quotient by the reciprocal and one correction by the remainder (a division is ten instructions a value)
-__device__ __forceinline__ u32x2 to_e4m3(const float* x, float s) {
-  const float inv = 1.f / s;
-  float y[8];
+__device__ __forceinline__ uint32_t to_e4m3(const float* x, float s, float inv) {
+  float y[4];
 #pragma unroll
-  for (int e = 0; e < 8; e++) {
-    float v = x[e] * inv;
-    const float r = __builtin_fmaf(-v, s, x[e]);
-    const float w = __builtin_fmaf(r, inv, v);
-    v = __builtin_isfinite(v) ? w : v;
-    y[e] = v != v ? v : fminf(fmaxf(v, -448.f), 448.f);
+  for (int e = 0; e < 4; e++) {
+    const float v = x[e] * inv, w = __builtin_fmaf(__builtin_fmaf(-v, s, x[e]), inv, v);
+    y[e] = __builtin_isinf(v) ? v : w;                       // (no remainder of an infinity)
+    y[e] = y[e] != y[e] ? y[e] : fminf(fmaxf(y[e], -448.f), 448.f);
   }
-  int w0 = 0, w1 = 0;
-  w0 = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], w0, false);
-  w0 = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w0, true);
-  w1 = __builtin_amdgcn_cvt_pk_fp8_f32(y[4], y[5], w1, false);
-  w1 = __builtin_amdgcn_cvt_pk_fp8_f32(y[6], y[7], w1, true);
-  return u32x2{(uint32_t)w0, (uint32_t)w1};
+  int w = 0;
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], w, false);
+  w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+  return (uint32_t)w;
 }
 
 // T: the inputs' type; kLanes: lanes of a head; kFp8: an 8-bit cache; kPairs: interleaved pairs
 template <typename T, int kLanes, bool kFp8, bool kPairs>
 __global__ __launch_bounds__(256) void heads_prologue_kernel(const PrologueParams p) {
-  typedef typename Vec8<T>::type V8;
-  const int lane = threadIdx.x & 63, j = lane & (kLanes - 1);
+  typedef typename Vec4<T>::type V4;
+  struct Eight { V4 a, b; };
+  const int j = threadIdx.x & (kLanes - 1);
   const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kLanes;
-  const int64_t t = group / p.parts;
-  const int part = (int)(group - t * p.parts);
+  const uint32_t t32 = (uint32_t)group / (uint32_t)p.parts;  // (host: fewer than 2^32 groups)
+  const int64_t t = t32;
+  const int part = (int)((uint32_t)group - t32 * (uint32_t)p.parts);
   if (t >= p.num_tokens) return;
   const int64_t pos = p.positions[t];
-  if (pos < 0 || pos >= p.table_rows) return;                // a position that the tables do not have: nothing is written
   const int64_t slot = p.slots ? p.slots[t] : -1;
+  if (pos < 0 || pos >= p.table_rows) return;                // a position that the tables do not have: nothing is written
   const bool store = p.cache[0] && slot >= 0 && slot < p.num_pages * p.page_size;
   const SlotAt at = slot_at(store ? slot : 0, store ? p.page_size : 1);
   const bool mine = j * 8 < p.dim;                           // (heads of fewer values than the group has room for)
-  const int r = p.rotary, half_lanes = r >> 4;
-  const bool turns = j * 8 < r;
-  const bool first = j < half_lanes;
-  float c[8], s[8];
-#pragma unroll
-  for (int e = 0; e < 8; e++) { c[e] = 1.f; s[e] = 0.f; }
+  // A lane's eight values are two fours at a and b.  A lane that turns half pairs has four pairs: 4j .. of the rotated part's first
+  // half and 4j .. of its second.  Lanes that do not exist in the head repeat its lane 0.
+  const bool turns = j * 8 < p.rotary;
+  const int a0 = !mine ? 0 : !kPairs && turns ? j * 4 : j * 8, b0 = !kPairs && turns && mine ? j * 4 + p.rotary / 2 : a0 + 4;
+  f32x4 c{}, s{};
   if (turns) {
-    if constexpr (kPairs) {
-      entries4(p.cos + pos * p.cs_st, j * 4, p.table_f32, c);
-      entries4(p.sin + pos * p.cs_st, j * 4, p.table_f32, s);
+    c = entries(p.cos + pos * p.cs_st, j * 4, p.table_f32);
+    s = entries(p.sin + pos * p.cs_st, j * 4, p.table_f32);
+  }
+  auto load = [&](const char* at) { return Eight{*(const V4*)(at + a0 * 2), *(const V4*)(at + b0 * 2)}; };
+  auto store8 = [&](char* at, const float* x) {
+    Eight y;
+#pragma unroll
+    for (int e = 0; e < 4; e++) { y.a[e] = (T)x[e]; y.b[e] = (T)x[4 + e]; }
+    *(V4*)(at + a0 * 2) = y.a;
+    *(V4*)(at + b0 * 2) = y.b;
+  };
+  auto store_cache = [&](int i, int h, const float* x) {
+    char* dst = p.cache[i] + at.pg * p.c_sp[i] + at.off * p.c_sr[i] + h * p.c_sh[i];
+    if constexpr (kFp8) {
+      const float sc = p.scale[i] ? p.scale[i][h] : 1.f, inv = 1.f / sc;
+      *(uint32_t*)(dst + a0) = to_e4m3(x, sc, inv);
+      *(uint32_t*)(dst + b0) = to_e4m3(x + 4, sc, inv);
     } else {
-      entries(p.cos + pos * p.cs_st, (first ? j : j - half_lanes) * 8, p.table_f32, c);
-      entries(p.sin + pos * p.cs_st, (first ? j : j - half_lanes) * 8, p.table_f32, s);
+      store8(dst, x);
+    }
+  };
+  const float inv_dim = 1.f / (float)p.dim;
+  auto turned = [&](const Eight& raw, const char* gamma, const Eight& g, float* x) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) { x[e] = (float)raw.a[e]; x[4 + e] = (float)raw.b[e]; }
+    if (gamma) {
+      float sum = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; e++) sum += x[e] * x[e];
+      const float inv = __builtin_amdgcn_rsqf(lanes_sum<kLanes>(mine ? sum : 0.f) * inv_dim + p.eps);
+#pragma unroll
+      for (int e = 0; e < 4; e++) { x[e] *= inv * (float)g.a[e]; x[4 + e] *= inv * (float)g.b[e]; }
+    }
+    if (!turns) return;                                      // (1 x + 0 y would not be x beside an infinity)
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      float &u = kPairs ? x[2 * e] : x[e], &v = kPairs ? x[2 * e + 1] : x[4 + e];
+      const float u0 = u, v0 = v;
+      u = u0 * c[e] - v0 * s[e];
+      v = v0 * c[e] + u0 * s[e];
+    }
+  };
+  // The token's heads in a row: queries, keys, values; this group takes every parts-th of them, the next one's values asked for ahead.
+  int head = part;
+  {
+    const char *gamma = p.gamma[0], *src = p.src[0] + t * p.src_st[0];
+    char* out = p.out[0] + t * p.out_st[0];
+    Eight g{}, next{};
+    if (gamma && head < p.q_heads) g = load(gamma);
+    if (head < p.q_heads) next = load(src + head * p.src_sh[0]);
+    for (; head < p.q_heads; head += p.parts) {
+      const Eight raw = next;
+      if (head + p.parts < p.q_heads) next = load(src + (head + p.parts) * p.src_sh[0]);
+      float x[8];
+      turned(raw, gamma, g, x);
+      if (mine) store8(out + head * p.out_sh[0], x);
     }
   }
-  const int other = (lane & ~(kLanes - 1)) + (first ? j + half_lanes : j - half_lanes);
-  const int heads = p.q_heads + (p.cache[0] || p.out[1] ? p.kv_heads : 0) + (p.cache[0] ? p.kv_heads : 0);
-  for (int head = part; head < heads; head += p.parts) {
-    const int what = head < p.q_heads ? 0 : head < p.q_heads + p.kv_heads ? 1 : 2;
-    const int h = head - (what == 0 ? 0 : what == 1 ? p.q_heads : p.q_heads + p.kv_heads);
-    if (what > 0 && !store && !(what == 1 && p.out[1])) continue;
-    V8 raw;
-#pragma unroll
-    for (int e = 0; e < 8; e++) raw[e] = (T)0.f;
-    if (mine) raw = *(const V8*)(p.src[what] + t * p.src_st[what] + h * p.src_sh[what] + j * 16);
+  const int keys = p.q_heads + (store || p.out[1] ? p.kv_heads : 0);
+  if (head < keys) {
+    const char *gamma = p.gamma[1], *src = p.src[1] + t * p.src_st[1];
+    Eight g{};
+    if (gamma) g = load(gamma);
+    for (; head < keys; head += p.parts) {
+      const int h = head - p.q_heads;
+      float x[8];
+      turned(load(src + h * p.src_sh[1]), gamma, g, x);
+      if (!mine) continue;
+      if (p.out[1]) store8(p.out[1] + t * p.out_st[1] + h * p.out_sh[1], x);
+      if (store) store_cache(0, h, x);
+    }
+  }
+  if (!store) return;
+  for (; head < keys + p.kv_heads; head += p.parts) {
+    const int h = head - keys;
+    const Eight raw = load(p.src[2] + t * p.src_st[2] + h * p.src_sh[2]);
     float x[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = (float)raw[e];
-    if (what < 2) {
-      if (p.gamma[what]) {
-        float sum = 0.f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) sum += x[e] * x[e];
-#pragma unroll
-        for (int o = 1; o < kLanes; o <<= 1) sum += __shfl_xor(sum, o, 64);
-        const float inv = 1.f / sqrtf(sum / (float)p.dim + p.eps);
-        V8 g;
-#pragma unroll
-        for (int e = 0; e < 8; e++) g[e] = (T)0.f;
-        if (mine) g = *(const V8*)(p.gamma[what] + j * 16);
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = x[e] * inv * (float)g[e];
-      }
-      if constexpr (kPairs) {
-        if (turns) {
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const float a = x[2 * e], b = x[2 * e + 1];
-            x[2 * e] = a * c[e] - b * s[e];
-            x[2 * e + 1] = b * c[e] + a * s[e];
-          }
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const float y = __shfl(x[e], other, 64);
-          if (turns) x[e] = first ? x[e] * c[e] - y * s[e] : x[e] * c[e] + y * s[e];
-        }
-      }
-    }
-    V8 y;
-#pragma unroll
-    for (int e = 0; e < 8; e++) y[e] = (T)x[e];
-    if (!mine) continue;
-    if (what < 2 && p.out[what]) *(V8*)(p.out[what] + t * p.out_st[what] + h * p.out_sh[what] + j * 16) = y;
-    if (what > 0 && store) {
-      const int i = what - 1;
-      char* dst = p.cache[i] + at.pg * p.c_sp[i] + at.off * p.c_sr[i] + h * p.c_sh[i];
-      if constexpr (kFp8) *(u32x2*)(dst + j * 8) = to_e4m3(x, p.scale[i] ? p.scale[i][h] : 1.f);
-      else *(V8*)(dst + j * 16) = y;
-    }
+    for (int e = 0; e < 4; e++) { x[e] = (float)raw.a[e]; x[4 + e] = (float)raw.b[e]; }
+    if (mine) store_cache(1, h, x);
   }
 }
 
@@ -232,7 +240,7 @@ extern "C" int mlahip_qk_norm_rope_cache(
   parts = parts < per_wave ? per_wave : parts;
   p.parts = (int)(parts < total ? parts : total);
   const int64_t blocks = (num_tokens * p.parts * lanes + 255) / 256;
-  MLA_REQUIRE(blocks < (1ll << 31), MLA_ERR_SHAPE, "%s: too many tokens for one launch", me);
+  MLA_REQUIRE(num_tokens * p.parts < (1ll << 32) && blocks < (1ll << 31), MLA_ERR_SHAPE, "%s: too many tokens for one launch", me);
 #define HEADS_LAUNCH(L)                                                                  \
   if (dtype == 0) heads::launch<__bf16, L>(p, fp8, interleaved != 0, (unsigned)blocks, stream); \
   else heads::launch<_Float16, L>(p, fp8, interleaved != 0, (unsigned)blocks, stream)

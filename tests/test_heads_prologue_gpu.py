@@ -161,6 +161,18 @@ def test_not_a_number_and_infinities(dev, fp8):
     assert torch.isnan(k2[0]).nonzero().flatten().tolist() == [5, 37]   # the pair
 
 
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_an_infinity_stays_where_it_is(dev, interleaved):
+    """Behind the rotated part, and in a pair of its own: no other value of the head changes."""
+    c = make(4, 2, 2, 128, 32, seed=8, norm=False)
+    ref, _, _ = run(dev, c, interleaved)
+    c["qkv"][1, 40], c["qkv"][2, 128 + 127], c["qkv"][3, 4] = float("inf"), float("nan"), float("inf")
+    got, _, _ = run(dev, c, interleaved)
+    changed = (got != ref).nonzero().tolist()
+    pair = [4, 5] if interleaved else [4, 20]
+    assert changed == [[1, 0, 40], [2, 1, 127], [3, 0, pair[0]], [3, 0, pair[1]]]
+
+
 def test_head_major_and_side_by_side_caches(dev):
     from omni_npu_amd import kernels as K
     c = make(21, 4, 2, 128, 128, seed=6)
