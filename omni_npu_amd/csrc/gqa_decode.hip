@@ -6,7 +6,8 @@
 //
 // What bounds it is the cache stream: 4 D bytes of a 16-bit cache per key and head against 4 D G multiply-adds, which the matrix
 // cores do with most of their rows empty.  So the cache goes from memory straight into LDS (no registers held while it is under
-// way), every wavefront has its own ring there, and wavefronts do not wait for each other until a piece of a sequence ends.
+// way), every wavefront has its own ring there (two tiles; the
+// waits count copies, so that the next tile's stay under way), and wavefronts do not wait for each other until a piece of a sequence ends.
 //
 //   work        units of 64 keys of all sequences end to end, cut into equal chunks, one workgroup each (times head and row groups)
 //   wavefront   one key head, 16 or 32 query rows (row = token * G + head in the group), tiles of KT keys; with fewer heads than
@@ -30,6 +31,7 @@ struct Params {
   const int32_t* block_table; int64_t bt_stride; int32_t max_blocks;
   const int32_t *seq_lens, *qsl;
   int64_t num_tokens, num_pages;
+  int32_t page_shift;                                        // log2 of the page, -1 where it is no power of two
   int32_t page_size, batch, max_q_len, kv_heads, group, window;
   int32_t num_chunks;                                        // 0: a workgroup takes a whole sequence
   int32_t heads_shift;                                       // log2 of the heads of a workgroup
@@ -95,7 +97,7 @@ template <typename T, int D, bool kFp8> struct Shape {
   static constexpr int es = kFp8 ? 1 : 2, row_b = D * es;
   static constexpr int kt = 8192 / (2 * row_b) < 16 ? 16 : 8192 / (2 * row_b);   // keys of a tile
   static constexpr int subs = kt / 16, half_b = kt * row_b, copies = half_b / 1024;
-  static constexpr int waves = half_b > 4096 ? 4 : 8;
+  static constexpr int waves = D == 256 ? 4 : 8;
   static constexpr int wave_b = 4 * half_b;                  // two tiles, keys and values
   static constexpr int keys_per_copy = 1024 / row_b, lanes_per_key = row_b / 16;
   // position of granule c (16 bytes) of a key's row: c ^ swz(key): sixteen keys read at one granule hit different banks
@@ -103,6 +105,8 @@ template <typename T, int D, bool kFp8> struct Shape {
     return row_b >= 256 ? key & 15 : row_b == 128 ? (key >> 1) & 7 : (key >> 2) & 3;
   }
 };
+// Until at most N of the wavefront's copies are on their way.
+template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 constexpr int kStatFloats = 8 * 2 * 32;                      // maxima and sums of up to 8 wavefronts x 32 rows
 
 template <typename T, int D, bool kFp8, int MT>
@@ -147,7 +151,6 @@ __global__ __launch_bounds__((Shape<T, D, kFp8>::waves * 64)) void gqa_split_ker
   const int rows_max = p.max_q_len * p.group;
   const int64_t k_head = (int64_t)(has_head ? head : 0) * p.k_sh, v_head = (int64_t)(has_head ? head : 0) * p.v_sh;
   const float scale_log2 = p.scale_log2 * (kFp8 && p.k_scale && has_head ? p.k_scale[head] : 1.f);
-  const float v_scale = kFp8 && p.v_scale && has_head ? p.v_scale[head] : 1.f;
 
   for (; p.num_chunks == 0 || v_cur < v_end; b++) {
     if (b >= p.batch) break;
@@ -176,6 +179,57 @@ __global__ __launch_bounds__((Shape<T, D, kFp8>::waves * 64)) void gqa_split_ker
       key1 = key1 < sq.len ? key1 : sq.len;
       const int tiles = key1 > key0 ? (key1 - key0 + Sh::kt - 1) / Sh::kt : 0;
       const int mine = has_head && tiles > kw ? (tiles - kw + kws - 1) / kws : 0;
+
+      // ---- copies of a tile's keys or values into the ring ----
+      const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
+      const int lk = lane / Sh::lanes_per_key, lp = lane % Sh::lanes_per_key;
+      // page numbers of the wavefront's next 64 pages, one to a lane
+      int have0 = 0, have = 0;
+      auto pages_from = [&](int pi) {
+        const int at = pi + lane;
+        have0 = pi;
+        have = bt[at < p.max_blocks ? at : p.max_blocks - 1];
+      };
+      struct Place { int64_t pg; int off; } place[Sh::subs];
+      auto find = [&](int tile) {
+#pragma unroll
+        for (int s = 0; s < Sh::subs; s++) {
+          const int key = key0 + (kw + tile * kws) * Sh::kt + s * 16;
+          const int pi = p.page_shift >= 0 ? key >> p.page_shift : (int)((uint32_t)key / (uint32_t)p.page_size);
+          place[s].off = __builtin_amdgcn_readfirstlane(p.page_shift >= 0 ? key & (p.page_size - 1) : key - pi * p.page_size);
+          if (__builtin_amdgcn_readfirstlane(pi - have0) > 63) pages_from(__builtin_amdgcn_readfirstlane(pi));
+          const int64_t pg = __builtin_amdgcn_readlane(have, __builtin_amdgcn_readfirstlane(pi - have0));
+          place[s].pg = pg < 0 ? 0 : pg < p.num_pages ? pg : p.num_pages - 1;
+        }
+      };
+      auto copy = [&](int tile, bool values) {
+        const char* base = values ? p.v + v_head : p.k + k_head;
+        const int64_t sp = values ? p.v_sp : p.k_sp, sr = values ? p.v_sr : p.k_sr;
+        const uint32_t to = ring0 + (tile & 1) * 2 * Sh::half_b + (values ? Sh::half_b : 0);
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");     // (what was read of the place has arrived)
+#pragma unroll
+        for (int s = 0; s < Sh::subs; s++) {
+          const char* from = base + place[s].pg * sp + (int64_t)place[s].off * sr;
+#pragma unroll
+          for (int c = 0; c < Sh::copies / Sh::subs; c++) {
+            const int kk = c * Sh::keys_per_copy + lk;       // (key of the sixteen)
+            const uint32_t at = (uint32_t)kk * (uint32_t)sr + (uint32_t)((lp ^ Sh::swz(kk)) << 4);
+            dma16_sv_nt(from, at, to + (s * (Sh::copies / Sh::subs) + c) * 1024);
+          }
+        }
+      };
+      if (mine > 0) {
+        const int key = key0 + kw * Sh::kt;
+        pages_from(__builtin_amdgcn_readfirstlane((int)((uint32_t)key / (uint32_t)p.page_size)));
+        find(0);
+        copy(0, false);
+        copy(0, true);
+        if (mine > 1) {
+          find(1);
+          copy(1, false);
+          copy(1, true);
+        }
+      }
 
       // ---- the query: row l16 of each row tile, eight dims a step; zeros in rows that do not exist ----
       v8 qf[MT][D / 32];
@@ -216,37 +270,12 @@ __global__ __launch_bounds__((Shape<T, D, kFp8>::waves * 64)) void gqa_split_ker
         for (int d = 0; d < D / 16; d++) acc[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
 
-      // ---- copies of a tile's keys or values into the ring ----
-      const int32_t* bt = p.block_table + (int64_t)b * p.bt_stride;
-      const int lk = lane / Sh::lanes_per_key, lp = lane % Sh::lanes_per_key;
-      auto copy = [&](int tile, bool values) {
-        const char* base = values ? p.v : p.k;
-        const int64_t sp = values ? p.v_sp : p.k_sp, sr = values ? p.v_sr : p.k_sr, hd = values ? v_head : k_head;
-        const uint32_t to = ring0 + (tile & 1) * 2 * Sh::half_b + (values ? Sh::half_b : 0);
-#pragma unroll
-        for (int s = 0; s < Sh::subs; s++) {
-          const int key = key0 + (kw + tile * kws) * Sh::kt + s * 16;
-          int pi = (int)((uint32_t)key / (uint32_t)p.page_size);
-          const int off = key - pi * p.page_size;
-          pi = pi < p.max_blocks ? pi : p.max_blocks - 1;
-          int64_t pg = __builtin_amdgcn_readfirstlane(bt[pi]);
-          pg = pg < 0 ? 0 : pg < p.num_pages ? pg : p.num_pages - 1;
-          const char* from = base + pg * sp + (int64_t)off * sr + hd;
-#pragma unroll
-          for (int c = 0; c < Sh::copies / Sh::subs; c++) {
-            const int kk = c * Sh::keys_per_copy + lk;       // (key of the sixteen)
-            const uint32_t at = (uint32_t)kk * (uint32_t)sr + (uint32_t)((lp ^ Sh::swz(kk)) << 4);
-            dma16_sv_nt(from, at, to + (s * (Sh::copies / Sh::subs) + c) * 1024);
-          }
-        }
-      };
-
       for (int i = 0; i < mine; i++) {
         const int tile_key = key0 + (kw + i * kws) * Sh::kt;
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        copy(i, false);
-        copy(i, true);
-        MLA_WAIT_VMCNT(0);
+        // (younger than the tile's keys: its values, and the next tile's keys and values)
+        const bool next = i + 1 < mine, after = i + 2 < mine;
+        if (next) wait_copies<3 * Sh::copies>();
+        else wait_copies<Sh::copies>();
         const char* kt = ring + (i & 1) * 2 * Sh::half_b;
         const char* vt = kt + Sh::half_b;
         const bool partial = tile_key + Sh::kt > all_hi || tile_key < all_lo;
@@ -282,6 +311,10 @@ __global__ __launch_bounds__((Shape<T, D, kFp8>::waves * 64)) void gqa_split_ker
               for (int m = 0; m < MT; m++) sc[m][s] = Ty::qk(a, qf[m][t], sc[m][s]);
             }
           }
+        }
+        if (after) {
+          find(i + 2);
+          copy(i + 2, false);
         }
         // ---- probabilities against the rows' references ----
         u32x2 pf[MT][Sh::subs];
@@ -325,6 +358,9 @@ __global__ __launch_bounds__((Shape<T, D, kFp8>::waves * 64)) void gqa_split_ker
             pf[m][s] = __builtin_bit_cast(u32x2, pr);
           }
         }
+        if (after) wait_copies<3 * Sh::copies>();
+        else if (next) wait_copies<2 * Sh::copies>();
+        else wait_copies<0>();
         // ---- O^T += V^T P^T ----
         // A tile with keys that a row does not see is done token by token with those keys' values cleared (0 times what lies there,
         // an infinity or stale NaN, would not be 0), and a lane takes the product of its own row's token.
@@ -382,6 +418,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8>::waves * 64)) void gqa_split_ker
             }
           }
         }
+        if (after) copy(i + 2, true);
       }
 
       // ---- join of the wavefronts of a head, a row tile at a time, and the rows' results ----
@@ -445,7 +482,6 @@ __global__ __launch_bounds__((Shape<T, D, kFp8>::waves * 64)) void gqa_split_ker
         }
         lds_barrier();
       }
-      (void)v_scale;
     }
     if (p.num_chunks == 0) break;
   }
@@ -580,6 +616,7 @@ extern "C" int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_st
   p.block_table = block_table; p.bt_stride = bt_stride; p.max_blocks = max_blocks;
   p.seq_lens = seq_lens; p.qsl = query_start_loc;
   p.num_tokens = num_tokens; p.num_pages = num_pages;
+  p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
   p.page_size = page_size; p.batch = batch; p.max_q_len = max_q_len; p.kv_heads = kv_heads; p.group = q_heads / kv_heads;
   p.window = window; p.num_chunks = num_chunks;
   p.scale_log2 = scale * kLog2e;
@@ -592,7 +629,7 @@ extern "C" int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_st
     p.part_acc = (float*)((char*)p.part_lse + gqa::align256(n * 4));
   }
   const int rows = max_q_len * p.group, mt = rows > 16 ? 2 : 1;
-  const int waves = dim == 256 && es == 2 ? 4 : 8;
+  const int waves = dim == 256 ? 4 : 8;
   // heads of a workgroup: as many as it has wavefronts, where they are a power of two's multiple
   int shift = 0;
   while ((2 << shift) <= waves && kv_heads % (2 << shift) == 0) shift++;

@@ -639,7 +639,7 @@ bool qk_norm_rope_cache(const Tensor& q, const OptTensor& k, const OptTensor& v,
 
 // kernels.gqa_chunks
 int gqa_chunks(int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads, int64_t dim, bool fp8, int64_t max_seq_len) {
-  const int64_t rows = q_len * q_heads / kv_heads, waves = dim == 256 && !fp8 ? 4 : 8;
+  const int64_t rows = q_len * q_heads / kv_heads, waves = dim == 256 ? 4 : 8;
   int64_t heads = 1;
   while (heads * 2 <= waves && kv_heads % (heads * 2) == 0) heads *= 2;
   const int64_t groups = kv_heads / heads * div_up(rows, rows <= 16 ? 16 : 32), units = batch * div_up(max_seq_len, 64);
@@ -679,21 +679,51 @@ bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, c
                           ws ? ws->data_ptr() : nullptr, ws ? (size_t)ws->numel() : 0, chunks, st), "mlahip_gqa_decode");
 }
 
-// The launch of kernels.copy_pages, which has checked the tensors and the pairs: the library's code.
-int copy_pages(const std::vector<Tensor>& caches, const std::vector<int32_t>& src, const std::vector<int32_t>& dst,
-                const std::optional<std::vector<int32_t>>& rows, const OptTensor& table) {
+// kernels.copy_pages
+bool whole_numbers(py::handle list, std::vector<int32_t>& to) {
+  if (!PyList_CheckExact(list.ptr())) return false;
+  const Py_ssize_t n = PyList_GET_SIZE(list.ptr());
+  to.resize(n);
+  for (Py_ssize_t i = 0; i < n; i++) {
+    PyObject* x = PyList_GET_ITEM(list.ptr(), i);
+    if (!PyLong_CheckExact(x)) return false;
+    int over = 0;
+    const long v = PyLong_AsLongAndOverflow(x, &over);
+    if (over || v < 0 || v > 0x7fffffff) return false;
+    to[i] = (int32_t)v;
+  }
+  return true;
+}
+bool copy_pages(const std::vector<Tensor>& caches, py::handle src_list, py::handle dst_list, py::handle rows_list, const OptTensor& table) {
+  if (caches.empty() || !current_gpu(caches[0])) return false;
+  const at::Device dev = caches[0].device();
+  std::vector<int32_t> src, dst, rows;
+  const bool part = !rows_list.is_none();
+  if (!whole_numbers(src_list, src) || !whole_numbers(dst_list, dst) || (part && !whole_numbers(rows_list, rows)) || dst.size() != src.size() ||
+      (part && rows.size() != src.size()))
+    return false;
+  if (table && (table->scalar_type() != at::kInt || table->dim() != 2 || table->device() != dev || (table->size(1) > 1 && table->stride(1) != 1) ||
+                (table->size(0) > 1 && table->stride(0) < table->size(1))))
+    return false;
   std::vector<mlahip_page_cache> list;
   list.reserve(caches.size());
   for (const Tensor& c : caches) {
-    const int64_t es = c.element_size(), row = c.numel() / (c.size(0) * c.size(1)) * es;
+    if (c.dim() < 2 || c.device() != dev || c.size(0) < 1 || c.size(1) < 1 || c.size(0) != caches[0].size(0) || c.size(1) != caches[0].size(1) ||
+        wants_grad({&c}))
+      return false;
+    int64_t width = 1;
+    for (int64_t i = c.dim() - 1; i >= 2; i--) {               // (rows of contiguous elements)
+      if (c.size(i) != 1 && c.stride(i) != width) return false;
+      width *= c.size(i);
+    }
     // (the stride of a dim of one entry says nothing)
-    const int64_t row_stride = c.size(1) > 1 ? c.stride(1) * es : row, page_stride = c.size(0) > 1 ? c.stride(0) * es : row_stride * c.size(1);
-    list.push_back({c.data_ptr(), page_stride, row_stride, row});
+    const int64_t es = c.element_size(), row = width * es, row_stride = c.size(1) > 1 ? c.stride(1) * es : row;
+    list.push_back({c.data_ptr(), c.size(0) > 1 ? c.stride(0) * es : row_stride * c.size(1), row_stride, row});
   }
-  return mlahip_copy_pages(list.data(), (int)list.size(), src.data(), dst.data(), rows ? rows->data() : nullptr, (int)src.size(), caches[0].size(0),
-                          (int)caches[0].size(1), table ? (int32_t*)table->data_ptr() : nullptr,
-                          table ? (table->size(0) > 1 ? table->stride(0) : table->size(1)) : 0, table ? (int)table->size(0) : 0,
-                          table ? (int)table->size(1) : 0, stream_of(caches[0]));
+  return done(mlahip_copy_pages(list.data(), (int)list.size(), src.data(), dst.data(), part ? rows.data() : nullptr, (int)src.size(),
+                                caches[0].size(0), (int)caches[0].size(1), table ? (int32_t*)table->data_ptr() : nullptr,
+                                table ? (table->size(0) > 1 ? table->stride(0) : table->size(1)) : 0, table ? (int)table->size(0) : 0,
+                                table ? (int)table->size(1) : 0, stream_of(caches[0])), "mlahip_copy_pages");
 }
 
 }  // namespace

@@ -3,6 +3,7 @@ strides and the current HIP stream, and never allocates behind the caller's back
 split-KV workspace, which is cached per (device, size)."""
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Optional
 
@@ -1486,7 +1487,7 @@ def qk_norm_rope_cache(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[t
 def gqa_chunks(batch: int, q_len: int, q_heads: int, kv_heads: int, dim: int, fp8: bool, max_seq_len: int, num_cus: int = 256) -> int:
     """Pieces that gqa_decode cuts the cached keys of a step into (0: a request to a workgroup, one launch)."""
     rows = q_len * q_heads // kv_heads
-    waves = 4 if dim == 256 and not fp8 else 8
+    waves = 4 if dim == 256 else 8
     heads = 1
     while heads * 2 <= waves and kv_heads % (heads * 2) == 0:
         heads *= 2
@@ -1581,6 +1582,8 @@ def copy_pages(caches, src, dst, rows=None, block_table: Optional[torch.Tensor] 
         raise ValueError(f"{what}: src, dst and rows are read on the host: lists or CPU tensors")
     caches = [caches] if torch.is_tensor(caches) else list(caches)
     src, dst, rows = as_list(src), as_list(dst), None if rows is None else as_list(rows)
+    if _host.load().copy_pages(caches, src, dst, rows, block_table):
+        return
     if any(isinstance(i, bool) or not isinstance(i, int) for x in (src, dst, rows or ()) for i in x):
         raise TypeError(f"{what}: page numbers and rows are whole numbers")
     if not caches or len(src) != len(dst) or rows is not None and len(rows) != len(src):
@@ -1609,5 +1612,12 @@ def copy_pages(caches, src, dst, rows=None, block_table: Optional[torch.Tensor] 
             raise ValueError(f"{what}: block_table must be int32 [requests, blocks] with contiguous rows")
     if not src:
         return
+    row_bytes = [math.prod(c.shape[2:]) * c.element_size() for c in caches]
+    geometry = [(c.stride(0) * c.element_size() if pages > 1 else w * page, c.stride(1) * c.element_size() if page > 1 else w, w)
+                for c, w in zip(caches, row_bytes)]
+    words = (ctypes.c_int64 * (4 * len(caches)))(*(x for c, geo in zip(caches, geometry) for x in (c.data_ptr(), *geo)))
+    ints = lambda x: None if x is None else (ctypes.c_int32 * len(x))(*x)
+    table = (None, 0, 0, 0) if block_table is None else (block_table.data_ptr(), max(block_table.stride(0), block_table.shape[1]), *block_table.shape)
     with torch.cuda.device(dev):
-        _lib.check(_host.load().copy_pages(caches, src, dst, rows, block_table), "mlahip_copy_pages")
+        rc = _lib.load().mlahip_copy_pages(words, len(caches), ints(src), ints(dst), ints(rows), len(src), pages, page, *table, _stream(caches[0]))
+    _lib.check(rc, "mlahip_copy_pages")
