@@ -22,6 +22,7 @@
 #include <map>
 #include <mutex>
 #include <optional>
+#include <tuple>
 #include <utility>
 
 #include "../../../include/mla_hip.h"
@@ -623,6 +624,7 @@ bool qk_norm_rope_cache(const Tensor& q, const OptTensor& k, const OptTensor& v,
   }
   if (!head_scale(k_scale, fp8, hk, dev) || !head_scale(v_scale, fp8, hk, dev) || wants_grad({&q, &*k, ptr_of(v), ptr_of(q_gamma), ptr_of(k_gamma)}))
     return false;
+  if (t == 0) return true;
   const Tensor& qo = q_out ? *q_out : q;
   const Tensor* ko = k_out ? &*k_out : cached ? nullptr : &*k;
   const Tensor *kc = cached ? &*k_cache : nullptr, *vc = cached ? &*v_cache : nullptr;
@@ -637,24 +639,38 @@ bool qk_norm_rope_cache(const Tensor& q, const OptTensor& k, const OptTensor& v,
             ko ? ko->data_ptr() : nullptr, ko ? ko->stride(0) : 0, ko ? ko->stride(1) : 0, stream_of(q)), "mlahip_qk_norm_rope_cache");
 }
 
-// kernels.gqa_chunks
-int gqa_chunks(int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads, int64_t dim, bool fp8, int64_t max_seq_len) {
-  const int64_t rows = q_len * q_heads / kv_heads, waves = dim == 256 ? 4 : 8;
-  int64_t heads = 1;
-  while (heads * 2 <= waves && kv_heads % (heads * 2) == 0) heads *= 2;
-  const int64_t groups = kv_heads / heads * div_up(rows, rows <= 16 ? 16 : 32), units = batch * div_up(max_seq_len, 64);
-  return (int)std::max<int64_t>(1, std::min(256 / groups, units));
+// kernels.gqa_plan
+std::pair<int, int> gqa_plan(int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t element_bytes, int64_t max_seq_len) {
+  const int64_t rows = q_len * q_heads / kv_heads, waves = dim == 256 ? 4 : 8, row_groups = div_up(rows, rows <= 16 ? 16 : 32);
+  const int64_t key = 2 * dim * element_bytes, units = batch * div_up(max_seq_len, 64);
+  std::tuple<double, int64_t, int64_t> best{INFINITY, 1, 1};
+  for (int64_t heads = 1; heads <= waves && kv_heads % heads == 0; heads *= 2) {
+    const int64_t groups = kv_heads / heads * row_groups;
+    const double run = heads == kv_heads ? 1.0 : std::min(1.0, std::sqrt((double)(heads * key) / 750.0));
+    const double stream = (double)(batch * max_seq_len * kv_heads * row_groups * key) / (6.75e6 * run);
+    const auto walk = [&](int64_t keys) {
+      return std::max((double)(div_up(keys * heads, 32 * waves) * key) / 225.0, (double)(keys * heads * key) / 27e3);
+    };
+    if (max_seq_len <= 1280) {
+      const int64_t rounds = div_up(batch * groups, 256);
+      best = std::min(best, {3.0 + std::max(3.0 * (double)(rounds - 1) + (double)rounds * walk(max_seq_len), stream), 0, heads});
+    }
+    const int64_t chunks = std::max<int64_t>(1, std::min(units, 256 / groups)), size = div_up(units, chunks) * 64;
+    const double joins = 4.5 * std::max(1.0, (double)batch / (double)chunks) * (double)div_up(chunks * groups, 256);
+    best = std::min(best, {7.0 + std::max(walk(std::min(size, batch * max_seq_len)), stream) + joins, chunks, heads});
+  }
+  return {(int)std::get<1>(best), (int)std::get<2>(best)};
 }
 
 // kernels.gqa_decode
 bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& seq_lens, double scale,
                 const Tensor& out, int64_t q_len, const OptTensor& qsl, int64_t window, const OptTensor& k_scale, const OptTensor& v_scale,
-                const OptTensor& lse, int64_t num_chunks, int64_t max_seq_len, const OptTensor& workspace) {
+                const OptTensor& lse, int64_t num_chunks, int64_t max_seq_len, const OptTensor& workspace, int64_t heads_per_group) {
   if (!current_gpu(q) || q.dim() != 3 || workspace || k_cache.dim() != 4 || num_chunks > (1 << 16)) return false;
   const at::Device dev = q.device();
   const at::ScalarType dt = q.scalar_type();
   const int64_t t = q.size(0), hq = q.size(1), d = q.size(2), hk = k_cache.size(2), b = seq_lens.numel();
-  if ((dt != at::kBFloat16 && dt != at::kHalf) || q.stride(2) != 1 || !heads_of(out, t, hq, d, dt, dev) || hk < 1 || hq < 1 || hq % hk ||
+  if ((dt != at::kBFloat16 && dt != at::kHalf) || t < 1 || q.stride(2) != 1 || !heads_of(out, t, hq, d, dt, dev) || hk < 1 || hq < 1 || hq % hk ||
       !head_cache(k_cache, hk, d, dt, dev) || !head_cache(v_cache, hk, d, dt, dev) || k_cache.sizes() != v_cache.sizes() ||
       k_cache.scalar_type() != v_cache.scalar_type() || q_len < 1 || window < 0 || !is_i32(seq_lens, 1, dev) || !seq_lens.is_contiguous() ||
       !is_i32(block_table, 2, dev) || block_table.size(0) < b || block_table.size(1) < 1 || b < 1 ||
@@ -666,7 +682,8 @@ bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, c
   int64_t longest = block_table.size(1) * k_cache.size(1);
   if (max_seq_len > 0 && c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) longest = std::min(longest, max_seq_len);
   if (window > 0) longest = std::min(longest, window + q_len + 62);
-  const int chunks = num_chunks >= 0 ? (int)num_chunks : gqa_chunks(b, q_len, hq, hk, d, fp8, longest);
+  const auto [by_rule, heads] = gqa_plan(b, q_len, hq, hk, d, k_cache.element_size(), longest);
+  const int chunks = num_chunks >= 0 ? (int)num_chunks : by_rule;
   Stream st = stream_of(q);
   const int64_t need = (int64_t)mlahip_gqa_decode_workspace_bytes((int)b, (int)q_len, (int)hq, (int)d, chunks);
   Tensor* ws = need ? &scratch(q, st, need, 3) : nullptr;
@@ -676,7 +693,8 @@ bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, c
                           (const int32_t*)seq_lens.data_ptr(), (const int32_t*)data_of(qsl), (int)b, (int)q_len, (int)hq, (int)hk, (int)d,
                           type_code(dt), type_code(k_cache.scalar_type()), (const float*)data_of(k_scale), (const float*)data_of(v_scale),
                           (float)scale, (int)window, out.data_ptr(), out.stride(0), out.stride(1), (float*)data_of(lse),
-                          ws ? ws->data_ptr() : nullptr, ws ? (size_t)ws->numel() : 0, chunks, st), "mlahip_gqa_decode");
+                          ws ? ws->data_ptr() : nullptr, ws ? (size_t)ws->numel() : 0, chunks, heads_per_group > 0 ? (int)heads_per_group : heads, st),
+              "mlahip_gqa_decode");
 }
 
 // kernels.copy_pages
@@ -743,7 +761,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("copy_pages", &copy_pages);
   // (what this file has a copy of, for a test to hold against kernels.py)
   m.def("launch_splits", &launch_splits, py::arg("batch"), py::arg("q_len"), py::arg("heads"), py::arg("max_seq_len"), py::arg("full") = false);
-  m.def("gqa_chunks", &gqa_chunks);
+  m.def("gqa_plan", &gqa_plan);
   m.def("prefill_long_rows", &prefill_long_rows);
   m.def("prefill_blocks", &prefill_blocks);
   m.def("prefill_pieces", &prefill_pieces);

@@ -1474,6 +1474,8 @@ def qk_norm_rope_cache(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[t
         cache_args = (k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(), *v_cache.stride()[:3], k_cache.shape[1], k_cache.shape[0])
     elif k_scale is not None or v_scale is not None:
         raise ValueError(f"{what}: scales go with a float8_e4m3fn cache")
+    if t == 0:
+        return
     row = lambda x: (x.data_ptr(), x.stride(0), x.stride(1)) if x is not None else (None, 0, 0)
     ptr = lambda x: x.data_ptr() if x is not None else None
     with torch.cuda.device(dev):
@@ -1484,23 +1486,44 @@ def qk_norm_rope_cache(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[t
     _lib.check(rc, "mlahip_qk_norm_rope_cache")
 
 
-def gqa_chunks(batch: int, q_len: int, q_heads: int, kv_heads: int, dim: int, fp8: bool, max_seq_len: int, num_cus: int = 256) -> int:
-    """Pieces that gqa_decode cuts the cached keys of a step into (0: a request to a workgroup, one launch)."""
+def gqa_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, dim: int, element_bytes: int, max_seq_len: int):
+    """(pieces that gqa_decode cuts the cached keys of a step into, key heads of a workgroup); 0 pieces: a request to a workgroup, one
+    launch.  The fastest by an estimate in us of what was measured (9016 launches, 1-128 requests of 64-10 000 keys, heads of 64-256
+    values, 1-8 of them; the estimate's choice is 1.2 % slower than the best one on average):
+    a wavefront's step of 32 keys x 512 bytes 2.3 and a CU's share of the memory 27 KB per us (short contexts are bound by these: few heads
+    to a workgroup, so that its eight wavefronts share their keys), the cache stream 6.75 MB per us, less where a key's heads of a
+    workgroup are few bytes (4 x 128 x 64 heads of 64 x 10 000: 72 in workgroups of 8 heads, 122 of 1); 3 for one launch, 3 for
+    each further round of workgroups, 7 for two launches and 4.5 for each piece of a sequence in a chunk.  32/8 heads of 128, us in one launch / cut:
+    1 x 256 keys 8.7 / 10.8, 1 x 1024 16.8 / 10.8, 32 x 1024 26.8 / 28.8, 128 x 64 10.9 / 14.6.  Longer than 1280 keys a request to a workgroup loses up
+    to two thirds where lengths are ragged, which the host does not know."""
     rows = q_len * q_heads // kv_heads
     waves = 4 if dim == 256 else 8
+    row_groups = -(-rows // (16 if rows <= 16 else 32))
+    key = 2 * dim * element_bytes
+    units = batch * -(-max_seq_len // 64)
+    best = (math.inf, 1, 1)
     heads = 1
-    while heads * 2 <= waves and kv_heads % (heads * 2) == 0:
+    while heads <= waves and kv_heads % heads == 0:
+        groups = kv_heads // heads * row_groups
+        run = 1.0 if heads == kv_heads else min(1.0, math.sqrt(heads * key / 750.0))
+        stream = batch * max_seq_len * kv_heads * row_groups * key / (6.75e6 * run)
+        walk = lambda keys: max(-(-keys * heads // (32 * waves)) * key / 225.0, keys * heads * key / 27e3)
+        if max_seq_len <= 1280:
+            rounds = -(-batch * groups // 256)
+            best = min(best, (3.0 + max(3.0 * (rounds - 1) + rounds * walk(max_seq_len), stream), 0, heads))
+        chunks = max(1, min(units, 256 // groups))
+        size = -(-units // chunks) * 64
+        joins = 4.5 * max(1.0, batch / chunks) * -(-chunks * groups // 256)
+        best = min(best, (7.0 + max(walk(min(size, batch * max_seq_len)), stream) + joins, chunks, heads))
         heads *= 2
-    groups = kv_heads // heads * math.ceil(rows / (16 if rows <= 16 else 32))
-    units = batch * math.ceil(max_seq_len / 64)
-    return max(1, min(num_cus // groups, units))
+    return best[1:]
 
 
 def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
                scale: float, out: torch.Tensor, q_len: int = 1, query_start_loc: Optional[torch.Tensor] = None,
                window: Optional[int] = None, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
                lse_out: Optional[torch.Tensor] = None, num_chunks: Optional[int] = None, max_seq_len: Optional[int] = None,
-               workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+               workspace: Optional[torch.Tensor] = None, heads_per_group: Optional[int] = None) -> torch.Tensor:
     """Attention of each request's newest tokens over a paged cache of ordinary key and value heads.
 
     q [T,Hq,D] bf16 or fp16, D 64, 128 or 256; caches [pages, page, Hk, D] of its type or float8_e4m3fn (times ``k_scale`` /
@@ -1513,7 +1536,8 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
     what = "gqa_decode"
     if _host.load().gqa_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out, q_len, query_start_loc,
                                0 if window is None else window or -1, k_scale, v_scale, lse_out,
-                               -1 if num_chunks is None else num_chunks, max_seq_len or 0, workspace):
+                               -1 if num_chunks is None else num_chunks, max_seq_len or 0, workspace,
+                               heads_per_group or 0):
         return out
     dev = _one_device(what, q, k_cache, v_cache, block_table, seq_lens, out, query_start_loc, k_scale, v_scale, lse_out, workspace)
     _no_grad(what, q, k_cache, v_cache)
@@ -1545,6 +1569,8 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
     if lse_out is not None and (lse_out.dtype != torch.float32 or lse_out.shape != (t, hq) or not lse_out.is_contiguous()):
         raise ValueError(f"{what}: lse_out must be contiguous fp32 [{t}, {hq}]")
     scales = _head_scales(what, code == _E4M3, hk, k_scale=k_scale, v_scale=v_scale)
+    if t == 0 or b == 0:
+        return out
     lib = _lib.load()
     with torch.cuda.device(dev):
         longest = block_table.shape[1] * k_cache.shape[1]
@@ -1552,8 +1578,8 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
             longest = min(longest, max_seq_len)
         if window is not None:
             longest = min(longest, window + q_len + 62)
-        if num_chunks is None:
-            num_chunks = gqa_chunks(b, q_len, hq, hk, d, code == _E4M3, longest)
+        chunks, heads = gqa_plan(b, q_len, hq, hk, d, k_cache.element_size(), longest)
+        num_chunks = chunks if num_chunks is None else num_chunks
         need = lib.mlahip_gqa_decode_workspace_bytes(b, q_len, hq, d, num_chunks)
         ws = workspace
         if ws is None and need:
@@ -1563,7 +1589,8 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
             k_cache.shape[0], k_cache.shape[1], block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
             query_start_loc.data_ptr() if query_start_loc is not None else None, b, q_len, hq, hk, d, _HEAD_DT[q.dtype], code, *scales,
             float(scale), window or 0, out.data_ptr(), out.stride(0), out.stride(1), lse_out.data_ptr() if lse_out is not None else None,
-            ws.data_ptr() if ws is not None else None, ws.numel() * ws.element_size() if ws is not None else 0, num_chunks, _stream(q))
+            ws.data_ptr() if ws is not None else None, ws.numel() * ws.element_size() if ws is not None else 0, num_chunks,
+            heads_per_group or heads, _stream(q))
     _lib.check(rc, "mlahip_gqa_decode")
     return out
 

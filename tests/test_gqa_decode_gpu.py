@@ -280,3 +280,12 @@ def test_refusals(dev):
     refused(K._lib.MlaHipError, "multiple of 16", {1: on["k"][:, :24], 2: on["v"][:, :24]})
     q = torch.zeros(2 * 8 * 128 + 1, dtype=torch.bfloat16, device=dev)[1:].view(2, 8, 128)
     refused(K._lib.MlaHipError, "16-byte aligned", {0: q})
+
+
+def test_no_tokens(dev):
+    from omni_npu_amd import kernels as K
+    c = make(dev, [5])
+    none = torch.empty(0, 8, 128, dtype=torch.bfloat16, device=dev)
+    K.gqa_decode(none, c["k"].to(dev), c["v"].to(dev), c["table"].to(dev), c["lens"].to(dev)[:0], 1.0, none)
+    K.gqa_decode(none, c["k"].to(dev), c["v"].to(dev), c["table"].to(dev), c["lens"].to(dev), 1.0, none,
+                 query_start_loc=torch.zeros(2, dtype=torch.int32, device=dev))

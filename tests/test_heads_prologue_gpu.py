@@ -246,3 +246,14 @@ def test_refusals(dev):
     refused(K._lib.MlaHipError, "aligned", {0: odd}, q_out=q)
     with pytest.raises(ValueError, match="go with k"):
         K.qk_norm_rope_cache(q, None, None, on["cos"], on["sin"], on["positions"], k_gamma=on["kg"])
+
+
+def test_no_tokens(dev):
+    from omni_npu_amd import kernels as K
+    c = make(1, 4, 2, 64, 64)
+    z = lambda h: torch.empty(0, h, 64, dtype=torch.bfloat16, device=dev)
+    i = torch.empty(0, dtype=torch.int64, device=dev)
+    kc = c["kc"].to(dev)
+    K.qk_norm_rope_cache(z(4), z(2), z(2), c["cos"].to(dev), c["sin"].to(dev), i, i, kc, kc.clone())
+    K.qk_norm_rope_cache(z(4), None, None, c["cos"].to(dev), c["sin"].to(dev), i)
+    assert torch.equal(kc.cpu(), c["kc"])
