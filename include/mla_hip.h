@@ -580,8 +580,9 @@ int mlahip_qk_norm_rope_cache(
  * seq_lens beyond the block table's room count as that room; page numbers outside the cache are read as its first or last page.
  * num_chunks > 0: the keys of all requests, end to end, are cut into that many equal pieces, a workgroup each (times groups of
  * heads and rows), and a second launch joins the pieces of a request, with mlahip_gqa_decode_workspace_bytes of workspace;
- * 0: one launch, a request to a workgroup, no workspace.  heads_per_group: key heads of a workgroup, a power of two that divides
- * kv_heads, up to its wavefronts (8; 4 for dim 256): the fewer, the more wavefronts share a head's keys. */
+ * 0: one launch, a request to a workgroup, no workspace.  rows_per_group: rows (tokens x query heads of a key head) of a workgroup, 16, 32
+ * or, of heads of up to 128, 64: the more, the fewer times keys are read.  heads_per_group: key heads of a workgroup, a power of two that
+ * divides kv_heads, up to its wavefronts (8; 4 for dim 256 and for 64 rows): the fewer, the more wavefronts share a head's keys. */
 size_t mlahip_gqa_decode_workspace_bytes(int32_t batch, int32_t max_q_len, int32_t q_heads, int32_t dim, int32_t num_chunks);
 int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t num_tokens, const void* k_cache,
                       int64_t kc_page_stride, int64_t kc_row_stride, int64_t kc_head_stride, const void* v_cache,
@@ -590,7 +591,8 @@ int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, int
                       const int32_t* query_start_loc /* may be NULL */, int32_t batch, int32_t max_q_len, int32_t q_heads,
                       int32_t kv_heads, int32_t dim, int32_t dtype, int32_t cache_dtype, const float* k_scale, const float* v_scale,
                       float scale, int32_t window, void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse_out,
-                      void* workspace, size_t workspace_bytes, int32_t num_chunks, int32_t heads_per_group, mlahip_stream_t stream);
+                      void* workspace, size_t workspace_bytes, int32_t num_chunks, int32_t heads_per_group,
+                      int32_t rows_per_group, mlahip_stream_t stream);
 
 /* ---- pages of a cache, any cache -------------------------------------------------------------
  * cache[dst[i], r] = cache[src[i], r] for r < rows[i] (rows = NULL: whole pages) in every cache of the list, in as few launches as

@@ -95,7 +95,7 @@ SIGNATURES = {
                                             I64, P]),
     "mlahip_gqa_decode_workspace_bytes": (SZ, [I32, I32, I32, I32, I32]),
     "mlahip_gqa_decode": (c_int32, [P, I64, I64, I64, P, I64, I64, I64, P, I64, I64, I64, I64, I32, P, I64, I32, P, P, I32, I32, I32, I32,
-                                    I32, I32, I32, P, P, F32, I32, P, I64, I64, P, P, SZ, I32, I32, P]),
+                                    I32, I32, I32, P, P, F32, I32, P, I64, I64, P, P, SZ, I32, I32, I32, P]),
     "mlahip_copy_pages": (c_int32, [P, I32, P, P, P, I32, I64, I32, P, I64, I32, I32, P]),
     "dsa_sparse_decode_heads_bf16": (c_int32, [P, I64, I64, P, I64, I64, P, I64, P, I64, I64, P, I64, P, I32, I32, F32, P, I64,
                                                I64, P, P]),

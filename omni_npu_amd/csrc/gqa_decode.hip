@@ -10,7 +10,7 @@
 // keys whose loads are all under way while it computes on the tile before.
 //
 //   work        units of 64 keys of all sequences end to end, cut into equal chunks, one workgroup each (times head and row groups)
-//   wavefront   one key head, 16 or 32 query rows (row = token * G + head in the group); several wavefronts share a head and take
+//   wavefront   one key head, 16, 32 or 64 query rows (row = token * G + head in the group); several wavefronts share a head and take
 //               every n-th tile
 //   S^T = K Q^T v_mfma_f32_16x16x32: 16 keys x 16 rows.  The operand is what a lane loads: 16 bytes of the key of its number, so keys go
 //               from memory into registers as they are used; a lane gets 4 keys of one row
@@ -122,11 +122,15 @@ __device__ __forceinline__ u32x4 load_nt(__amdgpu_buffer_rsrc_t from, int lane_o
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, lane_offset, offset, 2));
 }
 
+// Four wavefronts to a workgroup instead of eight: where a wavefront's sums, queries and the tile under way do not fit half of a SIMD's
+// registers (32 rows of 128 with 16-bit keys in eight spill: 128 requests x 2000 keys x 64/8 heads, 4 tokens each, 244 us against 135).
+constexpr bool few_waves(int rows, int dim, int element_bytes) { return dim == 256 || rows == 64 || (rows == 32 && dim == 128 && element_bytes == 2); }
+
 template <typename T, int D, bool kFp8, int MT> struct Shape {
   static constexpr int es = kFp8 ? 1 : 2, row_b = D * es;
   static constexpr int gran = row_b / 64;                    // loads of sixteen keys: a lane's granules (16 bytes) of its key
   static constexpr int v_loads = kTile * row_b / 1024, keys_per_load = 1024 / row_b, lanes_per_key = row_b / 16;
-  static constexpr int waves = D == 256 ? 4 : 8;
+  static constexpr int waves = few_waves(16 * MT, D, es) ? 4 : 8;
   static constexpr int ops = kFp8 ? 2 : 1;                   // operands of one transposed read
   static constexpr int join_b = 16 * D * 4, tile_b = kTile * row_b;
   static constexpr int wave_b = join_b > tile_b ? join_b : tile_b;
@@ -470,16 +474,20 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
       int tid = threadIdx.x;                                 // (hidden: the addresses below are not worked out, and kept, in front of the loop)
       asm volatile("" : "+v"(tid));
       const int jl = tid & 63, j16 = jl & 15, jg = jl >> 4;
-#pragma unroll
+#pragma unroll 1
       for (int m = 0; m < MT; m++) {
         // granule position in a row: granule ^ row, so that sixteen rows' writes at one granule hit different banks.  Granule:
         // four dims as the accumulator has them (8 bits: every other one of eight)
         char* to = mine_lds + j16 * (D * 4);
 #pragma unroll
-        for (int d = 0; d < D / 16; d++) *(f32x4*)(to + (((d * 4 + jg) ^ j16) << 4)) = acc[m][d];
-        if (jl < 16) {
-          stats[wave * 16 + jl] = m_ref[m];
-          stats[(Sh::waves + wave) * 16 + jl] = sum[m][0];
+        for (int k = 0; k < MT; k++) {
+          if (k != m) continue;
+#pragma unroll
+          for (int d = 0; d < D / 16; d++) *(f32x4*)(to + (((d * 4 + jg) ^ j16) << 4)) = acc[k][d];
+          if (jl < 16) {
+            stats[wave * 16 + jl] = m_ref[k];
+            stats[(Sh::waves + wave) * 16 + jl] = sum[k][0];
+          }
         }
         if (m == 0 && jl == 0) stats[Sh::waves * 32 + wave] = again ? 1.f : 0.f;
         lds_barrier();
@@ -556,7 +564,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
         };
         if (kws == 1) join(std::integral_constant<int, 1>{});
         else if (kws == 2) join(std::integral_constant<int, 2>{});
-        else if (kws == 4) join(std::integral_constant<int, 4>{});
+        else if (Sh::waves == 4 || kws == 4) join(std::integral_constant<int, 4>{});
         else join(std::integral_constant<int, 8>{});
         lds_barrier();
       }
@@ -677,8 +685,12 @@ int launch(const Params& p, int row_groups, unsigned x, hipStream_t st) {
   }
   return MLA_OK;
 }
+// 64 rows to a wavefront are for heads of up to 128: wider ones' sums of as many rows do not fit its registers.
 template <typename T, int D, bool kFp8>
 int pick(const Params& p, int mt, int row_groups, unsigned x, hipStream_t st) {
+  if constexpr (D < 256) {
+    if (mt == 4) return launch<T, D, kFp8, 4>(p, row_groups, x, st);
+  }
   return mt == 1 ? launch<T, D, kFp8, 1>(p, row_groups, x, st) : launch<T, D, kFp8, 2>(p, row_groups, x, st);
 }
 template <typename T, int D>
@@ -712,7 +724,8 @@ extern "C" int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_st
                                  int32_t q_heads, int32_t kv_heads, int32_t dim, int32_t dtype, int32_t cache_dtype,
                                  const float* k_scale, const float* v_scale, float scale, int32_t window, void* out,
                                  int64_t out_stride_t, int64_t out_stride_h, float* lse_out, void* workspace, size_t workspace_bytes,
-                                 int32_t num_chunks, int32_t heads_per_group, hipStream_t stream) {
+                                 int32_t num_chunks, int32_t heads_per_group, int32_t rows_per_group,
+                                 hipStream_t stream) {
   const char* me = "mlahip_gqa_decode";
   MLA_REQUIRE(q && k_cache && v_cache && block_table && seq_lens && out, MLA_ERR_NULL, "%s: null pointer argument", me);
   MLA_REQUIRE((dtype == 0 || dtype == 2) && (cache_dtype == dtype || cache_dtype == 3), MLA_ERR_UNSUPPORTED,
@@ -754,8 +767,9 @@ extern "C" int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_st
     p.part_lse = (float*)(ws + gqa::align256((int64_t)batch * 8));
     p.part_acc = (float*)((char*)p.part_lse + gqa::align256(n * 4));
   }
-  const int rows = max_q_len * p.group, mt = rows <= 16 ? 1 : 2;
-  const int waves = dim == 256 ? 4 : 8;
+  MLA_REQUIRE(rows_per_group == 16 || rows_per_group == 32 || (rows_per_group == 64 && dim < 256), MLA_ERR_SHAPE,
+              "%s: %d rows to a workgroup (16, 32, or 64 of heads of up to 128)", me, rows_per_group);
+  const int rows = max_q_len * p.group, mt = rows_per_group / 16, waves = gqa::few_waves(rows_per_group, dim, es) ? 4 : 8;
   MLA_REQUIRE(heads_per_group >= 1 && heads_per_group <= waves && (heads_per_group & (heads_per_group - 1)) == 0 && kv_heads % heads_per_group == 0,
               MLA_ERR_SHAPE, "%s: %d of %d key heads to a workgroup of %d wavefronts (a power of two that divides both)", me, heads_per_group,
               kv_heads, waves);

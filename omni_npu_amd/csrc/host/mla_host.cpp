@@ -640,32 +640,39 @@ bool qk_norm_rope_cache(const Tensor& q, const OptTensor& k, const OptTensor& v,
 }
 
 // kernels.gqa_plan
-std::pair<int, int> gqa_plan(int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t element_bytes, int64_t max_seq_len) {
-  const int64_t rows = q_len * q_heads / kv_heads, waves = dim == 256 ? 4 : 8, row_groups = div_up(rows, rows <= 16 ? 16 : 32);
-  const int64_t key = 2 * dim * element_bytes, units = batch * div_up(max_seq_len, 64);
-  std::tuple<double, int64_t, int64_t> best{INFINITY, 1, 1};
-  for (int64_t heads = 1; heads <= waves && kv_heads % heads == 0; heads *= 2) {
-    const int64_t groups = kv_heads / heads * row_groups;
-    const double run = heads == kv_heads ? 1.0 : std::min(1.0, std::sqrt((double)(heads * key) / 750.0));
-    const double stream = (double)(batch * max_seq_len * kv_heads * row_groups * key) / (6.75e6 * run);
-    const auto walk = [&](int64_t keys) {
-      return std::max((double)(div_up(keys * heads, 32 * waves) * key) / 225.0, (double)(keys * heads * key) / 27e3);
-    };
-    if (max_seq_len <= 1280) {
-      const int64_t rounds = div_up(batch * groups, 256);
-      best = std::min(best, {3.0 + std::max(3.0 * (double)(rounds - 1) + (double)rounds * walk(max_seq_len), stream), 0, heads});
+std::tuple<int, int, int> gqa_plan(int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t element_bytes,
+                                   int64_t max_seq_len) {
+  const int64_t rows = q_len * q_heads / kv_heads, key = 2 * dim * element_bytes, units = batch * div_up(max_seq_len, 64);
+  std::tuple<double, int64_t, int64_t, int64_t> best{INFINITY, 1, 1, 16};
+  for (int64_t tile = 16; tile <= 64; tile *= 2) {
+    if ((tile > 16 && tile / 2 >= rows) || (tile == 64 && dim == 256)) break;
+    const bool few = dim == 256 || tile == 64 || (tile == 32 && dim == 128 && element_bytes == 2);
+    const int64_t waves = few ? 4 : 8, slots = few && dim < 256 && !(tile == 64 && dim == 128) ? 512 : 256, row_groups = div_up(rows, tile);
+    for (int64_t heads = 1; heads <= waves && kv_heads % heads == 0; heads *= 2) {
+      const int64_t groups = kv_heads / heads * row_groups;
+      int halvings = 0;
+      while (heads < kv_heads && heads * key << halvings < 2048) halvings++;
+      const double stream = (double)(batch * max_seq_len * kv_heads * key) * (1.0 + 0.3 * (double)(row_groups - 1)) / (6.8e6 * (1.0 - 0.05 * halvings));
+      const double step = (double)key * (tile == 16 ? 1.0 : 1.35) / 217.0, more = 6.0 * (double)(tile / 16 - 1);
+      const auto walk = [&](int64_t keys) {
+        return std::max((double)div_up(keys * heads, 32 * waves) * step, (double)(keys * heads * key) / 26e3);
+      };
+      if (max_seq_len <= 2048) {
+        const int64_t rounds = div_up(batch * groups, slots);
+        best = std::min(best, {2.2 + more + std::max(5.6 * (double)(rounds - 1) + (double)rounds * walk(max_seq_len), stream), 0, heads, tile});
+      }
+      const int64_t chunks = std::max<int64_t>(1, std::min(units, 256 / groups)), size = div_up(units, chunks) * 64;
+      const double joins = 4.0 * std::max(1.0, (double)batch / (double)chunks) * (double)div_up(chunks * groups, 256);
+      best = std::min(best, {7.4 + more + std::max(walk(std::min(size, batch * max_seq_len)), stream) + joins, chunks, heads, tile});
     }
-    const int64_t chunks = std::max<int64_t>(1, std::min(units, 256 / groups)), size = div_up(units, chunks) * 64;
-    const double joins = 4.5 * std::max(1.0, (double)batch / (double)chunks) * (double)div_up(chunks * groups, 256);
-    best = std::min(best, {7.0 + std::max(walk(std::min(size, batch * max_seq_len)), stream) + joins, chunks, heads});
   }
-  return {(int)std::get<1>(best), (int)std::get<2>(best)};
+  return {(int)std::get<1>(best), (int)std::get<2>(best), (int)std::get<3>(best)};
 }
 
 // kernels.gqa_decode
 bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& seq_lens, double scale,
                 const Tensor& out, int64_t q_len, const OptTensor& qsl, int64_t window, const OptTensor& k_scale, const OptTensor& v_scale,
-                const OptTensor& lse, int64_t num_chunks, int64_t max_seq_len, const OptTensor& workspace, int64_t heads_per_group) {
+                const OptTensor& lse, int64_t num_chunks, int64_t max_seq_len, const OptTensor& workspace, int64_t heads_per_group, int64_t rows_per_group) {
   if (!current_gpu(q) || q.dim() != 3 || workspace || k_cache.dim() != 4 || num_chunks > (1 << 16)) return false;
   const at::Device dev = q.device();
   const at::ScalarType dt = q.scalar_type();
@@ -682,7 +689,7 @@ bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, c
   int64_t longest = block_table.size(1) * k_cache.size(1);
   if (max_seq_len > 0 && c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) longest = std::min(longest, max_seq_len);
   if (window > 0) longest = std::min(longest, window + q_len + 62);
-  const auto [by_rule, heads] = gqa_plan(b, q_len, hq, hk, d, k_cache.element_size(), longest);
+  const auto [by_rule, heads, rows] = gqa_plan(b, q_len, hq, hk, d, k_cache.element_size(), longest);
   const int chunks = num_chunks >= 0 ? (int)num_chunks : by_rule;
   Stream st = stream_of(q);
   const int64_t need = (int64_t)mlahip_gqa_decode_workspace_bytes((int)b, (int)q_len, (int)hq, (int)d, chunks);
@@ -693,7 +700,8 @@ bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, c
                           (const int32_t*)seq_lens.data_ptr(), (const int32_t*)data_of(qsl), (int)b, (int)q_len, (int)hq, (int)hk, (int)d,
                           type_code(dt), type_code(k_cache.scalar_type()), (const float*)data_of(k_scale), (const float*)data_of(v_scale),
                           (float)scale, (int)window, out.data_ptr(), out.stride(0), out.stride(1), (float*)data_of(lse),
-                          ws ? ws->data_ptr() : nullptr, ws ? (size_t)ws->numel() : 0, chunks, heads_per_group > 0 ? (int)heads_per_group : heads, st),
+                          ws ? ws->data_ptr() : nullptr, ws ? (size_t)ws->numel() : 0, chunks, heads_per_group > 0 ? (int)heads_per_group : heads,
+                                rows_per_group > 0 ? (int)rows_per_group : rows, st),
               "mlahip_gqa_decode");
 }
 

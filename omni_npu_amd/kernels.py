@@ -1487,35 +1487,43 @@ def qk_norm_rope_cache(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[t
 
 
 def gqa_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, dim: int, element_bytes: int, max_seq_len: int):
-    """(pieces that gqa_decode cuts the cached keys of a step into, key heads of a workgroup); 0 pieces: a request to a workgroup, one
-    launch.  The fastest by an estimate in us of what was measured (9016 launches, 1-128 requests of 64-10 000 keys, heads of 64-256
-    values, 1-8 of them; the estimate's choice is 1.2 % slower than the best one on average):
-    a wavefront's step of 32 keys x 512 bytes 2.3 and a CU's share of the memory 27 KB per us (short contexts are bound by these: few heads
-    to a workgroup, so that its eight wavefronts share their keys), the cache stream 6.75 MB per us, less where a key's heads of a
-    workgroup are few bytes (4 x 128 x 64 heads of 64 x 10 000: 72 in workgroups of 8 heads, 122 of 1); 3 for one launch, 3 for
-    each further round of workgroups, 7 for two launches and 4.5 for each piece of a sequence in a chunk.  32/8 heads of 128, us in one launch / cut:
-    1 x 256 keys 8.7 / 10.8, 1 x 1024 16.8 / 10.8, 32 x 1024 26.8 / 28.8, 128 x 64 10.9 / 14.6.  Longer than 1280 keys a request to a workgroup loses up
-    to two thirds where lengths are ragged, which the host does not know."""
+    """(pieces that gqa_decode cuts the cached keys of a step into, key heads of a workgroup, rows of a workgroup); 0 pieces: a request to a
+    workgroup, one launch.  The fastest by an estimate in us of what was measured (12 600 launches, 1-128 requests of 64-20 000 keys, heads
+    of 64-256 values, 1-8 of them, 1-64 rows; the estimate's choice is 2 % slower than the best one on average):
+    a wavefront's step of 32 keys x 512 bytes takes 2.4, a third more with more than 16 rows, and a CU takes 26 KB per us from the memory (short contexts
+    are bound by these: few heads to a workgroup, so that its wavefronts share their keys, and few rows, each workgroup reading the keys
+    again); the cache stream 6.8 MB per us, 5 % less for each halving of a key's heads of a workgroup below 2 KB, 30 % longer for each further
+    group of rows; 2.2 for one launch, 5.6 for each further round of workgroups, 7.4 for two launches, 4 for each piece of a sequence in a chunk, 6 for
+    each further 16 rows of a workgroup.  us, one launch / cut, 32/8 heads of 128: 1 x 256 keys 8.7 / 10.8, 1 x 1024 16.8 / 10.8, 32 x 1024 26.8 / 28.8, 128 x 64
+    10.9 / 14.6; workgroups of 1 / 8 heads, 32 x 8 heads of 64 x 10 000 keys 122 / 72; of 16 / 64 rows, 3 tokens x 48/3 heads of 128, 1 x 2000 keys 11.1 / 15.6, 128 x
+    6000 347 / 161.  Beyond 2048 keys a request to a workgroup loses up to two thirds where lengths are ragged, which the host does not know."""
     rows = q_len * q_heads // kv_heads
-    waves = 4 if dim == 256 else 8
-    row_groups = -(-rows // (16 if rows <= 16 else 32))
     key = 2 * dim * element_bytes
     units = batch * -(-max_seq_len // 64)
-    best = (math.inf, 1, 1)
-    heads = 1
-    while heads <= waves and kv_heads % heads == 0:
-        groups = kv_heads // heads * row_groups
-        run = 1.0 if heads == kv_heads else min(1.0, math.sqrt(heads * key / 750.0))
-        stream = batch * max_seq_len * kv_heads * row_groups * key / (6.75e6 * run)
-        walk = lambda keys: max(-(-keys * heads // (32 * waves)) * key / 225.0, keys * heads * key / 27e3)
-        if max_seq_len <= 1280:
-            rounds = -(-batch * groups // 256)
-            best = min(best, (3.0 + max(3.0 * (rounds - 1) + rounds * walk(max_seq_len), stream), 0, heads))
-        chunks = max(1, min(units, 256 // groups))
-        size = -(-units // chunks) * 64
-        joins = 4.5 * max(1.0, batch / chunks) * -(-chunks * groups // 256)
-        best = min(best, (7.0 + max(walk(min(size, batch * max_seq_len)), stream) + joins, chunks, heads))
-        heads *= 2
+    best = (math.inf, 1, 1, 16)
+    for tile in (16, 32, 64):
+        if tile > 16 and tile // 2 >= rows or tile == 64 and dim == 256:
+            break
+        few = dim == 256 or tile == 64 or tile == 32 and dim == 128 and element_bytes == 2
+        waves, slots = 4 if few else 8, 512 if few and dim < 256 and not (tile == 64 and dim == 128) else 256
+        row_groups = -(-rows // tile)
+        heads = 1
+        while heads <= waves and kv_heads % heads == 0:
+            groups = kv_heads // heads * row_groups
+            halvings = 0
+            while heads < kv_heads and heads * key << halvings < 2048:
+                halvings += 1
+            stream = batch * max_seq_len * kv_heads * key * (1.0 + 0.3 * (row_groups - 1)) / (6.8e6 * (1.0 - 0.05 * halvings))
+            step, more = key * (1.0 if tile == 16 else 1.35) / 217.0, 6.0 * (tile // 16 - 1)
+            walk = lambda keys: max(-(-keys * heads // (32 * waves)) * step, keys * heads * key / 26e3)
+            if max_seq_len <= 2048:
+                rounds = -(-batch * groups // slots)
+                best = min(best, (2.2 + more + max(5.6 * (rounds - 1) + rounds * walk(max_seq_len), stream), 0, heads, tile))
+            chunks = max(1, min(units, 256 // groups))
+            size = -(-units // chunks) * 64
+            joins = 4.0 * max(1.0, batch / chunks) * -(-chunks * groups // 256)
+            best = min(best, (7.4 + more + max(walk(min(size, batch * max_seq_len)), stream) + joins, chunks, heads, tile))
+            heads *= 2
     return best[1:]
 
 
@@ -1523,7 +1531,8 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
                scale: float, out: torch.Tensor, q_len: int = 1, query_start_loc: Optional[torch.Tensor] = None,
                window: Optional[int] = None, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
                lse_out: Optional[torch.Tensor] = None, num_chunks: Optional[int] = None, max_seq_len: Optional[int] = None,
-               workspace: Optional[torch.Tensor] = None, heads_per_group: Optional[int] = None) -> torch.Tensor:
+               workspace: Optional[torch.Tensor] = None, heads_per_group: Optional[int] = None,
+               rows_per_group: Optional[int] = None) -> torch.Tensor:
     """Attention of each request's newest tokens over a paged cache of ordinary key and value heads.
 
     q [T,Hq,D] bf16 or fp16, D 64, 128 or 256; caches [pages, page, Hk, D] of its type or float8_e4m3fn (times ``k_scale`` /
@@ -1537,7 +1546,7 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
     if _host.load().gqa_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out, q_len, query_start_loc,
                                0 if window is None else window or -1, k_scale, v_scale, lse_out,
                                -1 if num_chunks is None else num_chunks, max_seq_len or 0, workspace,
-                               heads_per_group or 0):
+                               heads_per_group or 0, rows_per_group or 0):
         return out
     dev = _one_device(what, q, k_cache, v_cache, block_table, seq_lens, out, query_start_loc, k_scale, v_scale, lse_out, workspace)
     _no_grad(what, q, k_cache, v_cache)
@@ -1578,7 +1587,7 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
             longest = min(longest, max_seq_len)
         if window is not None:
             longest = min(longest, window + q_len + 62)
-        chunks, heads = gqa_plan(b, q_len, hq, hk, d, k_cache.element_size(), longest)
+        chunks, heads, rows = gqa_plan(b, q_len, hq, hk, d, k_cache.element_size(), longest)
         num_chunks = chunks if num_chunks is None else num_chunks
         need = lib.mlahip_gqa_decode_workspace_bytes(b, q_len, hq, d, num_chunks)
         ws = workspace
@@ -1590,7 +1599,7 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
             query_start_loc.data_ptr() if query_start_loc is not None else None, b, q_len, hq, hk, d, _HEAD_DT[q.dtype], code, *scales,
             float(scale), window or 0, out.data_ptr(), out.stride(0), out.stride(1), lse_out.data_ptr() if lse_out is not None else None,
             ws.data_ptr() if ws is not None else None, ws.numel() * ws.element_size() if ws is not None else 0, num_chunks,
-            heads_per_group or heads, _stream(q))
+            heads_per_group or heads, rows_per_group or rows, _stream(q))
     _lib.check(rc, "mlahip_gqa_decode")
     return out
 

@@ -19,7 +19,7 @@ def test_gqa_decode_codes():
     raw, p = _buffer()
     #        q, strides, T, k cache, strides, v cache, strides, pages, page, table, stride, blocks, lens, qsl, B, s, Hq, Hk, D, types, scales
     base = [p, 1024, 128, 2, p, 32768, 256, 128, p, 32768, 256, 128, 4, 128, p, 4, 4, p, None, 2, 1, 8, 2, 128, 0, 0, None, None, 0.1, 0, p, 1024,
-            128, None, p, 1 << 20, 4, 2, None]
+            128, None, p, 1 << 20, 4, 2, 16, None]
 
     def rc(**swap):
         args = list(base)
@@ -36,7 +36,7 @@ def test_gqa_decode_codes():
     code, said = rc(_35=lib.mlahip_gqa_decode_workspace_bytes(2, 1, 8, 128, 4) - 1)
     assert code == -4 and "workspace" in said
     assert rc(_34=None)[0] == -4
-    assert all(rc(_37=n)[0] == -2 for n in (-1, 0, 3, 4, 16))
+    assert all(rc(_37=n)[0] == -2 for n in (-1, 0, 3, 4, 16)) and all(rc(_38=n)[0] == -2 for n in (0, 8, 48, 128))
     assert rc(_19=0)[0] == 0 and rc(_3=0)[0] == 0             # nothing to do
     assert lib.mlahip_gqa_decode_workspace_bytes(2, 1, 8, 128, 0) == 0
     del raw
@@ -106,6 +106,7 @@ def test_the_native_host_side_cuts_steps_as_the_wrapper_does():
                 for d in (64, 128, 256):
                     for es in (1, 2):
                         for longest in (1, 64, 300, 1280, 1281, 131072):
-                            chunks, heads = K.gqa_plan(batch, q_len, hq, hk, d, es, longest)
-                            assert (chunks, heads) == tuple(host.gqa_plan(batch, q_len, hq, hk, d, es, longest))
-                            assert chunks >= 0 and hk % heads == 0 and heads <= (4 if d == 256 else 8)
+                            chunks, heads, rows = K.gqa_plan(batch, q_len, hq, hk, d, es, longest)
+                            assert (chunks, heads, rows) == tuple(host.gqa_plan(batch, q_len, hq, hk, d, es, longest))
+                            assert chunks >= 0 and hk % heads == 0 and heads <= (4 if d == 256 or rows == 64 or rows == 32 and d == 128 and es == 2 else 8)
+                            assert rows in ((16, 32) if d == 256 else (16, 32, 64))
