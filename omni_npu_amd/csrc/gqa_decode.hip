@@ -9,7 +9,7 @@
 // where they are short: it issues one every five clocks.  So a wavefront works alone until a piece of a sequence ends, on tiles of 32
 // keys whose loads are all under way while it computes on the tile before.
 //
-//   work        units of 64 keys of all sequences end to end, cut into equal chunks, one workgroup each (times head and row groups)
+//   work        units of 32 keys of all sequences end to end, cut into equal chunks, one workgroup each (times head and row groups)
 //   wavefront   one key head, 16, 32 or 64 query rows (row = token * G + head in the group); several wavefronts share a head and take
 //               every n-th tile
 //   S^T = K Q^T v_mfma_f32_16x16x32: 16 keys x 16 rows.  The operand is what a lane loads: 16 bytes of the key of its number, so keys go
@@ -25,7 +25,7 @@
 namespace mlahip {
 namespace gqa {
 
-constexpr int kUnit = 64;                                    // keys of a plan unit
+constexpr int kUnit = 32;                                    // keys of a plan unit
 constexpr int kTile = 32;                                    // keys of a wavefront's step
 constexpr float kOutgrown = 8.f;                             // log2 units a score may lie above its row's reference
 
@@ -37,6 +37,7 @@ struct Params {
   int32_t max_blocks, num_pages, page_size, page_shift;      // log2 of the page, -1 where it is no power of two
   int32_t batch, max_q_len, kv_heads, group, window;
   int32_t num_chunks;                                        // 0: a workgroup takes a whole sequence
+  int32_t spare_units;                                       // by how much a chunk may be longer to be of one sequence
   int32_t heads_shift, head_groups;                          // log2 of the heads of a workgroup
   float scale_log2;
   // (from here on: what a piece's begin and end take)
@@ -170,7 +171,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
   Seq lane_seq{};
   const bool in_lanes = p.num_chunks > 0 && p.batch <= 64;    // a lane keeps a sequence
   if (p.num_chunks > 0) {
-    int ends, tot = 0;
+    int ends = 0, tot = 0;
     if (in_lanes) {
       if (lane < p.batch) lane_seq = seq_of(p, lane);
       ends = wave_incl_scan_dpp(lane_seq.units);
@@ -179,7 +180,19 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
       for (int i = lane; i < p.batch; i += 64) tot += seq_of(p, i).units;
       tot = __builtin_amdgcn_readlane(wave_incl_scan_dpp(tot), 63);
     }
-    const int size = __builtin_amdgcn_readfirstlane(chunk_units(tot, p.num_chunks));
+    int size = __builtin_amdgcn_readfirstlane(chunk_units(tot, p.num_chunks));
+    // Chunks of one sequence each, where they are few units longer for it: the start of a second piece costs more.
+    const int whole_size = in_lanes && p.num_chunks > p.batch ? __builtin_amdgcn_readfirstlane(chunk_units(tot, p.num_chunks - p.batch)) : 0x7fffffff;
+    if (whole_size <= size + p.spare_units) {
+      const int mine = chunk_units(lane_seq.units, whole_size);
+      const int chunk_ends = wave_incl_scan_dpp(mine);        // (lanes without a sequence: no units)
+      b = __builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < p.batch && chunk_ends <= (int)blockIdx.x));
+      if (b >= p.batch) return;
+      if (b > 0) v_seq = __builtin_amdgcn_readlane(ends, b - 1);
+      v_cur = v_seq + ((int)blockIdx.x - (b > 0 ? __builtin_amdgcn_readlane(chunk_ends, b - 1) : 0)) * whole_size;
+      const int seq_end = __builtin_amdgcn_readlane(ends, b);
+      v_end = v_cur + whole_size < seq_end ? v_cur + whole_size : seq_end;
+    } else {
     v_cur = blockIdx.x * size;
     v_end = v_cur + size < tot ? v_cur + size : tot;
     if (v_cur >= tot) return;
@@ -197,6 +210,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
         b += n;
         carry = __builtin_amdgcn_readlane(run, 63);
       }
+    }
     }
   }
 
@@ -776,6 +790,8 @@ extern "C" int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_st
   const int shift = __builtin_ctz(heads_per_group);
   p.heads_shift = shift;
   p.head_groups = kv_heads >> shift;
+  // (a piece's start and join take about 3.5 us, a CU 26 KB per us)
+  p.spare_units = (int32_t)(3.5f * 26e3f / (float)((int64_t)heads_per_group * 2 * dim * es * gqa::kUnit));
   const int row_groups = (rows + 16 * mt - 1) / (16 * mt);
   MLA_REQUIRE((int64_t)p.head_groups * row_groups <= 65535, MLA_ERR_SHAPE, "%s: %d head groups x %d row groups", me, p.head_groups, row_groups);
   const unsigned x = (unsigned)(num_chunks > 0 ? num_chunks : batch);

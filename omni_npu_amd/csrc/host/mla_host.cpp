@@ -642,7 +642,7 @@ bool qk_norm_rope_cache(const Tensor& q, const OptTensor& k, const OptTensor& v,
 // kernels.gqa_plan
 std::tuple<int, int, int> gqa_plan(int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t element_bytes,
                                    int64_t max_seq_len) {
-  const int64_t rows = q_len * q_heads / kv_heads, key = 2 * dim * element_bytes, units = batch * div_up(max_seq_len, 64);
+  const int64_t rows = q_len * q_heads / kv_heads, key = 2 * dim * element_bytes, units = batch * div_up(max_seq_len, 32);
   std::tuple<double, int64_t, int64_t, int64_t> best{INFINITY, 1, 1, 16};
   for (int64_t tile = 16; tile <= 64; tile *= 2) {
     if ((tile > 16 && tile / 2 >= rows) || (tile == 64 && dim == 256)) break;
@@ -652,8 +652,8 @@ std::tuple<int, int, int> gqa_plan(int64_t batch, int64_t q_len, int64_t q_heads
       const int64_t groups = kv_heads / heads * row_groups;
       int halvings = 0;
       while (heads < kv_heads && heads * key << halvings < 2048) halvings++;
-      const double stream = (double)(batch * max_seq_len * kv_heads * key) * (1.0 + 0.3 * (double)(row_groups - 1)) / (6.8e6 * (1.0 - 0.05 * halvings));
-      const double step = (double)key * (tile == 16 ? 1.0 : 1.35) / 217.0, more = 6.0 * (double)(tile / 16 - 1);
+      const double stream = (double)(batch * max_seq_len * kv_heads * key) * (1.0 + 0.25 * (double)(row_groups - 1)) / (6.8e6 * (1.0 - 0.05 * halvings));
+      const double step = (double)key * (tile == 16 ? 1.0 : 1.25) / 217.0, more = 5.0 * (double)(tile / 16 - 1);
       const auto walk = [&](int64_t keys) {
         return std::max((double)div_up(keys * heads, 32 * waves) * step, (double)(keys * heads * key) / 26e3);
       };
@@ -661,7 +661,7 @@ std::tuple<int, int, int> gqa_plan(int64_t batch, int64_t q_len, int64_t q_heads
         const int64_t rounds = div_up(batch * groups, slots);
         best = std::min(best, {2.2 + more + std::max(5.6 * (double)(rounds - 1) + (double)rounds * walk(max_seq_len), stream), 0, heads, tile});
       }
-      const int64_t chunks = std::max<int64_t>(1, std::min(units, 256 / groups)), size = div_up(units, chunks) * 64;
+      const int64_t chunks = std::max<int64_t>(1, std::min(units, 256 / groups)), size = div_up(units, chunks) * 32;
       const double joins = 4.0 * std::max(1.0, (double)batch / (double)chunks) * (double)div_up(chunks * groups, 256);
       best = std::min(best, {7.4 + more + std::max(walk(std::min(size, batch * max_seq_len)), stream) + joins, chunks, heads, tile});
     }
@@ -688,7 +688,7 @@ bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, c
   if (!head_scale(k_scale, fp8, hk, dev) || !head_scale(v_scale, fp8, hk, dev) || wants_grad({&q, &k_cache, &v_cache})) return false;
   int64_t longest = block_table.size(1) * k_cache.size(1);
   if (max_seq_len > 0 && c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) longest = std::min(longest, max_seq_len);
-  if (window > 0) longest = std::min(longest, window + q_len + 62);
+  if (window > 0) longest = std::min(longest, window + q_len + 30);
   const auto [by_rule, heads, rows] = gqa_plan(b, q_len, hq, hk, d, k_cache.element_size(), longest);
   const int chunks = num_chunks >= 0 ? (int)num_chunks : by_rule;
   Stream st = stream_of(q);
