@@ -71,6 +71,7 @@ __device__ __forceinline__ uint32_t to_e4m3(const float* x, float s, float inv) 
 template <typename T, int kLanes, bool kFp8, bool kPairs>
 __global__ __launch_bounds__(256) void heads_prologue_kernel(const PrologueParams p) {
   typedef typename Vec4<T>::type V4;
+  typedef T V8 __attribute__((ext_vector_type(8)));
   struct Eight { V4 a, b; };
   const int j = threadIdx.x & (kLanes - 1);
   const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kLanes;
@@ -93,24 +94,26 @@ __global__ __launch_bounds__(256) void heads_prologue_kernel(const PrologueParam
     c = entries(p.cos + pos * p.cs_st, j * 4, p.table_f32);
     s = entries(p.sin + pos * p.cs_st, j * 4, p.table_f32);
   }
-  auto load = [&](const char* at) { return Eight{*(const V4*)(at + a0 * 2), *(const V4*)(at + b0 * 2)}; };
-  auto store8 = [&](char* at, const float* x) {
-    Eight y;
-#pragma unroll
-    for (int e = 0; e < 4; e++) { y.a[e] = (T)x[e]; y.b[e] = (T)x[4 + e]; }
-    *(V4*)(at + a0 * 2) = y.a;
-    *(V4*)(at + b0 * 2) = y.b;
-  };
-  auto store_cache = [&](int i, int h, const float* x) {
-    char* dst = p.cache[i] + at.pg * p.c_sp[i] + at.off * p.c_sr[i] + h * p.c_sh[i];
-    if constexpr (kFp8) {
-      const float sc = p.scale[i] ? p.scale[i][h] : 1.f, inv = 1.f / sc;
-      *(uint32_t*)(dst + a0) = to_e4m3(x, sc, inv);
-      *(uint32_t*)(dst + b0) = to_e4m3(x + 4, sc, inv);
+  auto load = [&](const char* at) {
+    if constexpr (kPairs) {
+      const V8 x = *(const V8*)(at + a0 * 2);
+      return Eight{__builtin_shufflevector(x, x, 0, 1, 2, 3), __builtin_shufflevector(x, x, 4, 5, 6, 7)};
     } else {
-      store8(dst, x);
+      return Eight{*(const V4*)(at + a0 * 2), *(const V4*)(at + b0 * 2)};
     }
   };
+  auto store8 = [&](char* at, const float* x) {
+    V8 y;
+#pragma unroll
+    for (int e = 0; e < 8; e++) y[e] = (T)x[e];
+    if constexpr (kPairs) {
+      *(V8*)(at + a0 * 2) = y;
+    } else {
+      *(V4*)(at + a0 * 2) = __builtin_shufflevector(y, y, 0, 1, 2, 3);
+      *(V4*)(at + b0 * 2) = __builtin_shufflevector(y, y, 4, 5, 6, 7);
+    }
+  };
+  auto cache_row = [&](int i, int h) { return p.cache[i] + at.pg * p.c_sp[i] + at.off * p.c_sr[i] + h * p.c_sh[i]; };
   const float inv_dim = 1.f / (float)p.dim;
   auto turned = [&](const Eight& raw, const char* gamma, const Eight& g, float* x) {
 #pragma unroll
@@ -151,25 +154,50 @@ __global__ __launch_bounds__(256) void heads_prologue_kernel(const PrologueParam
   const int keys = p.q_heads + (store || p.out[1] ? p.kv_heads : 0);
   if (head < keys) {
     const char *gamma = p.gamma[1], *src = p.src[1] + t * p.src_st[1];
-    Eight g{};
+    Eight g{}, next = load(src + (head - p.q_heads) * p.src_sh[1]);
     if (gamma) g = load(gamma);
     for (; head < keys; head += p.parts) {
       const int h = head - p.q_heads;
+      const Eight raw = next;
+      if (head + p.parts < keys) next = load(src + (h + p.parts) * p.src_sh[1]);
       float x[8];
-      turned(load(src + h * p.src_sh[1]), gamma, g, x);
+      turned(raw, gamma, g, x);
       if (!mine) continue;
       if (p.out[1]) store8(p.out[1] + t * p.out_st[1] + h * p.out_sh[1], x);
-      if (store) store_cache(0, h, x);
+      if (!store) continue;
+      char* dst = cache_row(0, h);
+      if constexpr (kFp8) {
+        const float sc = p.scale[0] ? p.scale[0][h] : 1.f, inv = 1.f / sc;
+        const uint32_t lo = to_e4m3(x, sc, inv), hi = to_e4m3(x + 4, sc, inv);
+        if constexpr (kPairs) {
+          *(u32x2*)(dst + a0) = u32x2{lo, hi};
+        } else {
+          *(uint32_t*)(dst + a0) = lo;
+          *(uint32_t*)(dst + b0) = hi;
+        }
+      } else {
+        store8(dst, x);
+      }
     }
   }
-  if (!store) return;
+  if (!store || !mine || head >= keys + p.kv_heads) return;
+  // (values are not turned: eight in a row to a lane)
+  const char* src = p.src[2] + t * p.src_st[2] + j * 16;
+  V8 next = *(const V8*)(src + (head - keys) * p.src_sh[2]);
   for (; head < keys + p.kv_heads; head += p.parts) {
     const int h = head - keys;
-    const Eight raw = load(p.src[2] + t * p.src_st[2] + h * p.src_sh[2]);
-    float x[8];
+    const V8 raw = next;
+    if (head + p.parts < keys + p.kv_heads) next = *(const V8*)(src + (h + p.parts) * p.src_sh[2]);
+    char* dst = cache_row(1, h);
+    if constexpr (kFp8) {
+      float x[8];
 #pragma unroll
-    for (int e = 0; e < 4; e++) { x[e] = (float)raw.a[e]; x[4 + e] = (float)raw.b[e]; }
-    if (mine) store_cache(1, h, x);
+      for (int e = 0; e < 8; e++) x[e] = (float)raw[e];
+      const float sc = p.scale[1] ? p.scale[1][h] : 1.f, inv = 1.f / sc;
+      *(u32x2*)(dst + j * 8) = u32x2{to_e4m3(x, sc, inv), to_e4m3(x + 4, sc, inv)};
+    } else {
+      *(V8*)(dst + j * 16) = raw;
+    }
   }
 }
 
