@@ -260,7 +260,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
       struct Place { int page, row; };
       auto place_of = [&](int key) {                         // (sixteen keys from a multiple of sixteen on: one page)
         const int pi = page_of(key);
-        if (pi - have0 > 63) pages_from(b, pi);
+        if ((uint32_t)(pi - have0) > 63u) pages_from(b, pi);   // (in front of them where a piece is begun again)
         const int pg = __builtin_amdgcn_readlane(have, pi - have0);
         return Place{pg < 0 ? 0 : pg < p.num_pages ? pg : p.num_pages - 1, key - pi * p.page_size};
       };
@@ -751,10 +751,13 @@ extern "C" int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_st
               q_heads, kv_heads, (long long)num_pages, num_chunks, window);
   MLA_REQUIRE(page_size >= 16 && page_size % 16 == 0 && (int64_t)max_blocks * page_size <= 0x7fffff00, MLA_ERR_SHAPE,
               "%s: %d pages of %d tokens a request (pages of a multiple of 16, fewer than 2^31 tokens)", me, max_blocks, page_size);
+  MLA_REQUIRE((int64_t)batch * max_blocks * page_size < (1ll << 35) && num_chunks < (1 << 24), MLA_ERR_SHAPE,
+              "%s: %d requests of up to %lld tokens in %d chunks are more than the plan counts", me, batch, (long long)max_blocks * page_size, num_chunks);
   const int es = cache_dtype == 3 ? 1 : 2, unit = 16 / es;
   const int64_t c_strides = kc_page_stride | kc_row_stride | kc_head_stride | vc_page_stride | vc_row_stride | vc_head_stride;
   MLA_REQUIRE((q_stride_t | q_stride_h) % 8 == 0 && c_strides % unit == 0 && (out_stride_t | out_stride_h) % 4 == 0 &&
                   !(((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) && !((uintptr_t)out & 7) && kc_row_stride >= 0 &&
+                  vc_row_stride >= 0 && kc_row_stride >= 0 &&
                   vc_row_stride >= 0 && kc_row_stride * es * page_size < (1ll << 30) && vc_row_stride * es * page_size < (1ll << 30),
               MLA_ERR_SHAPE, "%s: heads must be 16-byte aligned (results: 8), the rows of a page within 1 GiB", me);
   if (batch == 0 || num_tokens == 0) return MLA_OK;

@@ -268,7 +268,7 @@ extern "C" int mlahip_qk_norm_rope_cache(
   parts = parts < per_wave ? per_wave : parts;
   p.parts = (int)(parts < total ? parts : total);
   const int64_t blocks = (num_tokens * p.parts * lanes + 255) / 256;
-  MLA_REQUIRE(num_tokens * p.parts < (1ll << 32) && blocks < (1ll << 31), MLA_ERR_SHAPE, "%s: too many tokens for one launch", me);
+  MLA_REQUIRE(num_tokens * p.parts < (1ll << 32) - 64 && blocks < (1ll << 31), MLA_ERR_SHAPE, "%s: too many tokens for one launch", me);
 #define HEADS_LAUNCH(L)                                                                  \
   if (dtype == 0) heads::launch<__bf16, L>(p, fp8, interleaved != 0, (unsigned)blocks, stream); \
   else heads::launch<_Float16, L>(p, fp8, interleaved != 0, (unsigned)blocks, stream)

@@ -144,6 +144,62 @@ def test_what_lies_in_masked_places_does_not_matter(dev, bad, q_len, window, fp8
             assert not torch.isfinite(got[~old].float()).all()
 
 
+@pytest.mark.parametrize("chunks,heads", [(0, 1), (0, 2), (3, 2)])
+def test_a_long_piece_is_begun_again_from_its_first_page(dev, chunks, heads):
+    """More pages than a wavefront holds numbers of, and an infinity that the newest token alone sees."""
+    c = make(dev, [9000, 4000], q_len=2, hq=6, hk=2, page=16, seed=13)
+    kw = dict(num_chunks=chunks, heads_per_group=heads)
+    ref, ref_lse = call(dev, c, 2, **kw)
+    check(c, ref, ref_lse)
+    for b, n in enumerate(c["lens"].tolist()):
+        c["v"][c["table"][b, (n - 1) // 16], (n - 1) % 16] = float("inf")
+    got, lse = call(dev, c, 2, **kw)
+    assert torch.equal(got[0::2], ref[0::2]) and torch.equal(lse, ref_lse) and torch.isinf(got[1::2].float()).all()
+
+
+def test_first_call_of_a_kernel_under_capture(dev):
+    """A graph may be captured from a shape that has not run before."""
+    from omni_npu_amd import kernels as K
+    c = make(dev, [500, 90], q_len=5, hq=26, hk=2, d=64, dtype=torch.float16, fp8=True, seed=14)
+    on = {n: c[n].to(dev) for n in ("q", "k", "v", "table", "lens", "k_scale", "v_scale")}
+    out = torch.zeros_like(on["q"])
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        K._workspace(dev, 1 << 26, "gqa")
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            K.gqa_decode(on["q"], on["k"], on["v"], on["table"], on["lens"], c["scale"], out, q_len=5, k_scale=on["k_scale"],
+                         v_scale=on["v_scale"], rows_per_group=64)
+        for _ in range(2):
+            out.fill_(float("nan"))
+            graph.replay()
+            torch.cuda.synchronize()
+            ref, _ = call(dev, c, 5, rows_per_group=64, num_chunks=0)
+            o, _, weight, reach = H.gqa(c["q"], c["k"].float(), c["v"].float(), c["table"], c["lens"], c["scale"], c["start"], 0, c["k_scale"],
+                                        c["v_scale"])
+            tol = H.gqa_tolerance(o, weight, reach, c["dtype"], 64)
+            assert ((out.cpu().double() - o).abs() <= tol).all() and ((ref.double() - o).abs() <= tol).all()
+    torch.cuda.current_stream().wait_stream(side)
+
+
+@pytest.mark.parametrize("rows", [16, 32, 64])
+@pytest.mark.parametrize("heads", [1, 2, 4, 8])
+@pytest.mark.parametrize("d,fp8", [(64, False), (64, True), (128, False), (128, True), (256, False), (256, True)])
+def test_every_form_of_a_workgroup(dev, rows, heads, d, fp8):
+    """Heads and rows of a workgroup as a caller asks for them: the same attention; what does not fit is refused."""
+    from omni_npu_amd import _lib
+    c = make(dev, [300, 47, 900], q_len=3, hq=88, hk=8, d=d, fp8=fp8, page=32, seed=rows + heads)
+    waves = 4 if d == 256 or rows == 64 or rows == 32 and d == 128 and not fp8 else 8
+    kw = dict(num_chunks=5, heads_per_group=heads, rows_per_group=rows)
+    if heads > waves or rows == 64 and d == 256:
+        with pytest.raises(_lib.MlaHipError, match="to a workgroup"):
+            call(dev, c, 3, **kw)
+        return
+    check(c, *call(dev, c, 3, **kw))
+    check(c, *call(dev, c, 3, **dict(kw, num_chunks=0)))
+
+
 def test_scores_that_outgrow_each_other(dev):
     """Keys of growing length: a row's reference is replaced again and again; and queries so large that one key takes everything."""
     c = make(dev, [1500, 700], hq=4, hk=2, seed=9)
