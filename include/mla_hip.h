@@ -560,7 +560,8 @@ int dsa_sparse_decode_heads_bf16(const void* q_nope, int64_t qn_stride_t, int64_
  * (i, i + rotary_dim / 2), 1: (2i, 2i + 1); the result is laid out as the input), all in fp32 and rounded once; queries to q_out
  * (may be q), keys and values to the cache row slot_mapping[t] (negative or past the cache: not written), rotated keys to k_out too
  * where it is not NULL (may be k).  Caches of the inputs' type, or e4m3 (code 3): x / k_scale[head], x / v_scale[head] (NULL: 1),
- * values beyond +-448 become +-448.  A token whose position is not in the tables is not written anywhere.  kv_heads = 0: queries
+ * values beyond +-448 become +-448.  A token whose position is not in the tables is not written anywhere.  A cache row that two tokens
+ * name holds one's or the other's values head by head: name it once.  Scales are positive normal numbers.  kv_heads = 0: queries
  * alone; without caches (all three pointers NULL) v is not read.  dim and rotary_dim: multiples of 16 up to 256. */
 int mlahip_qk_norm_rope_cache(
     const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t, int64_t k_stride_h, const void* v,
@@ -576,11 +577,15 @@ int mlahip_qk_norm_rope_cache(
  * [query_start_loc[b], query_start_loc[b + 1])) sees keys j <= seq_lens[b] - s + i, and with window > 0 only j > that - window.
  * q [num_tokens, q_heads, dim] (bf16 or fp16), caches of its type or e4m3 (times k_scale / v_scale [kv_heads] fp32, NULL: 1), query
  * head h with key head h / (q_heads / kv_heads), dim 64, 128 or 256, pages of a multiple of 16 tokens.  out as q through its
- * strides; lse_out fp32 [num_tokens, q_heads] or NULL: log of the sum of exp(scores).  A row that sees no key gives zeros and -inf.
+ * strides; lse_out fp32 [num_tokens, q_heads] or NULL: log of the sum of exp(scores).  A row that sees no key, or
+ * none with a score above -inf, gives zeros and -inf; what lies in keys and values that a row does not see (pages' free rows, other tokens' keys) does
+ * not reach it, infinities and NaN included.  Rows of q behind the last request, or of a request's tokens beyond max_q_len, are left as they
+ * were.  A request has room for at most 2^30 tokens (max_blocks * page_size).
  * seq_lens beyond the block table's room count as that room; page numbers outside the cache are read as its first or last page.
  * num_chunks > 0: the keys of all requests, end to end, are cut into that many equal pieces, a workgroup each (times groups of
  * heads and rows), and a second launch joins the pieces of a request, with mlahip_gqa_decode_workspace_bytes of workspace;
- * 0: one launch, a request to a workgroup, no workspace.  rows_per_group: rows (tokens x query heads of a key head) of a workgroup, 16, 32
+ * 0: one launch, a request to a workgroup, no workspace.  Calls that may run at once (on two streams, or in two graphs that are replayed
+ * side by side) need a workspace each.  rows_per_group: rows (tokens x query heads of a key head) of a workgroup, 16, 32
  * or, of heads of up to 128, 64: the more, the fewer times keys are read.  heads_per_group: key heads of a workgroup, a power of two that
  * divides kv_heads, up to its wavefronts (8; 4 for dim 256 and for 64 rows): the fewer, the more wavefronts share a head's keys. */
 size_t mlahip_gqa_decode_workspace_bytes(int32_t batch, int32_t max_q_len, int32_t q_heads, int32_t dim, int32_t num_chunks);

@@ -86,7 +86,7 @@ __device__ __forceinline__ Seq seq_from(const Params& p, int len, int q0, int q1
   x.q0 = q0;
   x.s = q1 - q0;
   x.s = x.s < 0 ? 0 : x.s < p.max_q_len ? x.s : p.max_q_len;
-  const int room = p.max_blocks * p.page_size;               // (host: below 2^31)
+  const int room = p.max_blocks * p.page_size;               // (host: at most 2^30)
   x.len = len < 0 ? 0 : len < room ? len : room;
   x.first = 0;
   if (p.window > 0) {
@@ -749,15 +749,14 @@ extern "C" int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_st
                   num_tokens >= 0 && num_chunks >= 0 && window >= 0 && max_blocks >= 1 && bt_stride >= max_blocks && (int64_t)max_q_len * q_heads < (1 << 24),
               MLA_ERR_SHAPE, "%s: batch %d, %d tokens each, %d query and %d key heads, %lld pages, %d chunks, window %d", me, batch, max_q_len,
               q_heads, kv_heads, (long long)num_pages, num_chunks, window);
-  MLA_REQUIRE(page_size >= 16 && page_size % 16 == 0 && (int64_t)max_blocks * page_size <= 0x7fffff00, MLA_ERR_SHAPE,
-              "%s: %d pages of %d tokens a request (pages of a multiple of 16, fewer than 2^31 tokens)", me, max_blocks, page_size);
+  MLA_REQUIRE(page_size >= 16 && page_size % 16 == 0 && (int64_t)max_blocks * page_size <= (1 << 30), MLA_ERR_SHAPE,
+              "%s: %d pages of %d tokens a request (pages of a multiple of 16, at most 2^30 tokens)", me, max_blocks, page_size);
   MLA_REQUIRE((int64_t)batch * max_blocks * page_size < (1ll << 35) && num_chunks < (1 << 24), MLA_ERR_SHAPE,
               "%s: %d requests of up to %lld tokens in %d chunks are more than the plan counts", me, batch, (long long)max_blocks * page_size, num_chunks);
   const int es = cache_dtype == 3 ? 1 : 2, unit = 16 / es;
   const int64_t c_strides = kc_page_stride | kc_row_stride | kc_head_stride | vc_page_stride | vc_row_stride | vc_head_stride;
   MLA_REQUIRE((q_stride_t | q_stride_h) % 8 == 0 && c_strides % unit == 0 && (out_stride_t | out_stride_h) % 4 == 0 &&
                   !(((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15) && !((uintptr_t)out & 7) && kc_row_stride >= 0 &&
-                  vc_row_stride >= 0 && kc_row_stride >= 0 &&
                   vc_row_stride >= 0 && kc_row_stride * es * page_size < (1ll << 30) && vc_row_stride * es * page_size < (1ll << 30),
               MLA_ERR_SHAPE, "%s: heads must be 16-byte aligned (results: 8), the rows of a page within 1 GiB", me);
   if (batch == 0 || num_tokens == 0) return MLA_OK;
@@ -774,7 +773,8 @@ extern "C" int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_st
   p.num_tokens = num_tokens; p.num_pages = (int32_t)(num_pages < 0x7fffffff ? num_pages : 0x7fffffff);
   p.page_shift = (page_size & (page_size - 1)) == 0 ? __builtin_ctz(page_size) : -1;
   p.page_size = page_size; p.batch = batch; p.max_q_len = max_q_len; p.kv_heads = kv_heads; p.group = q_heads / kv_heads;
-  p.window = window; p.num_chunks = num_chunks;
+  // (a window that no request outgrows is none; below it, window and tokens together stay within 32 bits)
+  p.window = window < max_blocks * page_size ? window : 0; p.num_chunks = num_chunks;
   p.scale_log2 = scale * kLog2e;
   p.out = (char*)out; p.o_st = out_stride_t * 2; p.o_sh = out_stride_h * 2; p.lse = lse_out;
   if (num_chunks > 0) {

@@ -670,16 +670,22 @@ std::tuple<int, int, int> gqa_plan(int64_t batch, int64_t q_len, int64_t q_heads
 }
 
 // kernels.gqa_decode
+using OptInt = std::optional<int64_t>;
 bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& seq_lens, double scale,
-                const Tensor& out, int64_t q_len, const OptTensor& qsl, int64_t window, const OptTensor& k_scale, const OptTensor& v_scale,
-                const OptTensor& lse, int64_t num_chunks, int64_t max_seq_len, const OptTensor& workspace, int64_t heads_per_group, int64_t rows_per_group) {
-  if (!current_gpu(q) || q.dim() != 3 || workspace || k_cache.dim() != 4 || num_chunks > (1 << 16)) return false;
+                const Tensor& out, int64_t q_len, const OptTensor& qsl, OptInt window_keys, const OptTensor& k_scale, const OptTensor& v_scale,
+                const OptTensor& lse, OptInt num_chunks, OptInt max_seq_len, const OptTensor& workspace, OptInt heads_per_group, OptInt rows_per_group) {
+  if (!current_gpu(q) || q.dim() != 3 || workspace || k_cache.dim() != 4) return false;
+  const int64_t window = std::min<int64_t>(window_keys.value_or(0), 0x7fffffff);
+  auto off = [](OptInt x, int64_t lo, int64_t hi) { return x && (*x < lo || *x > hi); };
+  if (q_len > (1 << 24) || off(window_keys, 1, INT64_MAX) || off(num_chunks, 0, 1 << 16) || off(max_seq_len, 1, INT64_MAX) || off(heads_per_group, 1, 8) ||
+      off(rows_per_group, 1, 64))
+    return false;
   const at::Device dev = q.device();
   const at::ScalarType dt = q.scalar_type();
   const int64_t t = q.size(0), hq = q.size(1), d = q.size(2), hk = k_cache.size(2), b = seq_lens.numel();
   if ((dt != at::kBFloat16 && dt != at::kHalf) || t < 1 || q.stride(2) != 1 || !heads_of(out, t, hq, d, dt, dev) || hk < 1 || hq < 1 || hq % hk ||
       !head_cache(k_cache, hk, d, dt, dev) || !head_cache(v_cache, hk, d, dt, dev) || k_cache.sizes() != v_cache.sizes() ||
-      k_cache.scalar_type() != v_cache.scalar_type() || q_len < 1 || window < 0 || !is_i32(seq_lens, 1, dev) || !seq_lens.is_contiguous() ||
+      k_cache.scalar_type() != v_cache.scalar_type() || q_len < 1 || !is_i32(seq_lens, 1, dev) || !seq_lens.is_contiguous() ||
       !is_i32(block_table, 2, dev) || block_table.size(0) < b || block_table.size(1) < 1 || b < 1 ||
       (qsl ? !(is_i32(*qsl, 1, dev) && qsl->is_contiguous() && qsl->numel() == b + 1) : t != b * q_len) ||
       (lse && !(lse->scalar_type() == at::kFloat && lse->dim() == 2 && lse->size(0) == t && lse->size(1) == hq && lse->is_contiguous() && lse->device() == dev)))
@@ -687,10 +693,10 @@ bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, c
   const bool fp8 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
   if (!head_scale(k_scale, fp8, hk, dev) || !head_scale(v_scale, fp8, hk, dev) || wants_grad({&q, &k_cache, &v_cache})) return false;
   int64_t longest = block_table.size(1) * k_cache.size(1);
-  if (max_seq_len > 0 && c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) longest = std::min(longest, max_seq_len);
+  if (max_seq_len && c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) longest = std::min(longest, *max_seq_len);
   if (window > 0) longest = std::min(longest, window + q_len + 30);
   const auto [by_rule, heads, rows] = gqa_plan(b, q_len, hq, hk, d, k_cache.element_size(), longest);
-  const int chunks = num_chunks >= 0 ? (int)num_chunks : by_rule;
+  const int chunks = (int)num_chunks.value_or(by_rule);
   Stream st = stream_of(q);
   const int64_t need = (int64_t)mlahip_gqa_decode_workspace_bytes((int)b, (int)q_len, (int)hq, (int)d, chunks);
   Tensor* ws = need ? &scratch(q, st, need, 3) : nullptr;
@@ -700,8 +706,8 @@ bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, c
                           (const int32_t*)seq_lens.data_ptr(), (const int32_t*)data_of(qsl), (int)b, (int)q_len, (int)hq, (int)hk, (int)d,
                           type_code(dt), type_code(k_cache.scalar_type()), (const float*)data_of(k_scale), (const float*)data_of(v_scale),
                           (float)scale, (int)window, out.data_ptr(), out.stride(0), out.stride(1), (float*)data_of(lse),
-                          ws ? ws->data_ptr() : nullptr, ws ? (size_t)ws->numel() : 0, chunks, heads_per_group > 0 ? (int)heads_per_group : heads,
-                                rows_per_group > 0 ? (int)rows_per_group : rows, st),
+                          ws ? ws->data_ptr() : nullptr, ws ? (size_t)ws->numel() : 0, chunks, (int)heads_per_group.value_or(heads),
+                          (int)rows_per_group.value_or(rows), st),
               "mlahip_gqa_decode");
 }
 

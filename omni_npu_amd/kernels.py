@@ -1434,7 +1434,7 @@ def qk_norm_rope_cache(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[t
     slot_mapping[t] of ``k_cache`` / ``v_cache`` [pages, page, Hk, D] of the inputs' type or float8_e4m3fn (x / k_scale[h],
     x / v_scale[h], fp32 [Hk], saturated); negative slots and slots past the cache are skipped.  Rotated keys go to ``k_out`` too
     where it is given (default without a cache: in place); ``k=None`` rotates queries alone.  A token whose position is not in
-    the tables is not written anywhere."""
+    the tables is not written anywhere.  A slot is for one token: named by two, it holds either's heads."""
     what = "qk_norm_rope_cache"
     if _host.load().qk_norm_rope_cache(q, k, v, cos, sin, positions, slot_mapping, k_cache, v_cache, q_gamma, k_gamma, eps, interleaved,
                                        q_out, k_out, k_scale, v_scale):
@@ -1540,13 +1540,13 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
     h // (Hq // Hk).  block_table int32 [B,maxblk], seq_lens int32 [B] on the device, the newest tokens included.  Sequence b owns
     query tokens [b*q_len, (b+1)*q_len), or with query_start_loc (int32 [B+1], device) those, at most q_len of them; token i of s
     sees keys [0, L - s + i], with ``window`` only the newest ``window`` of these.  ``out`` [T,Hq,D] like q; ``lse_out`` fp32
-    [T,Hq].  A row without keys gives zeros and -inf.  ``max_seq_len``: no request is longer (it shapes the launch; results are right
-    without); under capture the table's room counts, as a graph is replayed over others."""
+    [T,Hq].  A row without keys gives zeros and -inf; rows behind the last request stay as they were.  ``max_seq_len``: no request is
+    longer (it shapes the launch; results are right without); under capture the table's room counts, as a graph is replayed over
+    others.  Scratch memory is kept per stream: graphs captured on one stream share it and are replayed one after the other, or get a
+    ``workspace`` each (mlahip_gqa_decode_workspace_bytes)."""
     what = "gqa_decode"
     if _host.load().gqa_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out, q_len, query_start_loc,
-                               0 if window is None else window or -1, k_scale, v_scale, lse_out,
-                               -1 if num_chunks is None else num_chunks, max_seq_len or 0, workspace,
-                               heads_per_group or 0, rows_per_group or 0):
+                               window, k_scale, v_scale, lse_out, num_chunks, max_seq_len, workspace, heads_per_group, rows_per_group):
         return out
     dev = _one_device(what, q, k_cache, v_cache, block_table, seq_lens, out, query_start_loc, k_scale, v_scale, lse_out, workspace)
     _no_grad(what, q, k_cache, v_cache)
@@ -1564,8 +1564,13 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
         raise ValueError(f"{what}: {hq} query heads over {hk} key heads")
     if window is not None and window < 1:
         raise ValueError(f"{what}: a window of {window} keys")
-    if q_len < 1:
+    if not 1 <= q_len <= 1 << 24:
         raise ValueError(f"{what}: q_len {q_len}")
+    for name, x, most in (("num_chunks", num_chunks, 1 << 24), ("heads_per_group", heads_per_group, 8), ("rows_per_group", rows_per_group, 64)):
+        if x is not None and not 0 <= x <= most:
+            raise ValueError(f"{what}: {name} {x}")
+    if max_seq_len is not None and max_seq_len < 1:
+        raise ValueError(f"{what}: max_seq_len {max_seq_len}")
     b = seq_lens.numel()
     if seq_lens.dtype != torch.int32 or not seq_lens.is_contiguous() or block_table.dtype != torch.int32 or block_table.dim() != 2 or \
             block_table.shape[0] < b or block_table.shape[1] < 1 or block_table.stride(1) != 1 and block_table.shape[1] > 1:
@@ -1583,7 +1588,7 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
     lib = _lib.load()
     with torch.cuda.device(dev):
         longest = block_table.shape[1] * k_cache.shape[1]
-        if max_seq_len and not torch.cuda.is_current_stream_capturing():
+        if max_seq_len is not None and not torch.cuda.is_current_stream_capturing():
             longest = min(longest, max_seq_len)
         if window is not None:
             longest = min(longest, window + q_len + 30)
@@ -1597,9 +1602,9 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
             q.data_ptr(), q.stride(0), q.stride(1), t, k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(), *v_cache.stride()[:3],
             k_cache.shape[0], k_cache.shape[1], block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
             query_start_loc.data_ptr() if query_start_loc is not None else None, b, q_len, hq, hk, d, _HEAD_DT[q.dtype], code, *scales,
-            float(scale), window or 0, out.data_ptr(), out.stride(0), out.stride(1), lse_out.data_ptr() if lse_out is not None else None,
+            float(scale), min(window or 0, 0x7fffffff), out.data_ptr(), out.stride(0), out.stride(1), lse_out.data_ptr() if lse_out is not None else None,
             ws.data_ptr() if ws is not None else None, ws.numel() * ws.element_size() if ws is not None else 0, num_chunks,
-            heads_per_group or heads, rows_per_group or rows, _stream(q))
+            heads if heads_per_group is None else heads_per_group, rows if rows_per_group is None else rows_per_group, _stream(q))
     _lib.check(rc, "mlahip_gqa_decode")
     return out
 

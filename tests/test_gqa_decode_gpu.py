@@ -98,6 +98,65 @@ def test_windows(dev, window, q_len, d, page):
     check(c, *call(dev, c, q_len, window=window), window=window)
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 40, 1024])
+def test_a_window_wider_than_any_request(dev, window):
+    """No window then, with requests of fewer keys than tokens too."""
+    c = make(dev, [300, 2, 1, 64], q_len=5, hq=8, hk=4, seed=30)
+    ref, ref_lse = call(dev, c, 5)
+    check(c, ref, ref_lse)
+    got, lse = call(dev, c, 5, window=window)
+    assert torch.equal(got, ref) and torch.equal(lse, ref_lse)
+
+
+@pytest.mark.parametrize("chunks", [0, 6])
+def test_infinite_and_undefined_scores(dev, chunks):
+    """Scores of -inf weigh nothing wherever they come; one of +inf or NaN makes its row undefined, and no other row."""
+    c = make(dev, [400, 130], hq=4, hk=2, d=64, page=16, seed=31)
+    c["q"][...] = c["q"].abs() + 0.5
+    page = lambda b, key: (c["table"][b, key // 16], key % 16)
+    plain, plain_lse = call(dev, c, 1, num_chunks=chunks)
+    check(c, plain, plain_lse)
+    gone = [0, 1, *range(32, 64), 200, 399]                  # (a whole step of keys among them)
+    kept = torch.tensor([i for i in range(400) if i not in gone])
+    few = dict(c, table=torch.arange(26, dtype=torch.int32)[None], lens=torch.tensor([len(kept)], dtype=torch.int32), q=c["q"][:1],
+               start=torch.tensor([0, 1]))
+    for n in ("k", "v"):                                     # the request without them
+        rows = c[n][c["table"][0].long()[kept // 16], kept % 16]
+        few[n] = torch.cat([rows, torch.zeros(416 - len(kept), 2, 64, dtype=rows.dtype)]).view(26, 16, 2, 64)
+    for key in gone:
+        c["k"][page(0, key)][0] = -float("inf")
+    ref, ref_lse = call(dev, c, 1, num_chunks=chunks)
+    o, l, weight, reach = H.gqa(few["q"], few["k"], few["v"], few["table"], few["lens"], few["scale"], few["start"])
+    assert ((ref[0, :2].double() - o[0, :2]).abs() <= H.gqa_tolerance(o, weight, reach, c["dtype"], 64)[0, :2]).all()
+    assert torch.equal(ref[0, 2:], plain[0, 2:]) and torch.equal(ref[1], plain[1]) and torch.equal(ref_lse[1], plain_lse[1])
+    for bad in (float("inf"), float("nan")):
+        was = c["k"][page(0, 150)][1, 3].clone()
+        c["k"][page(0, 150)][1, 3] = bad
+        out, lse = call(dev, c, 1, num_chunks=chunks)
+        c["k"][page(0, 150)][1, 3] = was
+        assert torch.isnan(out[0, 2:].float()).all() and torch.isnan(lse[0, 2:]).all()
+        out[0, 2:], lse[0, 2:] = ref[0, 2:], ref_lse[0, 2:]
+        assert torch.equal(out, ref) and torch.equal(lse, ref_lse)
+    q = c["q"].clone()
+    c["q"][1, 0, 5] = float("nan")
+    out, lse = call(dev, c, 1, num_chunks=chunks)
+    assert torch.isnan(out[1, 0].float()).all() and torch.isnan(lse[1, 0])
+    c["q"] = q
+    out[1, 0], lse[1, 0] = ref[1, 0], ref_lse[1, 0]
+    assert torch.equal(out, ref) and torch.equal(lse, ref_lse)
+    c["k"][c["table"][1].long()[:9], :, 0] = -float("inf")    # every score of a row
+    out, lse = call(dev, c, 1, num_chunks=chunks)
+    assert (out[1, :2] == 0).all() and (lse[1, :2] == -float("inf")).all() and torch.equal(out[1, 2:], ref[1, 2:])
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 3.0])
+@pytest.mark.parametrize("fp8", [False, True], ids=["same", "e4m3"])
+def test_scales_of_any_sign(dev, scale, fp8):
+    c = make(dev, [500, 33], q_len=2, hq=6, hk=2, d=128, fp8=fp8, seed=32)
+    c["scale"] = scale
+    check(c, *call(dev, c, 2))
+
+
 def test_ragged_token_counts(dev):
     c = make(dev, [300, 40, 7, 0, 129], q_lens=[1, 4, 0, 2, 3], hq=12, hk=4, seed=3)
     for chunks in (None, 0, 9):
@@ -324,6 +383,11 @@ def test_refusals(dev):
     refused(ValueError, "query heads", {0: on["q"][:, :7], 6: torch.empty_like(on["q"][:, :7])})
     refused(ValueError, "window", {}, window=0)
     refused(ValueError, "q_len", {}, q_len=0)
+    refused(ValueError, "q_len", {}, q_len=(1 << 32) + 1, query_start_loc=torch.zeros(3, dtype=torch.int32, device=dev))
+    for name in ("num_chunks", "heads_per_group", "rows_per_group", "max_seq_len"):
+        refused(ValueError, name, {}, **{name: -1})
+        if name != "max_seq_len":
+            refused(ValueError, name, {}, **{name: 1 << 32})
     refused(ValueError, "query tokens", {}, q_len=2)
     refused(ValueError, "seq_lens", {4: on["lens"].long()})
     refused(ValueError, "block_table", {3: on["table"][:1]})
