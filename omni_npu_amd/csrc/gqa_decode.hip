@@ -135,7 +135,7 @@ template <typename T, int D, bool kFp8, int MT> struct Shape {
   static constexpr int ops = kFp8 ? 2 : 1;                   // operands of one transposed read
   static constexpr int join_b = 16 * D * 4, tile_b = kTile * row_b;
   static constexpr int wave_b = join_b > tile_b ? join_b : tile_b;
-  static constexpr int stat_floats = waves * (2 * 16 + 1);
+  static constexpr int stat_floats = waves * 2 * 16 * MT + 8 + waves * 16 * MT * 2;   // references, sums, flags, results' addresses
   static constexpr int lds_b = waves * wave_b + stat_floats * 4;
   // position of granule c of a key's row in LDS: c ^ swz(key), so that rows written and read together hit different banks
   static __device__ __forceinline__ int swz(int key) {
@@ -156,7 +156,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
   typedef Shape<T, D, kFp8, MT> Sh;
   typedef Types<T> Ty;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
-  float* stats = (float*)(lds + Sh::waves * Sh::wave_b);     // [wave][16] references, then sums; [wave] a piece has to be done again
+  float* stats = (float*)(lds + Sh::waves * Sh::wave_b);     // [wave][row] references, then sums; [wave] a piece has to be done again
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int l16 = lane & 15, g = lane >> 4;
   int hg = blockIdx.y, rg = 0;
@@ -481,106 +481,164 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
         }
       }
 
-      // ---- join of the wavefronts of a head, a row tile at a time, and the rows' results ----
+      // ---- join of the wavefronts of a head ----
       const bool several = only < 0 && tok_first != tok_last, again = several && __builtin_amdgcn_ballot_w64(odd != 0) != 0;
       bool by_token = false;
       const ParamsPtr last = reload();
       int tid = threadIdx.x;                                 // (hidden: the addresses below are not worked out, and kept, in front of the loop)
       asm volatile("" : "+v"(tid));
       const int jl = tid & 63, j16 = jl & 15, jg = jl >> 4;
-#pragma unroll 1
-      for (int m = 0; m < MT; m++) {
-        // granule position in a row: granule ^ row, so that sixteen rows' writes at one granule hit different banks.  Granule:
-        // four dims as the accumulator has them (8 bits: every other one of eight)
+      constexpr int kRows = 16 * MT, kGran = D / 4, kThreads = Sh::waves * 64;
+      float *refs = stats, *sums = refs + Sh::waves * kRows, *flags = sums + Sh::waves * kRows;
+      int64_t* places = (int64_t*)(flags + 8);               // [row][head]
+      const int rows_here = rows - row0 < kRows ? rows - row0 : kRows;
+      if (jl < 16) {
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+          refs[wave * kRows + m * 16 + jl] = m_ref[m];
+          sums[wave * kRows + m * 16 + jl] = sum[m][0];
+        }
+        if (jl == 0) flags[wave] = again ? 1.f : 0.f;
+      }
+      // Sixteen rows' sums go through LDS at a time.  Granule position in a row: granule ^ row, so that sixteen rows' writes at one granule
+      // hit different banks.  Granule: four dims as the accumulator has them (8 bits: every other one of eight)
+      auto put = [&](const f32x4 (&a)[D / 16]) {
         char* to = mine_lds + j16 * (D * 4);
 #pragma unroll
-        for (int k = 0; k < MT; k++) {
-          if (k != m) continue;
+        for (int d = 0; d < D / 16; d++) *(f32x4*)(to + (((d * 4 + jg) ^ j16) << 4)) = a[d];
+      };
+      if constexpr (MT == 1) put(acc[0]);
+      lds_barrier();
+      if (several) {
+        for (int k = 0; k < Sh::waves; k++) by_token |= flags[k] != 0.f;
+      }
+      // What is a row's, by kWs wavefronts of a head: their weights, and where the result goes (0: nowhere).
+      auto row_of = [&](auto kWs, int h, int rr, bool first_dims, float* wt) {
+        constexpr int kw_n = decltype(kWs)::value;
+        const int r = row0 + rr, hd = (hg << p.heads_shift) + h;
+        float part[kw_n], most = -INFINITY, total = 0.f;
 #pragma unroll
-          for (int d = 0; d < D / 16; d++) *(f32x4*)(to + (((d * 4 + jg) ^ j16) << 4)) = acc[k][d];
-          if (jl < 16) {
-            stats[wave * 16 + jl] = m_ref[k];
-            stats[(Sh::waves + wave) * 16 + jl] = sum[k][0];
+        for (int k = 0; k < kw_n; k++) {
+          const int w = (k << p.heads_shift) + h;
+          wt[k] = refs[w * kRows + rr];
+          part[k] = sums[w * kRows + rr];
+        }
+#pragma unroll
+        for (int k = 0; k < kw_n; k++) most = fmaxf(most, wt[k]);
+        const float base = most == -INFINITY ? 0.f : most;
+#pragma unroll
+        for (int k = 0; k < kw_n; k++) {
+          wt[k] = fast_exp2(wt[k] - base);                   // (a wavefront without keys for the row has zeros and weighs nothing)
+          total += wt[k] * part[k];
+        }
+        const float vs = kFp8 && last->v_scale ? last->v_scale[hd] : 1.f;
+        const float inv = total == 0.f ? 0.f : vs / total;
+#pragma unroll
+        for (int k = 0; k < kw_n; k++) wt[k] *= inv;
+        const int tk = p.max_q_len == 1 ? 0 : (int)((uint32_t)r / (uint32_t)p.group), qh = hd * p.group + (r - tk * p.group);
+        const int64_t t = (int64_t)sq.q0 + tk;
+        if ((only >= 0 && tk != only) || (whole && (t < 0 || t >= last->num_tokens))) return (char*)nullptr;
+        const float lse = total == 0.f ? -INFINITY : (most + fast_log2(total)) * kLn2;
+        if (whole) {
+          if (last->lse && first_dims) last->lse[t * (p.kv_heads * p.group) + qh] = lse;
+          return last->out + t * last->o_st + (int64_t)qh * last->o_sh;
+        }
+        const int64_t slot = ((int64_t)(blockIdx.x + b) * p.kv_heads + hd) * (p.max_q_len * p.group) + r;
+        if (first_dims) last->part_lse[slot] = lse;
+        return (char*)(last->part_acc + slot * D);
+      };
+      // Four dims of a row.  Granule gi = 4 d + g'
+      const int gi = tid & (kGran - 1), dim = kFp8 ? (gi >> 3) * 32 + (gi & 3) * 8 + ((gi >> 2) & 1) : gi * 4;
+      auto from = [&](int k, int h, int r16) {
+        return *(const f32x4*)(lds + ((k << p.heads_shift) + h) * Sh::wave_b + r16 * (D * 4) + ((gi ^ r16) << 4));
+      };
+      auto add = [&](auto kWs, const f32x4* a, const float* wt, char* place) {
+        f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < decltype(kWs)::value; k++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[e] += wt[k] * a[k][e];
+        if (!place) return;
+        if (whole) {
+          T* dst = (T*)place + dim;
+          if constexpr (kFp8) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) dst[2 * e] = (T)o[e];
+          } else {
+            typename Ty::v4 y;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = (T)o[e];
+            *(typename Ty::v4*)dst = y;
+          }
+        } else {
+          float* dst = (float*)place + dim;
+          if constexpr (kFp8) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) dst[2 * e] = o[e];
+          } else {
+            *(f32x4*)dst = o;
           }
         }
-        if (m == 0 && jl == 0) stats[Sh::waves * 32 + wave] = again ? 1.f : 0.f;
+      };
+      auto by_waves = [&](auto f) {
+        if (kws == 1) f(std::integral_constant<int, 1>{});
+        else if (kws == 2) f(std::integral_constant<int, 2>{});
+        else if (Sh::waves == 4 || kws == 4) f(std::integral_constant<int, 4>{});
+        else f(std::integral_constant<int, 8>{});
+      };
+      const int of_row = tid / kGran, heads_of = 1 << p.heads_shift;
+      if (by_token) {
+        lds_barrier();                                       // (the flags have been read)
+      } else if (MT == 1 && rows_here * heads_of <= kThreads / kGran) {
+        // Few enough for a granule to a thread: each works its row's weights out by itself.  (1 x 64 keys x 4/1 heads of 128 5.1 us, by a row to
+        // a thread first 5.8; the other way round, 1 x 26 keys x 64/4 heads of 256, four heads to a workgroup, 13.6 and 10.6.)
+        by_waves([&](auto n) {
+          const int h = of_row & (heads_of - 1), r16 = of_row >> p.heads_shift;
+          float wt[decltype(n)::value];
+          f32x4 a[decltype(n)::value];
+          if (r16 >= rows_here) return;
+#pragma unroll
+          for (int k = 0; k < decltype(n)::value; k++) a[k] = from(k, h, r16);
+          add(n, a, wt, row_of(n, h, r16, gi == 0, wt));
+        });
         lds_barrier();
-        if (m == 0 && several) {
-          bool any = false;
-          for (int k = 0; k < Sh::waves; k++) any |= stats[Sh::waves * 32 + k] != 0.f;
-          by_token = any;
-        }
-        if (by_token) { lds_barrier(); continue; }
-        constexpr int kGran = D / 4;
-        const int row_m = row0 + m * 16, there = rows - row_m < 16 ? rows - row_m : 16;   // rows of the tile
-        // kWs: wavefronts of a head
-        auto join = [&](auto kWs) {
-          constexpr int kw_n = decltype(kWs)::value;
-          const int items = (16 * kGran) << p.heads_shift;
-          for (int it = tid; it < items; it += Sh::waves * 64) {
-            const int gi = it & (kGran - 1), r16 = (it / kGran) & 15, h = it / (kGran * 16);
-            const int r = row_m + r16, hd = (hg << p.heads_shift) + h;
-            if (r16 >= there || (only >= 0 && (int)((uint32_t)r / (uint32_t)p.group) != only)) continue;
-            float ref[kw_n], part[kw_n], most = -INFINITY, total = 0.f;
-            f32x4 a[kw_n], o = {0.f, 0.f, 0.f, 0.f};
+      } else {
+        // first what is a row's, a row to a thread (a thousand clocks of one instruction after the other), then the sums
+        by_waves([&](auto n) {
+          for (int it = tid; it < rows_here * heads_of; it += kThreads) {
+            const int h = it & (heads_of - 1), rr = it >> p.heads_shift;
+            float wt[decltype(n)::value];
+            places[it] = (int64_t)row_of(n, h, rr, true, wt);
 #pragma unroll
-            for (int k = 0; k < kw_n; k++) {
-              const int w = (k << p.heads_shift) + h;
-              ref[k] = stats[w * 16 + r16];
-              part[k] = stats[(Sh::waves + w) * 16 + r16];
-              a[k] = *(const f32x4*)(lds + w * Sh::wave_b + r16 * (D * 4) + ((gi ^ r16) << 4));
-            }
-#pragma unroll
-            for (int k = 0; k < kw_n; k++) most = fmaxf(most, ref[k]);
-            const float base = most == -INFINITY ? 0.f : most;
-#pragma unroll
-            for (int k = 0; k < kw_n; k++) {
-              const float wt = fast_exp2(ref[k] - base);     // (a wavefront without keys for the row has zeros and weighs nothing)
-              total += wt * part[k];
-#pragma unroll
-              for (int e = 0; e < 4; e++) o[e] += wt * a[k][e];
-            }
-            const float vs = kFp8 && last->v_scale ? last->v_scale[hd] : 1.f;
-            const float inv = total == 0.f ? 0.f : vs / total;
-#pragma unroll
-            for (int e = 0; e < 4; e++) o[e] *= inv;
-            const float lse = total == 0.f ? -INFINITY : (most + fast_log2(total)) * kLn2;
-            // dims of the granule: gi = 4 d + g'
-            const int dim = kFp8 ? (gi >> 3) * 32 + (gi & 3) * 8 + ((gi >> 2) & 1) : gi * 4;
-            if (whole) {
-              const int tk = p.max_q_len == 1 ? 0 : (int)((uint32_t)r / (uint32_t)p.group);
-              const int64_t t = (int64_t)sq.q0 + tk;
-              if (t < 0 || t >= last->num_tokens) continue;
-              const int qh = hd * p.group + (r - tk * p.group);
-              T* dst = (T*)(last->out + t * last->o_st + (int64_t)qh * last->o_sh) + dim;
-              if constexpr (kFp8) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) dst[2 * e] = (T)o[e];
-              } else {
-                typename Ty::v4 y;
-#pragma unroll
-                for (int e = 0; e < 4; e++) y[e] = (T)o[e];
-                *(typename Ty::v4*)dst = y;
-              }
-              if (last->lse && gi == 0) last->lse[t * (p.kv_heads * p.group) + qh] = lse;
-            } else {
-              const int64_t slot = ((int64_t)(blockIdx.x + b) * p.kv_heads + hd) * (p.max_q_len * p.group) + r;
-              float* dst = last->part_acc + slot * D + dim;
-              if constexpr (kFp8) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) dst[2 * e] = o[e];
-              } else {
-                *(f32x4*)dst = o;
-              }
-              if (gi == 0) last->part_lse[slot] = lse;
-            }
+            for (int k = 0; k < decltype(n)::value; k++) refs[((k << p.heads_shift) + h) * kRows + rr] = wt[k];
           }
-        };
-        if (kws == 1) join(std::integral_constant<int, 1>{});
-        else if (kws == 2) join(std::integral_constant<int, 2>{});
-        else if (Sh::waves == 4 || kws == 4) join(std::integral_constant<int, 4>{});
-        else join(std::integral_constant<int, 8>{});
-        lds_barrier();
+        });
+#pragma unroll 1
+        for (int m = 0; m < MT; m++) {
+          if (m * 16 >= rows_here) break;
+          if constexpr (MT > 1) {
+#pragma unroll
+            for (int k = 0; k < MT; k++)
+              if (k == m) put(acc[k]);
+          }
+          lds_barrier();
+          const int there = rows_here - m * 16 < 16 ? rows_here - m * 16 : 16;
+          by_waves([&](auto n) {
+#pragma unroll 2
+            for (int it = of_row; it < there * heads_of; it += kThreads / kGran) {
+              const int h = it & (heads_of - 1), r16 = it >> p.heads_shift;
+              float wt[decltype(n)::value];
+              f32x4 a[decltype(n)::value];
+#pragma unroll
+              for (int k = 0; k < decltype(n)::value; k++) {
+                wt[k] = refs[((k << p.heads_shift) + h) * kRows + m * 16 + r16];
+                a[k] = from(k, h, r16);
+              }
+              add(n, a, wt, (char*)places[m * 16 * heads_of + it]);
+            }
+          });
+          lds_barrier();
+        }
       }
       if (by_token) only = tok_first;
       else if (only < 0 || ++only > tok_last) break;
