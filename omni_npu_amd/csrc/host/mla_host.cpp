@@ -652,18 +652,19 @@ std::tuple<int, int, int> gqa_plan(int64_t batch, int64_t q_len, int64_t q_heads
       const int64_t groups = kv_heads / heads * row_groups;
       int halvings = 0;
       while (heads < kv_heads && heads * key << halvings < 2048) halvings++;
-      const double stream = (double)(batch * max_seq_len * kv_heads * key) * (1.0 + 0.25 * (double)(row_groups - 1)) / (6.8e6 * (1.0 - 0.05 * halvings));
-      const double step = (double)key * (tile == 16 ? 1.0 : 1.25) / 217.0, more = 5.0 * (double)(tile / 16 - 1);
+      const double stream = (double)(batch * max_seq_len * kv_heads * key) * (1.0 + 0.25 * (double)(row_groups - 1)) / (7.1e6 * (1.0 - 0.05 * halvings));
+      const double step = (double)key * (tile == 16 ? 1.0 : 1.15) / 237.0, more = 1.8 * (double)(tile / 16 - 1);
       const auto walk = [&](int64_t keys) {
-        return std::max((double)div_up(keys * heads, 32 * waves) * step, (double)(keys * heads * key) / 26e3);
+        return std::max((double)div_up(keys * heads, 32 * waves) * step, (double)(keys * heads * key) / 31e3);
       };
       if (max_seq_len <= 2048) {
         const int64_t rounds = div_up(batch * groups, slots);
-        best = std::min(best, {2.2 + more + std::max(5.6 * (double)(rounds - 1) + (double)rounds * walk(max_seq_len), stream), 0, heads, tile});
+        best = std::min(best, {3.0 + more + std::max(6.0 * (double)(rounds - 1) + (double)rounds * walk(max_seq_len), stream), 0, heads, tile});
       }
       const int64_t chunks = std::max<int64_t>(1, std::min(units, 256 / groups)), size = div_up(units, chunks) * 32;
-      const double joins = 4.0 * std::max(1.0, (double)batch / (double)chunks) * (double)div_up(chunks * groups, 256);
-      best = std::min(best, {7.4 + more + std::max(walk(std::min(size, batch * max_seq_len)), stream) + joins, chunks, heads, tile});
+      const double parts = std::min(1.0 + (double)chunks / (double)batch, (double)chunks) * (double)(batch * q_len * q_heads * dim) / 1e6;
+      const double joins = 3.5 * std::max(1.0, (double)batch / (double)chunks) * (double)div_up(chunks * groups, 256);
+      best = std::min(best, {6.8 + more + parts + std::max(walk(std::min(size, batch * max_seq_len)), stream) + joins, chunks, heads, tile});
     }
   }
   return {(int)std::get<1>(best), (int)std::get<2>(best), (int)std::get<3>(best)};

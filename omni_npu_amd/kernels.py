@@ -1488,15 +1488,16 @@ def qk_norm_rope_cache(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[t
 
 def gqa_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, dim: int, element_bytes: int, max_seq_len: int):
     """(pieces that gqa_decode cuts the cached keys of a step into, key heads of a workgroup, rows of a workgroup); 0 pieces: a request to a
-    workgroup, one launch.  The fastest by an estimate in us of what was measured (12 500 launches, 1-128 requests of 64-20 000 keys, heads
-    of 64-256 values, 1-8 of them, 1-64 rows; the estimate's choice is 1.5 % slower than the best one on average):
-    a wavefront's step of 32 keys x 512 bytes takes 2.4, a quarter more with more than 16 rows, and a CU takes 26 KB per us from the memory (short contexts
-    are bound by these: few heads to a workgroup, so that its wavefronts share their keys, and few rows, each workgroup reading the keys
-    again); the cache stream 6.8 MB per us, 5 % less for each halving of a key's heads of a workgroup below 2 KB, a quarter longer for each
-    further group of rows; 2.2 for one launch, 5.6 for each further round of workgroups, 7.4 for two launches, 4 for each piece of a sequence in a chunk, 5 for
-    each further 16 rows of a workgroup.  us, one launch / cut, 32/8 heads of 128: 1 x 256 keys 8.7 / 10.8, 1 x 1024 16.8 / 10.8, 32 x 1024 26.8 / 28.8, 128 x 64
-    10.9 / 14.6; workgroups of 1 / 8 heads, 32 x 8 heads of 64 x 10 000 keys 122 / 72; of 16 / 64 rows, 3 tokens x 48/3 heads of 128, 1 x 2000 keys 11.1 / 15.6, 128 x
-    6000 347 / 161.  Beyond 2048 keys a request to a workgroup loses up to two thirds where lengths are ragged, which the host does not know."""
+    workgroup, one launch.  The fastest by an estimate in us of what was measured (13 200 launches, 1-128 requests of 64-20 000 keys, heads
+    of 64-256 values, 1-8 of them, 1-64 rows; the estimate's choice is 1.1 % slower than the best one on average, 31 % at worst):
+    a wavefront's step of 32 keys x 512 bytes takes 2.2, 15 % more with more than 16 rows, and a CU takes 31 KB per us from the memory (short
+    contexts are bound by these: few heads to a workgroup, so that its wavefronts share their keys, and few rows, each workgroup reading the
+    keys again); the cache stream 7.1 MB per us, 5 % less for each halving of a key's heads of a workgroup below 2 KB, a quarter longer for each
+    further group of rows; 3 for one launch, 6 for each further round of workgroups, 6.8 for two launches, 3.5 for each piece of a sequence in a
+    chunk, 1 for a million values of partial results, 1.8 for each further 16 rows of a workgroup.  us, one launch / cut, 32/8 heads of 128:
+    1 x 300 keys 9.3 / 9.6, 1 x 1200 18.9 / 10.0, 32 x 300 10.5 / 13.4, 32 x 1200 30.4 / 32.3; workgroups of 1 / 8 heads, 32 x 8 heads of 64 x
+    10 000 keys 125 / 103; of 16 / 64 rows, 3 tokens x 48/3 heads of 128, 1 x 2000 keys 11.7 / 15.2, 128 x 6000 347 / 166.  Beyond 2048 keys a request to a
+    workgroup loses up to two thirds where lengths are ragged, which the host does not know."""
     rows = q_len * q_heads // kv_heads
     key = 2 * dim * element_bytes
     units = batch * -(-max_seq_len // 32)
@@ -1513,16 +1514,17 @@ def gqa_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, dim: int, elem
             halvings = 0
             while heads < kv_heads and heads * key << halvings < 2048:
                 halvings += 1
-            stream = batch * max_seq_len * kv_heads * key * (1.0 + 0.25 * (row_groups - 1)) / (6.8e6 * (1.0 - 0.05 * halvings))
-            step, more = key * (1.0 if tile == 16 else 1.25) / 217.0, 5.0 * (tile // 16 - 1)
-            walk = lambda keys: max(-(-keys * heads // (32 * waves)) * step, keys * heads * key / 26e3)
+            stream = batch * max_seq_len * kv_heads * key * (1.0 + 0.25 * (row_groups - 1)) / (7.1e6 * (1.0 - 0.05 * halvings))
+            step, more = key * (1.0 if tile == 16 else 1.15) / 237.0, 1.8 * (tile // 16 - 1)
+            walk = lambda keys: max(-(-keys * heads // (32 * waves)) * step, keys * heads * key / 31e3)
             if max_seq_len <= 2048:
                 rounds = -(-batch * groups // slots)
-                best = min(best, (2.2 + more + max(5.6 * (rounds - 1) + rounds * walk(max_seq_len), stream), 0, heads, tile))
+                best = min(best, (3.0 + more + max(6.0 * (rounds - 1) + rounds * walk(max_seq_len), stream), 0, heads, tile))
             chunks = max(1, min(units, 256 // groups))
             size = -(-units // chunks) * 32
-            joins = 4.0 * max(1.0, batch / chunks) * -(-chunks * groups // 256)
-            best = min(best, (7.4 + more + max(walk(min(size, batch * max_seq_len)), stream) + joins, chunks, heads, tile))
+            parts = min(1.0 + chunks / batch, float(chunks)) * (batch * q_len * q_heads * dim) / 1e6
+            joins = 3.5 * max(1.0, batch / chunks) * -(-chunks * groups // 256)
+            best = min(best, (6.8 + more + parts + max(walk(min(size, batch * max_seq_len)), stream) + joins, chunks, heads, tile))
             heads *= 2
     return best[1:]
 
