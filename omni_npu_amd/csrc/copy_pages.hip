@@ -18,6 +18,9 @@
 namespace mlahip {
 namespace pages {
 
+// (an address that comes as numbers is said to be in global memory: flat accesses wait for the LDS as well)
+#define GLOBAL __attribute__((address_space(1)))
+
 struct Cache { char* base; int64_t page_stride; uint32_t row_bytes, row_stride; };
 // caches, then sources and destinations, then filled rows (a launch takes as many of either as fit)
 constexpr int kArgBytes = 3840;
@@ -53,27 +56,27 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(const Params p) {
   const uint32_t rows = p.part ? pairs[2 * p.num_pairs + pair] : (uint32_t)p.page_size;
   const uint32_t row_units = c.row_bytes / sizeof(V), units = rows * row_units;
   const uint32_t begin = blockIdx.x * (uint32_t)p.piece, end = begin + p.piece < units ? begin + p.piece : units;
-  const char* src = c.base + (int64_t)(int32_t)pairs[2 * pair] * c.page_stride;
-  char* dst = c.base + (int64_t)(int32_t)pairs[2 * pair + 1] * c.page_stride;
+  const GLOBAL char* src = (const GLOBAL char*)c.base + (int64_t)(int32_t)pairs[2 * pair] * c.page_stride;
+  GLOBAL char* dst = (GLOBAL char*)c.base + (int64_t)(int32_t)pairs[2 * pair + 1] * c.page_stride;
   if (c.row_bytes == c.row_stride) {
     // (four loads on their way together: the compiler does not move one ahead of a store that might touch its bytes)
     uint32_t i = begin + threadIdx.x;
     for (; i + 768 < end; i += 1024) {
       V v[4];
 #pragma unroll
-      for (int k = 0; k < 4; k++) v[k] = kNt ? __builtin_nontemporal_load((const V*)src + i + k * 256) : ((const V*)src)[i + k * 256];
+      for (int k = 0; k < 4; k++) v[k] = kNt ? __builtin_nontemporal_load((const GLOBAL V*)src + i + k * 256) : ((const GLOBAL V*)src)[i + k * 256];
 #pragma unroll
       for (int k = 0; k < 4; k++) {
-        if constexpr (kNt) __builtin_nontemporal_store(v[k], (V*)dst + i + k * 256);
-        else ((V*)dst)[i + k * 256] = v[k];
+        if constexpr (kNt) __builtin_nontemporal_store(v[k], (GLOBAL V*)dst + i + k * 256);
+        else ((GLOBAL V*)dst)[i + k * 256] = v[k];
       }
     }
-    for (; i < end; i += 256) ((V*)dst)[i] = ((const V*)src)[i];
+    for (; i < end; i += 256) ((GLOBAL V*)dst)[i] = ((const GLOBAL V*)src)[i];
   } else {
     for (uint32_t i = begin + threadIdx.x; i < end; i += 256) {
       const uint32_t r = i / row_units;
       const uint64_t at = (uint64_t)r * c.row_stride + (i - r * row_units) * (uint32_t)sizeof(V);
-      *(V*)(dst + at) = *(const V*)(src + at);
+      *(GLOBAL V*)(dst + at) = *(const GLOBAL V*)(src + at);
     }
   }
 }

@@ -143,6 +143,8 @@ template <typename T, int D, bool kFp8, int MT> struct Shape {
   }
 };
 
+// (a pointer out of arguments loaded so is said to be in global memory: flat accesses wait for the LDS as well)
+#define GLOBAL __attribute__((address_space(1)))
 // The arguments again, to be loaded here: what a piece's begin and end take would hold scalar registers throughout its loop.
 typedef const __attribute__((address_space(4))) Params* ParamsPtr;
 __device__ __forceinline__ ParamsPtr reload() {
@@ -241,7 +243,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
       v_cur = v_seq < v_end ? v_seq : v_end;
       whole = u0 == 0 && u1 == sq.units;
       if (blockIdx.y == 0 && threadIdx.x == 0) {
-        int32_t* ids = reload()->seg_ids + 2 * b;
+        GLOBAL int32_t* ids = (GLOBAL int32_t*)reload()->seg_ids + 2 * b;
         if (u0 == 0) ids[0] = whole ? -1 : (int)blockIdx.x + b;
         if (u1 == sq.units && !whole) ids[1] = (int)blockIdx.x + b;
       }
@@ -304,12 +306,12 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
         tok[m] = p.max_q_len == 1 ? 0 : (int)((uint32_t)rr / (uint32_t)p.group);
         const int64_t t = (int64_t)sq.q0 + tok[m];
         const bool ok = there && t >= 0 && t < first->num_tokens;
-        const char* src = first->q + (ok ? t : 0) * first->q_st + (int64_t)(head * p.group + (rr - tok[m] * p.group)) * first->q_sh;
+        const GLOBAL char* src = (const GLOBAL char*)first->q + (ok ? t : 0) * first->q_st + (int64_t)(head * p.group + (rr - tok[m] * p.group)) * first->q_sh;
 #pragma unroll
         for (int s = 0; s < D / 32; s++) {
           // (an 8-bit key's granule of 16 dims is two steps' operands)
           const int dim = kFp8 ? (s >> 1) * 64 + g * 16 + (s & 1) * 8 : s * 32 + g * 8;
-          qf[m][s] = ok ? *(const u32x4*)(src + dim * 2) : u32x4{0u, 0u, 0u, 0u};
+          qf[m][s] = ok ? *(const GLOBAL u32x4*)(src + dim * 2) : u32x4{0u, 0u, 0u, 0u};
         }
         hi[m] = sq.len - sq.s + tok[m] + 1;
         lo[m] = p.window > 0 ? hi[m] - p.window : 0;
@@ -326,7 +328,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
       const int t0 = only < 0 ? tok_first : only, t1 = only < 0 ? tok_last : only;
       const int all_hi = key_0 + t0, any_hi = key_0 + t1, all_lo = p.window > 0 ? any_hi - p.window : 0, any_lo = p.window > 0 ? all_hi - p.window : 0;
       uint32_t odd = 0;
-      const float scale_log2 = first->scale_log2 * (kFp8 && first->k_scale ? first->k_scale[head] : 1.f);
+      const float scale_log2 = first->scale_log2 * (kFp8 && first->k_scale ? ((const GLOBAL float*)first->k_scale)[head] : 1.f);
 
       f32x4 acc[MT][D / 16], sum[MT];                        // sum: of the probabilities, by a product with ones
       float m_ref[MT];
@@ -531,7 +533,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
           wt[k] = fast_exp2(wt[k] - base);                   // (a wavefront without keys for the row has zeros and weighs nothing)
           total += wt[k] * part[k];
         }
-        const float vs = kFp8 && last->v_scale ? last->v_scale[hd] : 1.f;
+        const float vs = kFp8 && last->v_scale ? ((const GLOBAL float*)last->v_scale)[hd] : 1.f;
         const float inv = total == 0.f ? 0.f : vs / total;
 #pragma unroll
         for (int k = 0; k < kw_n; k++) wt[k] *= inv;
@@ -540,11 +542,11 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
         if ((only >= 0 && tk != only) || (whole && (t < 0 || t >= last->num_tokens))) return (char*)nullptr;
         const float lse = total == 0.f ? -INFINITY : (most + fast_log2(total)) * kLn2;
         if (whole) {
-          if (last->lse && first_dims) last->lse[t * (p.kv_heads * p.group) + qh] = lse;
+          if (last->lse && first_dims) ((GLOBAL float*)last->lse)[t * (p.kv_heads * p.group) + qh] = lse;
           return last->out + t * last->o_st + (int64_t)qh * last->o_sh;
         }
         const int64_t slot = ((int64_t)(blockIdx.x + b) * p.kv_heads + hd) * (p.max_q_len * p.group) + r;
-        if (first_dims) last->part_lse[slot] = lse;
+        if (first_dims) ((GLOBAL float*)last->part_lse)[slot] = lse;
         return (char*)(last->part_acc + slot * D);
       };
       // Four dims of a row.  Granule gi = 4 d + g'
@@ -560,7 +562,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
           for (int e = 0; e < 4; e++) o[e] += wt[k] * a[k][e];
         if (!place) return;
         if (whole) {
-          T* dst = (T*)place + dim;
+          GLOBAL T* dst = (GLOBAL T*)place + dim;
           if constexpr (kFp8) {
 #pragma unroll
             for (int e = 0; e < 4; e++) dst[2 * e] = (T)o[e];
@@ -568,15 +570,15 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
             typename Ty::v4 y;
 #pragma unroll
             for (int e = 0; e < 4; e++) y[e] = (T)o[e];
-            *(typename Ty::v4*)dst = y;
+            *(GLOBAL typename Ty::v4*)dst = y;
           }
         } else {
-          float* dst = (float*)place + dim;
+          GLOBAL float* dst = (GLOBAL float*)place + dim;
           if constexpr (kFp8) {
 #pragma unroll
             for (int e = 0; e < 4; e++) dst[2 * e] = o[e];
           } else {
-            *(f32x4*)dst = o;
+            *(GLOBAL f32x4*)dst = o;
           }
         }
       };
