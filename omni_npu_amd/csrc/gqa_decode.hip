@@ -168,11 +168,26 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
   const int row0 = rg * 16 * MT;
   char* mine_lds = lds + wave * Sh::wave_b;
 
+  // page numbers of the wavefront's next 64 pages, one to a lane; where the request is known, its first ones, before its length is
+  int have0 = 0, have = 0;
+  auto pages_from = [&](int b, int pi) {
+    const int at = pi + lane;
+    have0 = pi;
+    have = p.block_table[(int64_t)b * p.bt_stride + (at < p.max_blocks ? at : p.max_blocks - 1)];
+  };
+
   // ---- which units are mine ----
   int v_cur = 0, v_end = 0, b = blockIdx.x, v_seq = 0;
   Seq lane_seq{};
-  const bool in_lanes = p.num_chunks > 0 && p.batch <= 64;    // a lane keeps a sequence
-  if (p.num_chunks > 0) {
+  const bool in_lanes = p.num_chunks > 0 && p.batch <= 64 && p.batch > 1;    // a lane keeps a sequence
+  if (p.num_chunks > 0 && p.batch == 1) {                    // (nothing to look for)
+    pages_from(0, 0);
+    const int tot = seq_at(p, 0).units, size = __builtin_amdgcn_readfirstlane(chunk_units(tot, p.num_chunks));
+    v_cur = blockIdx.x * size;
+    v_end = v_cur + size < tot ? v_cur + size : tot;
+    if (v_cur >= tot) return;
+    b = 0;
+  } else if (p.num_chunks > 0) {
     int ends = 0, tot = 0;
     if (in_lanes) {
       if (lane < p.batch) lane_seq = seq_of(p, lane);
@@ -216,13 +231,6 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
     }
   }
 
-  // page numbers of the wavefront's next 64 pages, one to a lane; a request to a workgroup: its first ones, before its length is known
-  int have0 = 0, have = 0;
-  auto pages_from = [&](int b, int pi) {
-    const int at = pi + lane;
-    have0 = pi;
-    have = p.block_table[(int64_t)b * p.bt_stride + (at < p.max_blocks ? at : p.max_blocks - 1)];
-  };
   if (p.num_chunks == 0) pages_from(b, 0);
   do {
     if (b >= p.batch) break;
@@ -293,7 +301,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
             vr[s * (Sh::v_loads / 2) + n] = load_nt(from, v_off, (at[s].row + n * Sh::keys_per_load) * p.v_sr);
         }
       };
-      if (mine > 0 && (p.num_chunks > 0 || p.window > 0)) pages_from(b, page_of(key0 + kw * kTile));
+      if (mine > 0 && (p.num_chunks == 0 ? p.window > 0 : p.batch > 1)) pages_from(b, page_of(key0 + kw * kTile));
 
       // ---- the query: row l16 of each row tile, eight dims a step; zeros in rows that do not exist ----
       u32x4 qf[MT][D / 32];

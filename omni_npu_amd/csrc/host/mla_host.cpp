@@ -661,7 +661,8 @@ std::tuple<int, int, int> gqa_plan(int64_t batch, int64_t q_len, int64_t q_heads
         const int64_t rounds = div_up(batch * groups, slots);
         best = std::min(best, {3.0 + more + std::max(6.0 * (double)(rounds - 1) + (double)rounds * walk(max_seq_len), stream), 0, heads, tile});
       }
-      const int64_t chunks = std::max<int64_t>(1, std::min(units, 256 / groups)), size = div_up(units, chunks) * 32;
+      const int64_t most = batch == 1 ? std::max<int64_t>(std::min<int64_t>(units, 32), div_up(units, 2)) : units;
+      const int64_t chunks = std::max<int64_t>(1, std::min(most, 256 / groups)), size = div_up(units, chunks) * 32;
       const double parts = std::min(1.0 + (double)chunks / (double)batch, (double)chunks) * (double)(batch * q_len * q_heads * dim) / 1e6;
       const double joins = 3.5 * std::max(1.0, (double)batch / (double)chunks) * (double)div_up(chunks * groups, 256);
       best = std::min(best, {6.8 + more + parts + std::max(walk(std::min(size, batch * max_seq_len)), stream) + joins, chunks, heads, tile});

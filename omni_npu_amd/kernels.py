@@ -1496,8 +1496,10 @@ def gqa_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, dim: int, elem
     further group of rows; 3 for one launch, 6 for each further round of workgroups, 6.8 for two launches, 3.5 for each piece of a sequence in a
     chunk, 1 for a million values of partial results, 1.8 for each further 16 rows of a workgroup.  us, one launch / cut, 32/8 heads of 128:
     1 x 300 keys 9.3 / 9.6, 1 x 1200 18.9 / 10.0, 32 x 300 10.5 / 13.4, 32 x 1200 30.4 / 32.3; workgroups of 1 / 8 heads, 32 x 8 heads of 64 x
-    10 000 keys 125 / 103; of 16 / 64 rows, 3 tokens x 48/3 heads of 128, 1 x 2000 keys 11.7 / 15.2, 128 x 6000 347 / 166.  Beyond 2048 keys a request to a
-    workgroup loses up to two thirds where lengths are ragged, which the host does not know."""
+    10 000 keys 125 / 103; of 16 / 64 rows, 3 tokens x 48/3 heads of 128, 1 x 2000 keys 11.7 / 15.2, 128 x 6000 347 / 166.  A request of its
+    own has more than 32 pieces only of two steps or more, as they are joined one after the other: 4/1 heads of 128, 5000 keys, 157 / 79
+    pieces 11.3 / 9.9.  Beyond 2048 keys a request to a workgroup loses up to two thirds where lengths are ragged, which the host does not
+    know."""
     rows = q_len * q_heads // kv_heads
     key = 2 * dim * element_bytes
     units = batch * -(-max_seq_len // 32)
@@ -1520,7 +1522,7 @@ def gqa_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, dim: int, elem
             if max_seq_len <= 2048:
                 rounds = -(-batch * groups // slots)
                 best = min(best, (3.0 + more + max(6.0 * (rounds - 1) + rounds * walk(max_seq_len), stream), 0, heads, tile))
-            chunks = max(1, min(units, 256 // groups))
+            chunks = max(1, min(max(min(units, 32), -(-units // 2)) if batch == 1 else units, 256 // groups))
             size = -(-units // chunks) * 32
             parts = min(1.0 + chunks / batch, float(chunks)) * (batch * q_len * q_heads * dim) / 1e6
             joins = 3.5 * max(1.0, batch / chunks) * -(-chunks * groups // 256)
