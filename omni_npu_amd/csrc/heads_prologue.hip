@@ -10,7 +10,13 @@
 //
 // A group of 8, 16 or 32 lanes holds a head, four pairs a lane (of half pairs its values are four in either half, so that both of a pair
 // are the lane's own); the norm's sum goes by lane moves.  A group takes several heads of one token, so that the token's table entries
-// and the gains are read once.  What bounds it is memory: every value is read and written once.
+// and the gains are read once, and asks for the next head's values before it turns this one's; few tokens get more groups, so that the CUs
+// have work.
+//
+// What bounds it is memory, every value read and written once: 16 384 tokens x 64 + 2 x 8 heads of 128 into the 8-bit cache (646 MB) take
+// 136 us, 4.75 TB/s (a copy of 2 GiB on this card: 4.94).  2999 tokens x 16 + 2 x 4 heads of 64 (19 MB) take 6.6 us, and 1 token 2.7, 64 tokens 2.8 in
+// a graph, which is a launch and three dependent reads (slot and position, table row, values).  Without the next head's values on their
+// way 10 786 tokens x 8 + 2 x 8 heads of 256 took 72 us in place of 53.
 #include <type_traits>
 
 #include "cache_rows.hpp"
@@ -72,7 +78,7 @@ template <typename T, int kLanes, bool kFp8, bool kPairs>
 __global__ __launch_bounds__(256) void heads_prologue_kernel(const PrologueParams p) {
   typedef typename Vec4<T>::type V4;
   typedef T V8 __attribute__((ext_vector_type(8)));
-  struct Eight { V4 a, b; };
+  struct Eight { V4 a, b; };                                 // (filled by parts: as 16 bytes the compiler keeps it in LDS, three times the time)
   const int j = threadIdx.x & (kLanes - 1);
   const int64_t group = ((int64_t)blockIdx.x * 256 + threadIdx.x) / kLanes;
   const uint32_t t32 = (uint32_t)group / (uint32_t)p.parts;  // (host: fewer than 2^32 groups)
