@@ -203,6 +203,44 @@ def test_more_pages_than_a_wavefront_holds_numbers_of(dev, chunks, d, page):
     check(c, *call(dev, c, 2, num_chunks=chunks))
 
 
+@pytest.mark.parametrize("chunks", [None, 1, 2, 9, 200])
+@pytest.mark.parametrize("n,q_len,window", [(1, 1, None), (33, 2, None), (2100, 1, None), (2100, 3, None), (5000, 1, 40), (5000, 2, 1500), (0, 1, None)])
+def test_one_request_in_pieces(dev, chunks, n, q_len, window):
+    c = make(dev, [n], q_len=q_len, hq=6, hk=2, d=64, page=16, seed=n)
+    check(c, *call(dev, c, q_len, window=window, num_chunks=chunks), window=window)
+
+
+@pytest.mark.parametrize("chunks", [None, 0, 5])
+def test_many_tokens(dev, chunks):
+    """A prompt's tokens behind a context, and a request that is only a prompt: many groups of rows."""
+    c = make(dev, [500, 301, 77], q_lens=[150, 301, 1], hq=6, hk=2, d=64, page=16, seed=41)
+    check(c, *call(dev, c, 301, varlen=True, num_chunks=chunks))
+    check(c, *call(dev, c, 301, varlen=True, num_chunks=chunks, window=130), window=130)
+
+
+@pytest.mark.parametrize("fp8", [False, True], ids=["same", "e4m3"])
+def test_views_of_wider_tensors(dev, fp8):
+    """Queries as a view of the projection's result, results into a wider tensor, rows of a wider block table: nothing beside them is touched."""
+    from omni_npu_amd import kernels as K
+    c = make(dev, [300, 77, 640], q_len=2, hq=12, hk=4, d=128, fp8=fp8, page=64, seed=42)
+    ref, ref_lse = call(dev, c, 2)
+    check(c, ref, ref_lse)
+    on = {n: None if c[n] is None else c[n].to(dev) for n in ("q", "k", "v", "table", "lens", "k_scale", "v_scale")}
+    wide_q = torch.full((6, 12 + 8, 128), float("nan"), dtype=c["dtype"], device=dev)
+    wide_q[:, :12] = on["q"]
+    wide_out = torch.full((6, 2, 14, 128), 7.0, dtype=c["dtype"], device=dev)
+    table = torch.full((5, on["table"].shape[1] + 9), -3, dtype=torch.int32, device=dev)
+    table[:3, :on["table"].shape[1]] = on["table"]
+    for chunks in (None, 0, 6):
+        wide_out.fill_(7.0)
+        K.gqa_decode(wide_q[:, :12], on["k"], on["v"], table[:, :on["table"].shape[1]], on["lens"], c["scale"], wide_out[:, 1, 1:13], q_len=2,
+                     k_scale=on["k_scale"], v_scale=on["v_scale"], num_chunks=chunks)
+        got = wide_out.cpu()
+        check(c, got[:, 1, 1:13], ref_lse)
+        got[:, 1, 1:13] = 7.0
+        assert (got == 7.0).all()
+
+
 @pytest.mark.parametrize("kind", ["bf16", "e4m3"])
 def test_offsets_beyond_32_bits(dev, kind):
     """Caches of more than 2^32 elements: the pages in use lie at both ends."""
