@@ -268,11 +268,13 @@ extern "C" int mlahip_qk_norm_rope_cache(
   p.q_heads = q_heads; p.kv_heads = kv_heads; p.dim = dim; p.rotary = rotary_dim; p.table_f32 = table_dtype == 1;
   p.eps = eps;
   const int lanes = dim <= 64 ? 8 : dim <= 128 ? 16 : 32;
-  // groups to a token: a wavefront's lanes are full, and few tokens get more groups so that the CUs have work
-  const int total = q_heads + (has_k ? kv_heads : 0) + (cached ? kv_heads : 0), per_wave = 64 / lanes;
-  int64_t parts = (16384 + num_tokens - 1) / num_tokens;
-  parts = parts < per_wave ? per_wave : parts;
-  p.parts = (int)(parts < total ? parts : total);
+  // Groups to a token: a power of two, so that tokens do not straddle workgroups, with three to five heads each; a group to a head where
+  // that leaves CUs without work.  us by heads of a group, 1 / 2 / 3 / 5 / 10 / 20: 16 384 tokens x 80 heads of 128 171 / 132 / 131 / 120 / 126 /
+  // 136, 6000 x 48 39 / 34 / 32 / 34 / 35 / 35, 300 x 80 5.2 / 5.3 / 6.1 / 6.0 / 7.5 / 10.7, 200 x 48 3.7 / 4.0 / 4.2 / 5.1 / 6.7 / 8.5.
+  const int total = q_heads + (has_k ? kv_heads : 0) + (cached ? kv_heads : 0);
+  p.parts = 1;
+  while (p.parts * 6 <= total) p.parts *= 2;
+  if (num_tokens * p.parts < 8192) p.parts = total;
   const int64_t blocks = (num_tokens * p.parts * lanes + 255) / 256;
   MLA_REQUIRE(num_tokens * p.parts < (1ll << 32) - 64 && blocks < (1ll << 31), MLA_ERR_SHAPE, "%s: too many tokens for one launch", me);
 #define HEADS_LAUNCH(L)                                                                  \
