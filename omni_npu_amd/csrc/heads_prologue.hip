@@ -14,9 +14,10 @@
 // have work.
 //
 // What bounds it is memory, every value read and written once: 16 384 tokens x 64 + 2 x 8 heads of 128 into the 8-bit cache (646 MB) take
-// 136 us, 4.75 TB/s (a copy of 2 GiB on this card: 4.94).  2999 tokens x 16 + 2 x 4 heads of 64 (19 MB) take 6.6 us, and 1 token 2.7, 64 tokens 2.8 in
+// 120 us, 5.4 TB/s (a copy of 2 GiB on this card: 4.94).  2999 tokens x 16 + 2 x 4 heads of 64 (19 MB) take 6.6 us, and 1 token 2.7, 64 tokens 2.8 in
 // a graph, which is a launch and three dependent reads (slot and position, table row, values).  Without the next head's values on their
-// way 10 786 tokens x 8 + 2 x 8 heads of 256 took 72 us in place of 53.
+// way 10 786 tokens x 8 + 2 x 8 heads of 256 took 72 us in place of 53; with the first key and value head of a group asked for in front of its queries
+// (80 registers in place of 60) 16 384 x 32 + 2 x 8 of 128 took 81 in place of 78.
 #include <type_traits>
 
 #include "cache_rows.hpp"
@@ -268,13 +269,17 @@ extern "C" int mlahip_qk_norm_rope_cache(
   p.q_heads = q_heads; p.kv_heads = kv_heads; p.dim = dim; p.rotary = rotary_dim; p.table_f32 = table_dtype == 1;
   p.eps = eps;
   const int lanes = dim <= 64 ? 8 : dim <= 128 ? 16 : 32;
-  // Groups to a token: a power of two, so that tokens do not straddle workgroups, with three to five heads each; a group to a head where
-  // that leaves CUs without work.  us by heads of a group, 1 / 2 / 3 / 5 / 10 / 20: 16 384 tokens x 80 heads of 128 171 / 132 / 131 / 120 / 126 /
-  // 136, 6000 x 48 39 / 34 / 32 / 34 / 35 / 35, 300 x 80 5.2 / 5.3 / 6.1 / 6.0 / 7.5 / 10.7, 200 x 48 3.7 / 4.0 / 4.2 / 5.1 / 6.7 / 8.5.
+  // Groups to a token: a power of two, so that tokens do not straddle workgroups, with four to seven heads each, or three; a group to a head
+  // where that leaves CUs without work.  us by heads of a group, 1 / 2 / 3 / 4 / 5 / 6 / 10 / 20: 16 384 tokens x 80 heads of 128 into the 8-bit cache
+  // 171 / 132 / 131 / 121 / 120 / 125 / 126 / 136, 48 (16 each) 108 / 92 / 84 / 79 / 79 / 73 / 77 / 78, 10 786 x 24 of 256 77 / 65 / 59 / 56 / 55 / 52 / 54 /
+  // 53; 6000 x 48 of 128, 16 bits, 39 / 34 / 32 / 33 / 34 / 33 / 35 / 35; 700 x 48 7.3 / 6.6 / 6.6 / 7.0 / 7.7 / 7.9 / 9.2 / 11.4, 300 x 80 5.2 / 5.3 / 6.1 /
+  // 5.8 / 6.0 / 6.9 / 7.5 / 10.7.
   const int total = q_heads + (has_k ? kv_heads : 0) + (cached ? kv_heads : 0);
   p.parts = 1;
-  while (p.parts * 6 <= total) p.parts *= 2;
-  if (num_tokens * p.parts < 8192) p.parts = total;
+  while (p.parts * 8 <= total) p.parts *= 2;
+  constexpr int64_t kFew = 8 * 256 * 64;                     // threads of eight wavefronts to a CU
+  while (num_tokens * p.parts * lanes < kFew && p.parts * 6 <= total) p.parts *= 2;
+  if (num_tokens * p.parts * lanes < kFew) p.parts = total;
   const int64_t blocks = (num_tokens * p.parts * lanes + 255) / 256;
   MLA_REQUIRE(num_tokens * p.parts < (1ll << 32) - 64 && blocks < (1ll << 31), MLA_ERR_SHAPE, "%s: too many tokens for one launch", me);
 #define HEADS_LAUNCH(L)                                                                  \
