@@ -174,6 +174,34 @@ def test_two_streams_at_once(dev):
         assert torch.isfinite(ref[i]).all() and all(torch.equal(o, ref[i]) for o in outs[i])
 
 
+def test_two_graphs_of_one_stream_and_a_larger_call_between(dev):
+    """Graphs captured on one stream share its scratch memory, replayed one after the other; a call that needs more of it than there is
+    leaves what a graph holds where it is."""
+    from omni_npu_amd import kernels as K
+    cases = [make(dev, [700, 333], hq=8, hk=2, seed=51), make(dev, [1500, 20, 900], hq=16, hk=4, d=64, page=16, seed=52)]
+    refs = [call(dev, c, 1, num_chunks=12) for c in cases]
+    on = [{n: c[n].to(dev) for n in ("q", "k", "v", "table", "lens")} for c in cases]
+    outs = [torch.empty_like(o["q"]) for o in on]
+    side, graphs = torch.cuda.Stream(), []
+    for c, o, out in zip(cases, on, outs):
+        with torch.cuda.stream(side):
+            run = lambda: K.gqa_decode(o["q"], o["k"], o["v"], o["table"], o["lens"], c["scale"], out, num_chunks=12)
+            run()
+            torch.cuda.synchronize()
+            graphs.append(torch.cuda.CUDAGraph())
+            with torch.cuda.graph(graphs[-1], stream=side):
+                run()
+            torch.cuda.synchronize()
+            big = make(dev, [900] * 40, hq=64, hk=2, d=64, page=64, seed=53)
+            check(big, *call(dev, big, 1, num_chunks=300 * len(graphs)))
+    for i in (0, 1, 1, 0, 1, 0):
+        outs[i].fill_(float("nan"))
+        torch.cuda.synchronize()
+        graphs[i].replay()
+        torch.cuda.synchronize()
+        assert torch.equal(outs[i].cpu(), refs[i][0])
+
+
 def test_on_a_stream_that_is_not_the_current_one_of_the_tensors(dev):
     """Tensors made on one stream, used on another that waits for it."""
     c = make(dev, [300, 77], seed=21)
