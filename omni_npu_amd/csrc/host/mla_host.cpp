@@ -728,9 +728,16 @@ bool whole_numbers(py::handle list, std::vector<int32_t>& to) {
   }
   return true;
 }
-bool copy_pages(const std::vector<Tensor>& caches, py::handle src_list, py::handle dst_list, py::handle rows_list, const OptTensor& table) {
-  if (caches.empty() || !current_gpu(caches[0])) return false;
-  const at::Device dev = caches[0].device();
+bool copy_pages(py::handle cache_list, py::handle src_list, py::handle dst_list, py::handle rows_list, const OptTensor& table) {
+  // (the list's own tensors: a vector of them would count references up and down)
+  if (!PyList_CheckExact(cache_list.ptr())) return false;
+  const Py_ssize_t num = PyList_GET_SIZE(cache_list.ptr());
+  for (Py_ssize_t i = 0; i < num; i++)
+    if (!THPVariable_Check(PyList_GET_ITEM(cache_list.ptr(), i))) return false;
+  auto cache = [&](Py_ssize_t i) -> const Tensor& { return THPVariable_Unpack(PyList_GET_ITEM(cache_list.ptr(), i)); };
+  if (num == 0 || !current_gpu(cache(0))) return false;
+  const Tensor& first = cache(0);
+  const at::Device dev = first.device();
   std::vector<int32_t> src, dst, rows;
   const bool part = !rows_list.is_none();
   if (!whole_numbers(src_list, src) || !whole_numbers(dst_list, dst) || (part && !whole_numbers(rows_list, rows)) || dst.size() != src.size() ||
@@ -740,9 +747,10 @@ bool copy_pages(const std::vector<Tensor>& caches, py::handle src_list, py::hand
                 (table->size(0) > 1 && table->stride(0) < table->size(1))))
     return false;
   std::vector<mlahip_page_cache> list;
-  list.reserve(caches.size());
-  for (const Tensor& c : caches) {
-    if (c.dim() < 2 || c.device() != dev || c.size(0) < 1 || c.size(1) < 1 || c.size(0) != caches[0].size(0) || c.size(1) != caches[0].size(1) ||
+  list.reserve(num);
+  for (Py_ssize_t k = 0; k < num; k++) {
+    const Tensor& c = cache(k);
+    if (c.dim() < 2 || c.device() != dev || c.size(0) < 1 || c.size(1) < 1 || c.size(0) != first.size(0) || c.size(1) != first.size(1) ||
         wants_grad({&c}))
       return false;
     int64_t width = 1;
@@ -755,9 +763,9 @@ bool copy_pages(const std::vector<Tensor>& caches, py::handle src_list, py::hand
     list.push_back({c.data_ptr(), c.size(0) > 1 ? c.stride(0) * es : row_stride * c.size(1), row_stride, row});
   }
   return done(mlahip_copy_pages(list.data(), (int)list.size(), src.data(), dst.data(), part ? rows.data() : nullptr, (int)src.size(),
-                                caches[0].size(0), (int)caches[0].size(1), table ? (int32_t*)table->data_ptr() : nullptr,
+                                first.size(0), (int)first.size(1), table ? (int32_t*)table->data_ptr() : nullptr,
                                 table ? (table->size(0) > 1 ? table->stride(0) : table->size(1)) : 0, table ? (int)table->size(0) : 0,
-                                table ? (int)table->size(1) : 0, stream_of(caches[0])), "mlahip_copy_pages");
+                                table ? (int)table->size(1) : 0, stream_of(first)), "mlahip_copy_pages");
 }
 
 }  // namespace

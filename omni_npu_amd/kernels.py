@@ -1622,12 +1622,15 @@ def copy_pages(caches, src, dst, rows=None, block_table: Optional[torch.Tensor] 
     [requests, blocks] on the device) the pages move: entries that name a source name its destination afterwards.  In a captured graph
     the pairs are those of the capture."""
     what = "copy_pages"
+    native = _host.load().copy_pages
+    if native(caches, src, dst, rows, block_table):            # (lists of tensors and whole numbers)
+        return
     as_list = lambda x: x.tolist() if torch.is_tensor(x) else list(x)
     if any(torch.is_tensor(x) and x.is_cuda for x in (src, dst, rows)):
         raise ValueError(f"{what}: src, dst and rows are read on the host: lists or CPU tensors")
     caches = [caches] if torch.is_tensor(caches) else list(caches)
     src, dst, rows = as_list(src), as_list(dst), None if rows is None else as_list(rows)
-    if _host.load().copy_pages(caches, src, dst, rows, block_table):
+    if native(caches, src, dst, rows, block_table):
         return
     if any(isinstance(i, bool) or not isinstance(i, int) for x in (src, dst, rows or ()) for i in x):
         raise TypeError(f"{what}: page numbers and rows are whole numbers")

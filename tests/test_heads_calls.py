@@ -110,3 +110,17 @@ def test_the_native_host_side_cuts_steps_as_the_wrapper_does():
                             assert (chunks, heads, rows) == tuple(host.gqa_plan(batch, q_len, hq, hk, d, es, longest))
                             assert chunks >= 0 and hk % heads == 0 and heads <= (4 if d == 256 or rows == 64 or rows == 32 and d == 128 and es == 2 else 8)
                             assert rows in ((16, 32) if d == 256 else (16, 32, 64))
+
+
+def test_copy_pages_takes_what_the_native_side_does_not():
+    """Tuples, tensors of numbers, single tensors and mistakes: the general path takes or names them (no GPU here: it says so)."""
+    z = torch.zeros(4, 2, 8)
+    for caches, src, dst in ((z, [0], [1]), ((z, z), (0,), (1,)), ([z], torch.tensor([0]), torch.tensor([1])), (iter([z]), [0], [1])):
+        with pytest.raises(ValueError, match="no CPU path"):
+            K.copy_pages(caches, src, dst)
+    with pytest.raises(TypeError, match="whole numbers"):
+        K.copy_pages([z], [0.0], [1])
+    with pytest.raises(TypeError, match="whole numbers"):
+        K.copy_pages([z], [True], [1])
+    with pytest.raises(ValueError, match="sources"):
+        K.copy_pages([], [0], [1])
