@@ -6,9 +6,11 @@
 // them to the GPU in front of the launch, and they are checked before it: a destination is named once and is no pair's source, so
 // the order of the copies does not matter.
 //
-// What bounds it is memory, each byte read and written once; a workgroup copies a piece of one pair's page in one cache.  A launch of 64 MB or more
-// goes past the caches, which would not hold it: 100 pairs x 32 caches of 32 KB pages (210 MB moved) 45.8 -> 41.8 us, 5 GB 995 -> 966 (5.2 TB/s; a
-// plain copy of 2 GiB 4.9); 24 MB that the caches do hold 8.0, past them 9.9.
+// What bounds it is memory, each byte read and written once; a workgroup copies a piece of one pair's page in one cache.  A launch of 32 MB or
+// more goes past the caches, which would give up other lines for it, in pieces of 4 KB: together in flight they are neighbours in memory.  us
+// through the caches / past them, pieces of 4 KB / 32 KB, behind 2 GB of other writes: 63 MB (7 pairs x 34 caches) 37 / 27, 42 / 29; 418 MB 170 / 140, 185 /
+// 162; 2.5 GB 922 / 826, 1044 / 977.  Where the same pages are copied again and again, 47 MB 17.8 / 19.2, 105 MB 47 / 41, 2.5 GB 904 / 819 (6.1 TB/s read
+// and written; a plain copy of 2 GiB 4.9).  Smaller launches go through the caches, in pieces of 8 KB: 12 MB 5.6, past them 9.9.
 #include <stdlib.h>
 #include <string.h>
 
@@ -30,7 +32,7 @@ struct Params {
   int32_t num_caches, num_pairs, page_size, part, piece;     // piece: 16-byte (or smaller) units of a workgroup
 };
 
-// kNt: past the caches
+// kNt: past the caches (host: pieces of a unit to a thread)
 template <typename V, bool kNt>
 __global__ __launch_bounds__(256) void copy_pages_kernel(const Params p) {
   const uint32_t* pairs = p.words + p.num_caches * (int)(sizeof(Cache) / 4);
@@ -59,19 +61,20 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(const Params p) {
   const GLOBAL char* src = (const GLOBAL char*)c.base + (int64_t)(int32_t)pairs[2 * pair] * c.page_stride;
   GLOBAL char* dst = (GLOBAL char*)c.base + (int64_t)(int32_t)pairs[2 * pair + 1] * c.page_stride;
   if (c.row_bytes == c.row_stride) {
-    // (four loads on their way together: the compiler does not move one ahead of a store that might touch its bytes)
     uint32_t i = begin + threadIdx.x;
-    for (; i + 768 < end; i += 1024) {
-      V v[4];
+    if constexpr (kNt) {
+      if (i < end) __builtin_nontemporal_store(__builtin_nontemporal_load((const GLOBAL V*)src + i), (GLOBAL V*)dst + i);
+    } else {
+      // (four loads on their way together: the compiler does not move one ahead of a store that might touch its bytes)
+      for (; i + 768 < end; i += 1024) {
+        V v[4];
 #pragma unroll
-      for (int k = 0; k < 4; k++) v[k] = kNt ? __builtin_nontemporal_load((const GLOBAL V*)src + i + k * 256) : ((const GLOBAL V*)src)[i + k * 256];
+        for (int k = 0; k < 4; k++) v[k] = ((const GLOBAL V*)src)[i + k * 256];
 #pragma unroll
-      for (int k = 0; k < 4; k++) {
-        if constexpr (kNt) __builtin_nontemporal_store(v[k], (GLOBAL V*)dst + i + k * 256);
-        else ((GLOBAL V*)dst)[i + k * 256] = v[k];
+        for (int k = 0; k < 4; k++) ((GLOBAL V*)dst)[i + k * 256] = v[k];
       }
+      for (; i < end; i += 256) ((GLOBAL V*)dst)[i] = ((const GLOBAL V*)src)[i];
     }
-    for (; i < end; i += 256) ((GLOBAL V*)dst)[i] = ((const GLOBAL V*)src)[i];
   } else {
     for (uint32_t i = begin + threadIdx.x; i < end; i += 256) {
       const uint32_t r = i / row_units;
@@ -140,7 +143,7 @@ extern "C" int mlahip_copy_pages(const mlahip_page_cache* caches, int32_t num_ca
   // A launch takes as many pairs and caches as its arguments hold, the caches of one unit (16, 4 or 1 bytes: what addresses, strides and
   // rows are multiples of).  A batch of pairs takes the table along in its first launch.
   constexpr int kCacheBytes = (int)sizeof(pages::Cache), kMostPairs = 192;
-  constexpr uint64_t kPast = 64ull << 20;
+  constexpr uint64_t kPast = 32ull << 20;
   const int pair_bytes = rows ? 12 : 8;
   for (int32_t p0 = 0; p0 < num_pairs; p0 += kMostPairs) {
     const int32_t n = num_pairs - p0 < kMostPairs ? num_pairs - p0 : kMostPairs;
@@ -150,7 +153,7 @@ extern "C" int mlahip_copy_pages(const mlahip_page_cache* caches, int32_t num_ca
       int32_t next = 0;
       while (next < num_caches) {
         pages::Params p;
-        uint64_t most = 0, total = 0;
+        uint64_t most = 0, least = ~0ull, total = 0;
         int32_t m = 0;
         for (; next < num_caches && m < room; next++) {
           const mlahip_page_cache& c = caches[next];
@@ -161,6 +164,7 @@ extern "C" int mlahip_copy_pages(const mlahip_page_cache* caches, int32_t num_ca
           m++;
           const uint64_t units = (uint64_t)page_size * (uint64_t)c.row_bytes / unit;
           most = units > most ? units : most;
+          least = units < least ? units : least;
           total += units * n;
         }
         if (m == 0) break;
@@ -172,13 +176,18 @@ extern "C" int mlahip_copy_pages(const mlahip_page_cache* caches, int32_t num_ca
         }
         p.table = block_table; p.table_stride = bt_stride; p.table_rows = bt_rows; p.table_cols = bt_cols;
         p.num_caches = m; p.num_pairs = n; p.page_size = page_size; p.part = rows != nullptr;
-        // a unit to a thread where there is little, up to sixteen where every CU has 32 workgroups all the same
-        uint64_t piece = 256;
-        while (piece < 4096 && piece * 256 * 32 < total) piece *= 2;
+        const bool past = unit == 16 && total * 16 >= kPast;
+        // smaller units: up to sixteen to a thread where every CU has 32 workgroups all the same
+        uint64_t piece = unit == 16 && !past ? 512 : 256;
+        while (unit < 16 && piece < 4096 && piece * 256 * 32 < total) piece *= 2;
+        // Workgroups go to the eight XCDs in turn.  Where pages end at different pieces an odd number of them has a page's first ones, which all of
+        // them have, on every XCD: 6 pairs x 27 + 27 caches of 128 and 16 KB, filled rows, 16 / 17 pieces 7.5 / 6.1 us.
+        unsigned pieces = (unsigned)((most + piece - 1) / piece);
+        if (pieces > 1 && (rows || least != most)) pieces |= 1;
         p.piece = (int32_t)piece;
-        const dim3 grid((unsigned)((most + piece - 1) / piece), (unsigned)m, (unsigned)(n + (table ? 1 : 0)));
+        const dim3 grid(pieces, (unsigned)m, (unsigned)(n + (table ? 1 : 0)));
         table = false;
-        if (unit == 16 && total * 16 >= kPast) hipLaunchKernelGGL((pages::copy_pages_kernel<u32x4, true>), grid, dim3(256), 0, stream, p);
+        if (past) hipLaunchKernelGGL((pages::copy_pages_kernel<u32x4, true>), grid, dim3(256), 0, stream, p);
         else if (unit == 16) hipLaunchKernelGGL((pages::copy_pages_kernel<u32x4, false>), grid, dim3(256), 0, stream, p);
         else if (unit == 4) hipLaunchKernelGGL((pages::copy_pages_kernel<uint32_t, false>), grid, dim3(256), 0, stream, p);
         else hipLaunchKernelGGL((pages::copy_pages_kernel<uint8_t, false>), grid, dim3(256), 0, stream, p);
