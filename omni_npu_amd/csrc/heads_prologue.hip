@@ -14,7 +14,7 @@
 // have work.
 //
 // What bounds it is memory, every value read and written once: 16 384 tokens x 64 + 2 x 8 heads of 128 into the 8-bit cache (646 MB) take
-// 120 us, 5.4 TB/s (a copy of 2 GiB on this card: 4.94).  2999 tokens x 16 + 2 x 4 heads of 64 (19 MB) take 6.6 us, and 1 token 2.7, 64 tokens 2.8 in
+// 115 us, 5.6 TB/s (a copy of 2 GiB on this card: 4.94).  2999 tokens x 16 + 2 x 4 heads of 64 (19 MB) take 6.6 us, and 1 token 2.7, 64 tokens 2.8 in
 // a graph, which is a launch and three dependent reads (slot and position, table row, values).  Without the next head's values on their
 // way 10 786 tokens x 8 + 2 x 8 heads of 256 took 72 us in place of 53; with the first key and value head of a group asked for in front of its queries
 // (80 registers in place of 60) 16 384 x 32 + 2 x 8 of 128 took 81 in place of 78.
@@ -74,8 +74,17 @@ __device__ __forceinline__ uint32_t to_e4m3(const float* x, float s, float inv) 
   return (uint32_t)w;
 }
 
-// T: the inputs' type; kLanes: lanes of a head; kFp8: an 8-bit cache; kPairs: interleaved pairs
-template <typename T, int kLanes, bool kFp8, bool kPairs>
+// What is read and written once, past the caches or through them.
+template <bool kPast, typename V> __device__ __forceinline__ V take(const void* at) {
+  return kPast ? __builtin_nontemporal_load((const V*)at) : *(const V*)at;
+}
+template <bool kPast, typename V> __device__ __forceinline__ void give(void* at, V x) {
+  if constexpr (kPast) __builtin_nontemporal_store(x, (V*)at);
+  else *(V*)at = x;
+}
+
+// T: the inputs' type; kLanes: lanes of a head; kFp8: an 8-bit cache; kPairs: interleaved pairs; kPast: past the caches
+template <typename T, int kLanes, bool kFp8, bool kPairs, bool kPast>
 __global__ __launch_bounds__(256) void heads_prologue_kernel(const PrologueParams p) {
   typedef typename Vec4<T>::type V4;
   typedef T V8 __attribute__((ext_vector_type(8)));
@@ -103,10 +112,10 @@ __global__ __launch_bounds__(256) void heads_prologue_kernel(const PrologueParam
   }
   auto load = [&](const char* at) {
     if constexpr (kPairs) {
-      const V8 x = *(const V8*)(at + a0 * 2);
+      const V8 x = take<kPast, V8>(at + a0 * 2);
       return Eight{__builtin_shufflevector(x, x, 0, 1, 2, 3), __builtin_shufflevector(x, x, 4, 5, 6, 7)};
     } else {
-      return Eight{*(const V4*)(at + a0 * 2), *(const V4*)(at + b0 * 2)};
+      return Eight{take<kPast, V4>(at + a0 * 2), take<kPast, V4>(at + b0 * 2)};
     }
   };
   auto store8 = [&](char* at, const float* x) {
@@ -114,10 +123,10 @@ __global__ __launch_bounds__(256) void heads_prologue_kernel(const PrologueParam
 #pragma unroll
     for (int e = 0; e < 8; e++) y[e] = (T)x[e];
     if constexpr (kPairs) {
-      *(V8*)(at + a0 * 2) = y;
+      give<kPast>(at + a0 * 2, y);
     } else {
-      *(V4*)(at + a0 * 2) = __builtin_shufflevector(y, y, 0, 1, 2, 3);
-      *(V4*)(at + b0 * 2) = __builtin_shufflevector(y, y, 4, 5, 6, 7);
+      give<kPast, V4>(at + a0 * 2, __builtin_shufflevector(y, y, 0, 1, 2, 3));
+      give<kPast, V4>(at + b0 * 2, __builtin_shufflevector(y, y, 4, 5, 6, 7));
     }
   };
   auto cache_row = [&](int i, int h) { return p.cache[i] + at.pg * p.c_sp[i] + at.off * p.c_sr[i] + h * p.c_sh[i]; };
@@ -177,10 +186,10 @@ __global__ __launch_bounds__(256) void heads_prologue_kernel(const PrologueParam
         const float sc = p.scale[0] ? p.scale[0][h] : 1.f, inv = 1.f / sc;
         const uint32_t lo = to_e4m3(x, sc, inv), hi = to_e4m3(x + 4, sc, inv);
         if constexpr (kPairs) {
-          *(u32x2*)(dst + a0) = u32x2{lo, hi};
+          give<kPast>(dst + a0, u32x2{lo, hi});
         } else {
-          *(uint32_t*)(dst + a0) = lo;
-          *(uint32_t*)(dst + b0) = hi;
+          give<kPast>(dst + a0, lo);
+          give<kPast>(dst + b0, hi);
         }
       } else {
         store8(dst, x);
@@ -190,30 +199,30 @@ __global__ __launch_bounds__(256) void heads_prologue_kernel(const PrologueParam
   if (!store || !mine || head >= keys + p.kv_heads) return;
   // (values are not turned: eight in a row to a lane)
   const char* src = p.src[2] + t * p.src_st[2] + j * 16;
-  V8 next = *(const V8*)(src + (head - keys) * p.src_sh[2]);
+  V8 next = take<kPast, V8>(src + (head - keys) * p.src_sh[2]);
   for (; head < keys + p.kv_heads; head += p.parts) {
     const int h = head - keys;
     const V8 raw = next;
-    if (head + p.parts < keys + p.kv_heads) next = *(const V8*)(src + (h + p.parts) * p.src_sh[2]);
+    if (head + p.parts < keys + p.kv_heads) next = take<kPast, V8>(src + (h + p.parts) * p.src_sh[2]);
     char* dst = cache_row(1, h);
     if constexpr (kFp8) {
       float x[8];
 #pragma unroll
       for (int e = 0; e < 8; e++) x[e] = (float)raw[e];
       const float sc = p.scale[1] ? p.scale[1][h] : 1.f, inv = 1.f / sc;
-      *(u32x2*)(dst + j * 8) = u32x2{to_e4m3(x, sc, inv), to_e4m3(x + 4, sc, inv)};
+      give<kPast>(dst + j * 8, u32x2{to_e4m3(x, sc, inv), to_e4m3(x + 4, sc, inv)});
     } else {
-      *(V8*)(dst + j * 16) = raw;
+      give<kPast>(dst + j * 16, raw);
     }
   }
 }
 
-template <typename T, int kLanes>
+template <typename T, int kLanes, bool kPast>
 void launch(const PrologueParams& p, bool fp8, bool pairs, unsigned blocks, hipStream_t st) {
-  if (fp8 && pairs) hipLaunchKernelGGL((heads_prologue_kernel<T, kLanes, true, true>), dim3(blocks), dim3(256), 0, st, p);
-  else if (fp8) hipLaunchKernelGGL((heads_prologue_kernel<T, kLanes, true, false>), dim3(blocks), dim3(256), 0, st, p);
-  else if (pairs) hipLaunchKernelGGL((heads_prologue_kernel<T, kLanes, false, true>), dim3(blocks), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((heads_prologue_kernel<T, kLanes, false, false>), dim3(blocks), dim3(256), 0, st, p);
+  if (fp8 && pairs) hipLaunchKernelGGL((heads_prologue_kernel<T, kLanes, true, true, kPast>), dim3(blocks), dim3(256), 0, st, p);
+  else if (fp8) hipLaunchKernelGGL((heads_prologue_kernel<T, kLanes, true, false, kPast>), dim3(blocks), dim3(256), 0, st, p);
+  else if (pairs) hipLaunchKernelGGL((heads_prologue_kernel<T, kLanes, false, true, kPast>), dim3(blocks), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((heads_prologue_kernel<T, kLanes, false, false, kPast>), dim3(blocks), dim3(256), 0, st, p);
 }
 
 }  // namespace heads
@@ -282,9 +291,15 @@ extern "C" int mlahip_qk_norm_rope_cache(
   if (num_tokens * p.parts * lanes < kFew) p.parts = total;
   const int64_t blocks = (num_tokens * p.parts * lanes + 255) / 256;
   MLA_REQUIRE(num_tokens * p.parts < (1ll << 32) - 64 && blocks < (1ll << 31), MLA_ERR_SHAPE, "%s: too many tokens for one launch", me);
-#define HEADS_LAUNCH(L)                                                                  \
-  if (dtype == 0) heads::launch<__bf16, L>(p, fp8, interleaved != 0, (unsigned)blocks, stream); \
-  else heads::launch<_Float16, L>(p, fp8, interleaved != 0, (unsigned)blocks, stream)
+  // Past the caches from 64 MB of input on, which would not wait in them for the attention behind: us through / past them, 16 384 tokens x 64 + 2 x 8
+  // heads of 128 into the 8-bit cache 122 / 114, x 32 + 2 x 8 81 / 74, 6000 x 32 + 2 x 8 (74 MB) 34 / 30, 1674 x 64 + 2 x 8 of 256 (69 MB) 30.5 / 29.3; 16 384 x
+  // 8 + 2 x 8 of 64 (50 MB) 23.6 / 24.4, 3000 x 32 + 2 x 8 of 128 (37 MB) 13.7 / 16.3.
+  const bool past = num_tokens * total * dim * 2 >= (64ll << 20);
+#define HEADS_LAUNCH(L)                                                                                           \
+  if (dtype == 0 && past) heads::launch<__bf16, L, true>(p, fp8, interleaved != 0, (unsigned)blocks, stream);    \
+  else if (dtype == 0) heads::launch<__bf16, L, false>(p, fp8, interleaved != 0, (unsigned)blocks, stream);      \
+  else if (past) heads::launch<_Float16, L, true>(p, fp8, interleaved != 0, (unsigned)blocks, stream);           \
+  else heads::launch<_Float16, L, false>(p, fp8, interleaved != 0, (unsigned)blocks, stream)
   if (lanes == 8) { HEADS_LAUNCH(8); }
   else if (lanes == 16) { HEADS_LAUNCH(16); }
   else { HEADS_LAUNCH(32); }

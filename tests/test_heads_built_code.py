@@ -4,7 +4,7 @@ import pytest
 from tests.test_built_code import _built
 
 
-@pytest.mark.parametrize("source,kernel,count", [("gqa_decode.hip", "gqa_split_kernel", 32), ("heads_prologue.hip", "heads_prologue_kernel", 24),
+@pytest.mark.parametrize("source,kernel,count", [("gqa_decode.hip", "gqa_split_kernel", 32), ("heads_prologue.hip", "heads_prologue_kernel", 48),
                                                  ("copy_pages.hip", "copy_pages_kernel", 4)])
 def test_no_spills_and_no_flat_accesses(source, kernel, count, tmp_path):
     """Tiles, sums and the next tile's loads fill the registers: what the compiler would put into scratch memory comes back behind a wait

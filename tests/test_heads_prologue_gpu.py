@@ -257,3 +257,33 @@ def test_no_tokens(dev):
     K.qk_norm_rope_cache(z(4), z(2), z(2), c["cos"].to(dev), c["sin"].to(dev), i, i, kc, kc.clone())
     K.qk_norm_rope_cache(z(4), None, None, c["cos"].to(dev), c["sin"].to(dev), i)
     assert torch.equal(kc.cpu(), c["kc"])
+
+
+@pytest.mark.parametrize("d,interleaved", [(64, False), (128, True), (256, False)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("fp8", [False, True], ids=["same", "e4m3"])
+def test_large_batches_are_as_their_parts(dev, d, interleaved, dtype, fp8):
+    """From 64 MB of input on values go past the caches: the same bits as in calls of a few hundred tokens."""
+    from omni_npu_amd import kernels as K
+    hq, hk = 30, 5
+    t = (64 << 20) // (40 * d * 2) + 77
+    g = torch.Generator(device=dev).manual_seed(d)
+    qkv = torch.randn(t, 40 * d, generator=g, device=dev).to(dtype)
+    angle = torch.outer(torch.arange(t, device=dev).float(), 10000.0 ** (-torch.arange(0, d, 2, device=dev).float() / d))
+    gamma = (1 + 0.1 * torch.randn(d, generator=g, device=dev)).to(dtype)
+    scale = torch.full((hk,), 0.02, device=dev) if fp8 else None
+    positions, slots = torch.arange(t, device=dev), torch.randperm(t + 50, generator=g, device=dev)[:t]
+    slots[5] = -1
+
+    def outputs(step):
+        q_out = torch.zeros(t, hq, d, dtype=dtype, device=dev)
+        kc, vc = (torch.zeros(-(-(t + 50) // 16), 16, hk, d, device=dev).to(E4M3 if fp8 else dtype) for _ in range(2))
+        for a in range(0, t, step):
+            part = slice(a, min(a + step, t))
+            q, k, v = (x.unflatten(1, (-1, d)) for x in qkv[part].split([hq * d, hk * d, hk * d], dim=1))
+            K.qk_norm_rope_cache(q, k, v, angle.cos(), angle.sin(), positions[part], slots[part], kc, vc, q_gamma=gamma, k_gamma=gamma, eps=EPS,
+                                 interleaved=interleaved, q_out=q_out[part], k_scale=scale, v_scale=scale)
+        return q_out, kc.view(torch.uint8), vc.view(torch.uint8)
+
+    for whole, parts in zip(outputs(t), outputs(3001)):
+        assert torch.equal(whole, parts) and whole.any()
