@@ -136,3 +136,30 @@ def test_refusals(dev):
     refused(ValueError, "int32", c, [0], [1], block_table=torch.zeros(2, 2, device=dev))
     refused(TypeError, "whole numbers", c, [0.0], [1])
     refused(ValueError, "no CPU path", c.cpu(), [0], [1])
+
+
+@pytest.mark.parametrize("part", [False, True])
+@pytest.mark.parametrize("widths", [[1024, 1024], [1024, 128], [656, 656]])
+def test_copies_that_go_past_the_caches(dev, part, widths):
+    """32 MB and more: whole pages and filled rows, caches of one size and of two, a table that follows."""
+    from omni_npu_amd import kernels as K
+    g = torch.Generator(device=dev).manual_seed(7)
+    pairs, page = 400, 128
+    pages = 2 * pairs + 5
+    caches = [torch.randint(0, 256, (pages, page, w), generator=g, device=dev, dtype=torch.uint8) for w in widths]
+    order = torch.randperm(pages, generator=g, device=dev)
+    src, dst = order[:pairs], order[pairs:2 * pairs]
+    rows = torch.randint(0, page + 1, (pairs,), generator=g, device=dev) if part else None
+    table = None if part else torch.randint(0, pages, (37, 65), generator=g, device=dev, dtype=torch.int32)
+    want = [c.clone() for c in caches]
+    for c, old in zip(want, caches):
+        keep = torch.arange(page, device=dev)[None, :, None] >= (rows[:, None, None] if part else page)
+        c[dst] = torch.where(keep, old[dst], old[src])
+    if table is not None:
+        follow = torch.arange(pages, device=dev, dtype=torch.int32)
+        follow[src] = dst.int()
+        want_table = follow[table.long()]
+    K.copy_pages(caches, src.tolist(), dst.tolist(), rows.tolist() if part else None, table)
+    for got, ref in zip(caches, want):
+        assert torch.equal(got, ref)
+    assert table is None or torch.equal(table, want_table)
