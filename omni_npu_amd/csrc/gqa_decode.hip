@@ -34,6 +34,10 @@ namespace gqa {
 constexpr int kUnit = 32;                                    // keys of a plan unit
 constexpr int kTile = 32;                                    // keys of a wavefront's step
 constexpr float kOutgrown = 8.f;                             // log2 units a score may lie above its row's reference
+// Probabilities go to the products in two operands of the matrix instruction's type: exp2(score - reference) =: x, rounded, and the rest up to
+// (1 + 2^-6) x, the probability that both stand for.  More than x, so that the rest is positive whichever way x was rounded: an infinite value gives an
+// infinity twice then, and never one less another.  Rounded, the rest is off by (2^-6 + 2^-8) 2^-8 of x in bf16, (2^-6 + 2^-11) 2^-11 in fp16.
+constexpr float kWhole = 1.f + 0x1p-6f, kWholeLog2 = 0.02236781302845451f;
 
 struct Params {
   const char *k, *v; int64_t k_sp, v_sp;                     // strides in bytes
@@ -390,7 +394,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
         if (i + 1 < mine) ask_keys(i + 1);
         __builtin_amdgcn_sched_barrier(0);
         // ---- probabilities against the rows' references ----
-        u32x4 pf[MT];
+        u32x4 pf[MT], pl[MT];
 #pragma unroll
         for (int m = 0; m < MT; m++) {
           float most = -INFINITY;
@@ -424,16 +428,25 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
           const float ref = m_ref[m] == -INFINITY ? 0.f : m_ref[m];
 #pragma unroll
           for (int s = 0; s < 2; s++) {
-            // probabilities are rounded to the operand's type, and the rounded ones are what the sum counts: the weights that are
-            // applied add up to one
-            typename Ty::v4 pr;
+            // One operand alone would be off by 2^-8 of a probability in bf16, 2^-11 in fp16: as much as a result's own rounding.  The second
+            // takes up to 1.5 % of the time with 16 and 32 rows (64 x 4096-8192 keys x 32/8 heads 252 us / 254), with 64 rows, which the products
+            // bound, 2-9 (64 x 4 tokens x 2000-6000 keys x 64/4 of 128 125 / 127.5, e4m3 95.5 / 103), long prompts 20.  The sum counts what the
+            // products take: the weights that are applied add up to one.
+            typename Ty::v4 pr, rest;
 #pragma unroll
-            for (int e = 0; e < 4; e++) pr[e] = (T)fast_exp2(sc[m][s][e] - ref);
-            const u32x2 w = __builtin_bit_cast(u32x2, pr);
+            for (int e = 0; e < 4; e++) {
+              const float x = fast_exp2(sc[m][s][e] - ref);
+              pr[e] = (T)x;
+              rest[e] = (T)__builtin_fmaf(x, kWhole, -(float)pr[e]);
+            }
+            const u32x2 w = __builtin_bit_cast(u32x2, pr), z = __builtin_bit_cast(u32x2, rest);
             pf[m][2 * s] = w[0];
             pf[m][2 * s + 1] = w[1];
+            pl[m][2 * s] = z[0];
+            pl[m][2 * s + 1] = z[1];
           }
-          sum[m] = Ty::mm(u32x4{Ty::kOnes, Ty::kOnes, Ty::kOnes, Ty::kOnes}, pf[m], sum[m]);
+          const u32x4 ones = {Ty::kOnes, Ty::kOnes, Ty::kOnes, Ty::kOnes};
+          sum[m] = Ty::mm(ones, pl[m], Ty::mm(ones, pf[m], sum[m]));
         }
         // the values have arrived: into LDS (a wavefront's LDS operations keep their order: the reads of the tile before are done)
         __builtin_amdgcn_sched_barrier(0);
@@ -494,6 +507,10 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
           for (int o = 0; o < Sh::ops; o++)
 #pragma unroll
             for (int m = 0; m < MT; m++) acc[m][d * Sh::ops + o] = Ty::mm(a[o], pf[m], acc[m][d * Sh::ops + o]);
+#pragma unroll
+          for (int o = 0; o < Sh::ops; o++)
+#pragma unroll
+            for (int m = 0; m < MT; m++) acc[m][d * Sh::ops + o] = Ty::mm(a[o], pl[m], acc[m][d * Sh::ops + o]);
         }
       }
 
@@ -554,7 +571,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
         const int tk = p.max_q_len == 1 ? 0 : (int)((uint32_t)r / (uint32_t)p.group), qh = hd * p.group + (r - tk * p.group);
         const int64_t t = (int64_t)sq.q0 + tk;
         if ((only >= 0 && tk != only) || (whole && (t < 0 || t >= last->num_tokens))) return (char*)nullptr;
-        const float lse = total == 0.f ? -INFINITY : (most + fast_log2(total)) * kLn2;
+        const float lse = total == 0.f ? -INFINITY : (most + (fast_log2(total) - kWholeLog2)) * kLn2;
         if (whole) {
           if (last->lse && first_dims) ((GLOBAL float*)last->lse)[t * (p.kv_heads * p.group) + qh] = lse;
           return last->out + t * last->o_st + (int64_t)qh * last->o_sh;

@@ -1,0 +1,62 @@
+"""How near the attention over ordinary key and value heads comes to its 64-bit statement: results are off by their own rounding, and by
+little else."""
+import pytest
+import torch
+
+from oracle import heads_oracle as H
+from tests.test_gqa_decode_gpu import call, make
+
+pytestmark = pytest.mark.gpu
+
+# Of a probability, what two operands leave of it: the first part, 1 - 2^-6 of it, is rounded by a relative u, so the rest is at most 2^-6 + u of it,
+# and is rounded by u again.
+LEFT = {t: H.U[t] * (2.0 ** -6 + H.U[t]) for t in (torch.bfloat16, torch.float16)}
+
+
+def tolerance(c, o, weight, reach, lse):
+    """The result's own rounding; probabilities off by LEFT (of which numerator and denominator take the same ones: weight + |o| in all); in fp16 a
+    rest below 2^-14 is rounded by 2^-25, for every key, against a sum of at least one; a sum of n products in fp32, n 2^-24 of their sizes; scores' errors
+    and the smaller roundings as H.gqa_tolerance has them."""
+    n = int(c["lens"].max())
+    v = c["v"].float().abs().amax() * (1.0 if c["v_scale"] is None else c["v_scale"].max())
+    small = n * 2.0 ** -25 * (c["dtype"] == torch.float16)
+    part = 1.01 * LEFT[c["dtype"]] + n * 2.0 ** -24 + 2 * (c["d"] + 4) * 2.0 ** -24 * reach[..., None] + 2.0 ** -19
+    return H.U[c["dtype"]] * o.abs() + part * (weight + o.abs()) + small * (float(v) + o.abs()) + 1e-30
+
+
+def close(c, out, lse):
+    k, v = (c[n].float() for n in ("k", "v"))
+    o, l, weight, reach = H.gqa(c["q"], k, v, c["table"], c["lens"], c["scale"], c["start"], 0, c["k_scale"], c["v_scale"])
+    tol = tolerance(c, o, weight, reach, l)
+    err = (out.double() - o).abs()
+    assert (err <= tol).all(), f"worst {(err / tol).max():.3g} of the tolerance"
+    n = int(c["lens"].max())
+    off = 1.01 * LEFT[c["dtype"]] + n * (2.0 ** -24 + 2.0 ** -25 * (c["dtype"] == torch.float16)) + (c["d"] + 4) * 2.0 ** -24 * reach + 2.0 ** -18 * (1 + l.abs())
+    assert ((lse.double() - l).abs() <= off).all()
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("fp8", [False, True], ids=["same", "e4m3"])
+@pytest.mark.parametrize("q_len,hq,hk", [(1, 8, 2), (3, 16, 2), (5, 26, 2)])
+@pytest.mark.parametrize("chunks", [0, 7])
+def test_results_are_off_by_their_own_rounding(dev, d, dtype, fp8, q_len, hq, hk, chunks):
+    """Few keys and many, so that probabilities' roundings would not average out."""
+    c = make(dev, [6, 11, 40, 700, 7], q_len=q_len, hq=hq, hk=hk, d=d, dtype=dtype, fp8=fp8, page=16, seed=d + q_len)
+    close(c, *call(dev, c, q_len, num_chunks=chunks))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("chunks", [0, 6])
+def test_an_infinite_value_gives_an_infinity(dev, dtype, chunks):
+    """In every key's place once, of its sign, whatever its probability: 64 requests of 64 keys, each with one; the other dims are as without it."""
+    c = make(dev, [64] * 64, hq=8, hk=2, d=64, dtype=dtype, page=16, seed=3)
+    ref, ref_lse = call(dev, c, 1, num_chunks=chunks)
+    for b in range(64):
+        c["v"][c["table"][b, b // 16], b % 16, :, b] = float("inf") if b % 2 else -float("inf")
+    out, lse = call(dev, c, 1, num_chunks=chunks)
+    at = torch.arange(64)
+    there = out[at, :, at].float()
+    assert torch.isinf(there).all() and ((there > 0) == (at % 2 == 1)[:, None]).all()
+    out[at, :, at] = ref[at, :, at]
+    assert torch.equal(out, ref) and torch.equal(lse, ref_lse)
