@@ -33,7 +33,6 @@ namespace gqa {
 
 constexpr int kUnit = 32;                                    // keys of a plan unit
 constexpr int kTile = 32;                                    // keys of a wavefront's step
-constexpr float kOutgrown = 8.f;                             // log2 units a score may lie above its row's reference
 // Probabilities go to the products in two operands of the matrix instruction's type: exp2(score - reference) =: x, rounded, and the rest up to
 // (1 + 2^-6) x, the probability that both stand for.  More than x, so that the rest is positive whichever way x was rounded: an infinite value gives an
 // infinity twice then, and never one less another.  Rounded, the rest is off by (2^-6 + 2^-8) 2^-8 of x in bf16, (2^-6 + 2^-11) 2^-11 in fp16.
@@ -73,6 +72,8 @@ template <> struct Types<__bf16> {
     return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
   }
   static constexpr uint32_t kOnes = 0x3f803f80u;
+  // log2 units: how far a row's reference is set below its largest score, and how far above that a later one may lie before it is set anew
+  static constexpr float kBelow = 0.f, kOutgrown = 8.f;
   static constexpr uint32_t kExp = 0x7f807f80u, kLow = 0x00800080u;   // a number's exponent bits and the lowest of them
 };
 template <> struct Types<_Float16> {
@@ -86,6 +87,10 @@ template <> struct Types<_Float16> {
     return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, false));
   }
   static constexpr uint32_t kOnes = 0x3c003c00u;
+  // Probabilities of 2^13 to 2^15 for the largest scores: an fp16 below 2^-14 loses bits, and one below 2^-25 is none.  8192 keys that are worth
+  // 2^-26 each beside one key are 2^-13 of the result; with 1 for the largest they were left out of it.  (Setting references anew more often:
+  // 64 x 4096-8192 keys x 32/8 heads 263.5 us / 263.6, 33 x 1024 x 16/4 of 256 35.7 / 35.9.)
+  static constexpr float kBelow = 13.f, kOutgrown = 2.f;
   static constexpr uint32_t kExp = 0x7c007c00u, kLow = 0x04000400u;
 };
 
@@ -415,10 +420,11 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
           for (int s = 0; s < 2; s++)
 #pragma unroll
             for (int e = 0; e < 4; e++) most = fmaxf(most, sc[m][s][e]);
-          if (__builtin_amdgcn_ballot_w64(most > m_ref[m] + kOutgrown)) {
+          // (a difference: beyond 2^24 a sum would round to a larger one, and fp16 ends at 2^16)
+          if (__builtin_amdgcn_ballot_w64(most - m_ref[m] > Ty::kBelow + Ty::kOutgrown)) {
             most = fmaxf(most, __shfl_xor(most, 16, 64));
             most = fmaxf(most, __shfl_xor(most, 32, 64));
-            const float next = fmaxf(m_ref[m], most);
+            const float next = fmaxf(m_ref[m], most - (fabsf(most) < 0x1p20f ? Ty::kBelow : 0.f));
             const float f = next > m_ref[m] ? fast_exp2(m_ref[m] - next) : 1.f;
             m_ref[m] = next;
             sum[m] *= f;
@@ -435,6 +441,8 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
             typename Ty::v4 pr, rest;
 #pragma unroll
             for (int e = 0; e < 4; e++) {
+              // (not one operation with the product above: scores of 2^25 and more lie further from their unrounded ones than fp16 reaches)
+#pragma clang fp contract(off)
               const float x = fast_exp2(sc[m][s][e] - ref);
               pr[e] = (T)x;
               rest[e] = (T)__builtin_fmaf(x, kWhole, -(float)pr[e]);

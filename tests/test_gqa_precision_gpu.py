@@ -60,3 +60,49 @@ def test_an_infinite_value_gives_an_infinity(dev, dtype, chunks):
     assert torch.isinf(there).all() and ((there > 0) == (at % 2 == 1)[:, None]).all()
     out[at, :, at] = ref[at, :, at]
     assert torch.equal(out, ref) and torch.equal(lse, ref_lse)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("gap", [4, 14, 22, 24, 26, 30])
+@pytest.mark.parametrize("heads,chunks", [(8, 0), (1, 0), (8, 5)])
+def test_many_keys_far_below_one(dev, dtype, gap, heads, chunks):
+    """The first key takes nearly everything and has small values; 8191 others lie ``gap`` powers of two below it.  In fp16 a probability is off by
+    2^-25 at most where the largest are 2^13 and more, and a result below 2^-14 by 2^-25."""
+    n, g = 8192, torch.Generator().manual_seed(gap)
+    c = make(dev, [n], hq=8, hk=8, d=64, dtype=dtype, page=128, seed=gap)
+    c["scale"] = 1.0
+    c["q"].zero_()
+    c["q"][..., 0] = 8.0
+    c["k"][..., 0] = (4.0 + (torch.rand(c["k"].shape[:3], generator=g) * 0.4 - gap * 0.6931) / 8).to(dtype)
+    c["v"] += 1.0
+    first = c["table"][0, 0]
+    c["k"][first, 0, :, 0] = 4.0
+    c["v"][first, 0] = c["v"][first, 0] * 2.0 ** -10
+    out, lse = call(dev, c, 1, heads_per_group=heads, num_chunks=chunks)
+    o, l, weight, reach = H.gqa(c["q"], c["k"], c["v"], c["table"], c["lens"], 1.0, c["start"])
+    tol = H.gqa_tolerance(o, weight, reach, dtype, 64)
+    if dtype == torch.float16:
+        tol = tol + 1.02 * n * 2.0 ** -38 * (c["v"].abs().max().double() + o.abs()) + 2.0 ** -25
+    err = (out.double() - o).abs()
+    assert (err <= tol).all(), f"worst {(err / tol).max():.3g} of the tolerance"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("scale", [1.0, 8.0, 64.0, 4096.0])
+@pytest.mark.parametrize("order", ["rising", "falling", "mixed"])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_whose_steps_are_large(dev, dtype, scale, order, sign):
+    """Scores of up to 2^36, whose neighbours in fp32 lie further apart than a reference below them: one key takes everything."""
+    n, g = 200, torch.Generator().manual_seed(1)
+    c = make(dev, [n], hq=4, hk=2, d=64, dtype=dtype, page=16, seed=2)
+    c["scale"] = scale
+    c["q"].zero_()
+    c["q"][..., 0] = 32768.0 * sign
+    size = {"rising": torch.arange(n), "falling": torch.arange(n).flip(0), "mixed": torch.randperm(n, generator=g)}[order] + 1.0
+    rows = c["table"][0].long()[torch.arange(n) // 16], torch.arange(n) % 16
+    c["k"][rows[0], rows[1], :, 0] = size.to(dtype)[:, None]
+    key = int((size * sign).argmax())
+    for heads in (1, 2):
+        out, lse = call(dev, c, 1, heads_per_group=heads, num_chunks=0)
+        assert torch.equal(out[0], c["v"][rows[0][key], rows[1][key]].repeat_interleave(2, 0))
+        assert torch.allclose(lse.double(), torch.tensor(32768.0 * sign * scale * float(size[key]), dtype=torch.float64), rtol=2.0 ** -21)
