@@ -57,7 +57,7 @@ struct Params {
   char* out; int64_t o_st, o_sh;
   float* lse;                                                // [T, heads] or null
   int32_t* seg_ids;                                          // [batch][2]: first and last partial of a sequence, or -1
-  float *part_lse, *part_acc;                                // [slot][kv head][row](, [D])
+  float *part_lse, *part_acc;                                // [slot][kv head][row](, [D]); log-sum-exps in log2 units
 };
 
 template <typename T> struct Types;
@@ -579,13 +579,13 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
         const int tk = p.max_q_len == 1 ? 0 : (int)((uint32_t)r / (uint32_t)p.group), qh = hd * p.group + (r - tk * p.group);
         const int64_t t = (int64_t)sq.q0 + tk;
         if ((only >= 0 && tk != only) || (whole && (t < 0 || t >= last->num_tokens))) return (char*)nullptr;
-        const float lse = total == 0.f ? -INFINITY : (most + (fast_log2(total) - kWholeLog2)) * kLn2;
+        const float lse2 = total == 0.f ? -INFINITY : most + (fast_log2(total) - kWholeLog2);
         if (whole) {
-          if (last->lse && first_dims) ((GLOBAL float*)last->lse)[t * (p.kv_heads * p.group) + qh] = lse;
+          if (last->lse && first_dims) ((GLOBAL float*)last->lse)[t * (p.kv_heads * p.group) + qh] = lse2 * kLn2;
           return last->out + t * last->o_st + (int64_t)qh * last->o_sh;
         }
         const int64_t slot = ((int64_t)(blockIdx.x + b) * p.kv_heads + hd) * (p.max_q_len * p.group) + r;
-        if (first_dims) ((GLOBAL float*)last->part_lse)[slot] = lse;
+        if (first_dims) ((GLOBAL float*)last->part_lse)[slot] = lse2;
         return (char*)(last->part_acc + slot * D);
       };
       // Four dims of a row.  Granule gi = 4 d + g'
@@ -689,8 +689,9 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
   } while (v_cur < v_end);
 }
 
-// The partials of a sequence's chunks into its rows, by the weights exp(lse_k - max lse): kWaves wavefronts for a row, lanes of 4 dims,
+// The partials of a sequence's chunks into its rows, by the weights exp2(lse_k - max lse): kWaves wavefronts for a row, lanes of 4 dims,
 // several partials at once.  A wavefront goes by its own partials' largest log-sum-exp, so that all it reads of them is asked for together.
+// They are kept in log2 units: behind a product the compiler would subtract from the unrounded one, which is far off beyond 2^32.
 // Bound by the launch and two dependent reads: 2.2 us for 4 rows of 32 partials, 4.4 for 64 x 32 rows of 2 to 4, 8.4 for 128 x 128 of them, 45 MB.
 template <typename T, int D, int kWaves>
 __global__ __launch_bounds__(256) void gqa_join_kernel(const Params p) {
@@ -716,7 +717,7 @@ __global__ __launch_bounds__(256) void gqa_join_kernel(const Params p) {
       const int s = s0 + k * kWaves * kPer, at = s <= last ? s : last;
       l[k] = p.part_lse[at * stride + base];
       a[k] = *(const f32x4*)(p.part_acc + (at * stride + base) * D + gi * 4);
-      l[k] = s <= last ? l[k] * kLog2e : -INFINITY;
+      l[k] = s <= last ? l[k] : -INFINITY;
     }
 #pragma unroll
     for (int k = 0; k < 4; k++) next = fmaxf(next, l[k]);

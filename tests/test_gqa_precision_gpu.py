@@ -106,3 +106,22 @@ def test_scores_whose_steps_are_large(dev, dtype, scale, order, sign):
         out, lse = call(dev, c, 1, heads_per_group=heads, num_chunks=0)
         assert torch.equal(out[0], c["v"][rows[0][key], rows[1][key]].repeat_interleave(2, 0))
         assert torch.allclose(lse.double(), torch.tensor(32768.0 * sign * scale * float(size[key]), dtype=torch.float64), rtol=2.0 ** -21)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("scale", [1.0, 64.0, 4096.0, 2.0 ** 20])
+@pytest.mark.parametrize("requests,chunks", [(1, 3), (1, 20), (3, 5), (3, 40)])
+def test_pieces_with_scores_whose_steps_are_large(dev, dtype, scale, requests, chunks):
+    """The same with each request in pieces, the largest score in its first, last or a middle one."""
+    n = 400
+    c = make(dev, [n] * requests, hq=4, hk=2, d=64, dtype=dtype, page=16, seed=2)
+    c["scale"] = scale
+    c["q"].zero_()
+    c["q"][..., 0] = 32768.0
+    c["k"][..., 0] = -(torch.arange(c["k"].shape[0] * 16).view(-1, 16, 1) % 251 + 1.0).to(dtype)
+    at = torch.tensor([(0, n - 1, 170)[b] for b in range(requests)])
+    page, row = c["table"][torch.arange(requests), at // 16].long(), at % 16
+    c["k"][page, row, :, 0] = 200.0
+    out, lse = call(dev, c, 1, num_chunks=chunks)
+    assert torch.equal(out, c["v"][page, row].repeat_interleave(2, 1))
+    assert torch.allclose(lse.double(), torch.tensor(32768.0 * 200 * scale, dtype=torch.float64), rtol=2.0 ** -21)
