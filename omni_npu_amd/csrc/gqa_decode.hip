@@ -94,21 +94,22 @@ template <> struct Types<_Float16> {
   static constexpr uint32_t kExp = 0x7c007c00u, kLow = 0x04000400u;
 };
 
-// A request's tokens and keys: tokens [q0, q0 + s) of the batch, first key that any token sees, plan units.
-struct Seq { int len, q0, s, first, units; };
+// A request's tokens and keys: the first s of its tokens, [q0, q0 + s) of the batch, are done (s <= max_q_len, however many it has); token i sees
+// keys below key_0 + i; first key that any of them sees, plan units.
+struct Seq { int len, q0, s, key_0, units; };
+__device__ __forceinline__ int first_key(const Params& p, int key_0) {
+  return p.window > 0 && key_0 > p.window ? key_0 - p.window : 0;
+}
 __device__ __forceinline__ Seq seq_from(const Params& p, int len, int q0, int q1) {
   Seq x;
   x.q0 = q0;
-  x.s = q1 - q0;
-  x.s = x.s < 0 ? 0 : x.s < p.max_q_len ? x.s : p.max_q_len;
   const int room = p.max_blocks * p.page_size;               // (host: at most 2^30)
   x.len = len < 0 ? 0 : len < room ? len : room;
-  x.first = 0;
-  if (p.window > 0) {
-    const int f = x.len - x.s + 1 - p.window;
-    x.first = f > 0 ? f : 0;
-  }
-  const int n = (x.len + kUnit - 1) / kUnit - x.first / kUnit;
+  // (where a request has more tokens than keys, those of its first ones that are done see none either way)
+  const int most = x.len + p.max_q_len, tokens = q1 <= q0 ? 0 : (uint32_t)q1 - (uint32_t)q0 < (uint32_t)most ? q1 - q0 : most;
+  x.s = tokens < p.max_q_len ? tokens : p.max_q_len;
+  x.key_0 = x.len - tokens + 1;
+  const int n = (x.len + kUnit - 1) / kUnit - first_key(p, x.key_0) / kUnit;
   x.units = n > 0 ? n : 1;                                   // (a request without keys: its rows are written all the same)
   return x;
 }
@@ -252,7 +253,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
     Seq sq;
     if (in_lanes) {
       sq.len = __builtin_amdgcn_readlane(lane_seq.len, b); sq.q0 = __builtin_amdgcn_readlane(lane_seq.q0, b);
-      sq.s = __builtin_amdgcn_readlane(lane_seq.s, b); sq.first = __builtin_amdgcn_readlane(lane_seq.first, b);
+      sq.s = __builtin_amdgcn_readlane(lane_seq.s, b); sq.key_0 = __builtin_amdgcn_readlane(lane_seq.key_0, b);
       sq.units = __builtin_amdgcn_readlane(lane_seq.units, b);
     } else {
       sq = seq_at(p, b);
@@ -273,9 +274,9 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
     }
     const int rows = sq.s * p.group;
     if (row0 < rows) {
-      const int unit0 = sq.first / kUnit;
+      const int first_seen = first_key(p, sq.key_0), unit0 = first_seen / kUnit;
       int key0 = (unit0 + u0) * kUnit, key1 = (unit0 + u1) * kUnit;
-      key0 = key0 > sq.first ? key0 : sq.first & ~(kTile - 1);
+      key0 = key0 > first_seen ? key0 : first_seen & ~(kTile - 1);
       key1 = key1 < sq.len ? key1 : sq.len;
       const int tiles = key1 > key0 ? (key1 - key0 + kTile - 1) / kTile : 0;
       const int mine = tiles > kw ? (tiles - kw + kws - 1) >> kws_shift : 0;
@@ -336,7 +337,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
           const int dim = kFp8 ? (s >> 1) * 64 + g * 16 + (s & 1) * 8 : s * 32 + g * 8;
           qf[m][s] = ok ? *(const GLOBAL u32x4*)(src + dim * 2) : u32x4{0u, 0u, 0u, 0u};
         }
-        hi[m] = sq.len - sq.s + tok[m] + 1;
+        hi[m] = sq.key_0 + tok[m];
         lo[m] = p.window > 0 ? hi[m] - p.window : 0;
       }
       // keys that all of the rows see, keys that any of them sees
@@ -345,11 +346,10 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
         tok_first = (int)((uint32_t)row0 / (uint32_t)p.group);
         tok_last = (int)((uint32_t)((row0 + 16 * MT < rows ? row0 + 16 * MT : rows) - 1) / (uint32_t)p.group);
       }
-      const int key_0 = sq.len - sq.s + 1;                   // (keys of token 0)
       int only = -1;                                         // the token that a pass is for, where the piece is done token by token
       while (true) {
       const int t0 = only < 0 ? tok_first : only, t1 = only < 0 ? tok_last : only;
-      const int all_hi = key_0 + t0, any_hi = key_0 + t1, all_lo = p.window > 0 ? any_hi - p.window : 0, any_lo = p.window > 0 ? all_hi - p.window : 0;
+      const int all_hi = sq.key_0 + t0, any_hi = sq.key_0 + t1, all_lo = p.window > 0 ? any_hi - p.window : 0, any_lo = p.window > 0 ? all_hi - p.window : 0;
       uint32_t odd = 0;
       const float scale_log2 = first->scale_log2 * (kFp8 && first->k_scale ? ((const GLOBAL float*)first->k_scale)[head] : 1.f);
 
