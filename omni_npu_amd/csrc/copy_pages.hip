@@ -4,7 +4,7 @@
 //   table entries that name a source name its destination afterwards
 // The pairs are known on the host (the scheduler makes them) and travel as kernel arguments, with the caches' addresses: no copy of
 // them to the GPU in front of the launch, and they are checked before it: a destination is named once and is no pair's source, so
-// the order of the copies does not matter.
+// the order of the copies does not matter.  Where a table follows, a source is named once too: a page moves to one place.
 //
 // What bounds it is memory, each byte read and written once; a workgroup copies a piece of one pair's page in one cache.  A launch of 32 MB or
 // more goes past the caches, which would give up other lines for it, in pieces of 4 KB: together in flight they are neighbours in memory.  us
@@ -84,21 +84,27 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(const Params p) {
   }
 }
 
-// A destination twice, or one that is a source too: the pair's number, or -1.
-int64_t clash(const int32_t* src, const int32_t* dst, int32_t n, int64_t num_pages, bool* no_memory) {
-  *no_memory = false;
+// A destination twice, or one that is a source too, or, where pages move, a source twice: what is wrong and the pair's number.
+enum { kFine, kNoMemory, kDestination, kSource };
+struct Clash { int what; int32_t pair; };
+Clash clash(const int32_t* src, const int32_t* dst, int32_t n, int64_t num_pages, bool moves) {
   if (n <= 48) {
     for (int32_t i = 0; i < n; i++)
-      for (int32_t k = 0; k < n; k++)
-        if ((k < i && dst[k] == dst[i]) || src[k] == dst[i]) return i;
-    return -1;
+      for (int32_t k = 0; k < n; k++) {
+        if ((k < i && dst[k] == dst[i]) || src[k] == dst[i]) return {kDestination, i};
+        if (moves && k < i && src[k] == src[i]) return {kSource, i};
+      }
+    return {kFine, -1};
   }
   unsigned char* seen = (unsigned char*)calloc((size_t)num_pages, 1);
-  if (!seen) { *no_memory = true; return -1; }
-  for (int32_t i = 0; i < n; i++) seen[src[i]] = 1;
-  int64_t at = -1;
-  for (int32_t i = 0; i < n && at < 0; i++) {
-    if (seen[dst[i]]) at = i;
+  if (!seen) return {kNoMemory, -1};
+  Clash at{kFine, -1};
+  for (int32_t i = 0; i < n; i++) {
+    if (moves && seen[src[i]] && at.what == kFine) at = {kSource, i};
+    seen[src[i]] = 1;
+  }
+  for (int32_t i = 0; i < n && at.what == kFine; i++) {
+    if (seen[dst[i]]) at = {kDestination, i};
     seen[dst[i]] = 1;
   }
   free(seen);
@@ -133,11 +139,11 @@ extern "C" int mlahip_copy_pages(const mlahip_page_cache* caches, int32_t num_ca
     MLA_REQUIRE(!rows || (rows[i] >= 0 && rows[i] <= page_size), MLA_ERR_SHAPE, "%s: pair %d copies %d rows of %d", me, i,
                 rows ? rows[i] : 0, page_size);
   }
-  bool no_memory;
-  const int64_t bad = pages::clash(src, dst, num_pairs, num_pages, &no_memory);
-  MLA_REQUIRE(!no_memory, MLA_ERR_WORKSPACE, "%s: no host memory for %lld marks", me, (long long)num_pages);
-  MLA_REQUIRE(bad < 0, MLA_ERR_UNSUPPORTED, "%s: page %d is written by pair %lld and read or written by another", me, bad < 0 ? 0 : dst[bad],
-              (long long)bad);
+  const pages::Clash bad = pages::clash(src, dst, num_pairs, num_pages, block_table != nullptr);
+  MLA_REQUIRE(bad.what != pages::kNoMemory, MLA_ERR_WORKSPACE, "%s: no host memory for %lld marks", me, (long long)num_pages);
+  MLA_REQUIRE(bad.what != pages::kDestination, MLA_ERR_UNSUPPORTED, "%s: page %d is written by pair %d and read or written by another", me,
+              dst[bad.pair], bad.pair);
+  MLA_REQUIRE(bad.what != pages::kSource, MLA_ERR_UNSUPPORTED, "%s: page %d moves to two places (again by pair %d)", me, src[bad.pair], bad.pair);
   if (num_pairs == 0) return MLA_OK;
 
   // A launch takes as many pairs and caches as its arguments hold, the caches of one unit (16, 4 or 1 bytes: what addresses, strides and

@@ -1619,8 +1619,8 @@ def copy_pages(caches, src, dst, rows=None, block_table: Optional[torch.Tensor] 
 
     ``src``, ``dst`` and ``rows`` are host values (lists, or CPU tensors): the scheduler has them there, and they are checked
     before anything is launched.  A destination may be named once and not be a source of the same call.  With ``block_table`` (int32
-    [requests, blocks] on the device) the pages move: entries that name a source name its destination afterwards.  In a captured graph
-    the pairs are those of the capture."""
+    [requests, blocks] on the device) the pages move: entries that name a source, each named once then, name its destination afterwards.
+    In a captured graph the pairs are those of the capture."""
     what = "copy_pages"
     native = _host.load().copy_pages
     if native(caches, src, dst, rows, block_table):            # (lists of tensors and whole numbers)
@@ -1653,6 +1653,8 @@ def copy_pages(caches, src, dst, rows=None, block_table: Optional[torch.Tensor] 
     if len(set(dst)) != len(dst) or set(src) & set(dst):
         raise ValueError(f"{what}: a page is the destination of two pairs, or a source and a destination")
     if block_table is not None:
+        if len(set(src)) != len(src):
+            raise ValueError(f"{what}: a page moves to two places: with a block table a source is named once")
         if rows is not None:
             raise ValueError(f"{what}: a moved page is moved whole: no rows beside a block table")
         if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.stride(1) != 1 and block_table.shape[1] > 1 or \
