@@ -642,6 +642,10 @@ bool qk_norm_rope_cache(const Tensor& q, const OptTensor& k, const OptTensor& v,
 // kernels.gqa_plan
 std::tuple<int, int, int> gqa_plan(int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t element_bytes,
                                    int64_t max_seq_len) {
+  if (batch < 1 || q_len < 1 || kv_heads < 1 || dim < 1 || element_bytes < 1 || q_heads < kv_heads)
+    throw std::invalid_argument("gqa_plan: " + std::to_string(batch) + " requests of " + std::to_string(q_len) + " tokens, " + std::to_string(q_heads) +
+                                " query and " + std::to_string(kv_heads) + " key heads of " + std::to_string(dim) + " values, " +
+                                std::to_string(element_bytes) + " bytes each");
   const int64_t rows = q_len * q_heads / kv_heads, key = 2 * dim * element_bytes, units = batch * div_up(max_seq_len, 32);
   std::tuple<double, int64_t, int64_t, int64_t> best{INFINITY, 1, 1, 16};
   for (int64_t tile = 16; tile <= 64; tile *= 2) {
@@ -685,7 +689,7 @@ bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, c
   const at::Device dev = q.device();
   const at::ScalarType dt = q.scalar_type();
   const int64_t t = q.size(0), hq = q.size(1), d = q.size(2), hk = k_cache.size(2), b = seq_lens.numel();
-  if ((dt != at::kBFloat16 && dt != at::kHalf) || t < 1 || q.stride(2) != 1 || !heads_of(out, t, hq, d, dt, dev) || hk < 1 || hq < 1 || hq % hk ||
+  if ((dt != at::kBFloat16 && dt != at::kHalf) || t < 1 || q.stride(2) != 1 || !heads_of(out, t, hq, d, dt, dev) || hk < 1 || hq < 1 || hq % hk || d < 1 ||
       !head_cache(k_cache, hk, d, dt, dev) || !head_cache(v_cache, hk, d, dt, dev) || k_cache.sizes() != v_cache.sizes() ||
       k_cache.scalar_type() != v_cache.scalar_type() || q_len < 1 || !is_i32(seq_lens, 1, dev) || !seq_lens.is_contiguous() ||
       !is_i32(block_table, 2, dev) || block_table.size(0) < b || block_table.size(1) < 1 || b < 1 ||

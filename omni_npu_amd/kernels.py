@@ -1500,6 +1500,8 @@ def gqa_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, dim: int, elem
     own has more than 32 pieces only of two steps or more, as they are joined one after the other: 4/1 heads of 128, 5000 keys, 157 / 79
     pieces 11.3 / 9.9.  Beyond 2048 keys a request to a workgroup loses up to two thirds where lengths are ragged, which the host does not
     know."""
+    if min(batch, q_len, kv_heads, dim, element_bytes) < 1 or q_heads < kv_heads:
+        raise ValueError(f"gqa_plan: {batch} requests of {q_len} tokens, {q_heads} query and {kv_heads} key heads of {dim} values, {element_bytes} bytes each")
     rows = q_len * q_heads // kv_heads
     key = 2 * dim * element_bytes
     units = batch * -(-max_seq_len // 32)
@@ -1564,8 +1566,10 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
     code = _head_cache(what, "k_cache", k_cache, hk, d, q.dtype)
     if _head_cache(what, "v_cache", v_cache, hk, d, q.dtype) != code or k_cache.shape != v_cache.shape:
         raise ValueError(f"{what}: k_cache and v_cache must agree in shape and type")
-    if hk < 1 or hq % hk:
+    if hk < 1 or hq < 1 or hq % hk:
         raise ValueError(f"{what}: {hq} query heads over {hk} key heads")
+    if d < 1:
+        raise ValueError(f"{what}: heads of {d} values")
     if window is not None and window < 1:
         raise ValueError(f"{what}: a window of {window} keys")
     if not 1 <= q_len <= 1 << 24:
