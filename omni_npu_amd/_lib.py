@@ -102,6 +102,9 @@ SIGNATURES = {
 }
 
 
+ERR_WORKSPACE = -4                       # MLA_ERR_WORKSPACE: the scratch memory given is too small, or none
+
+
 class MlaHipError(RuntimeError):
     """A C-ABI entry point returned a negative code."""
 

@@ -861,9 +861,6 @@ extern "C" int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_st
                   vc_row_stride >= 0 && kc_row_stride * es * page_size < (1ll << 30) && vc_row_stride * es * page_size < (1ll << 30),
               MLA_ERR_SHAPE, "%s: heads must be 16-byte aligned (results: 8), the rows of a page within 1 GiB", me);
   if (batch == 0 || num_tokens == 0) return MLA_OK;
-  const size_t need = mlahip_gqa_decode_workspace_bytes(batch, max_q_len, q_heads, dim, num_chunks);
-  MLA_REQUIRE(num_chunks == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need), MLA_ERR_WORKSPACE,
-              "%s: workspace of %zu bytes, %zu are needed", me, workspace ? workspace_bytes : 0, need);
   gqa::Params p{};
   p.q = (const char*)q; p.q_st = q_stride_t * 2; p.q_sh = q_stride_h * 2;
   p.k = (const char*)k_cache; p.k_sp = kc_page_stride * es; p.k_sr = (int32_t)kc_row_stride * es; p.k_sh = kc_head_stride * es;
@@ -878,13 +875,6 @@ extern "C" int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_st
   p.window = window < max_blocks * page_size ? window : 0; p.num_chunks = num_chunks;
   p.scale_log2 = scale * kLog2e;
   p.out = (char*)out; p.o_st = out_stride_t * 2; p.o_sh = out_stride_h * 2; p.lse = lse_out;
-  if (num_chunks > 0) {
-    char* ws = (char*)workspace;
-    const int64_t n = gqa::slots(batch, num_chunks) * max_q_len * q_heads;
-    p.seg_ids = (int32_t*)ws;
-    p.part_lse = (float*)(ws + gqa::align256((int64_t)batch * 8));
-    p.part_acc = (float*)((char*)p.part_lse + gqa::align256(n * 4));
-  }
   MLA_REQUIRE(rows_per_group == 16 || rows_per_group == 32 || (rows_per_group == 64 && dim < 256), MLA_ERR_SHAPE,
               "%s: %d rows to a workgroup (16, 32, or 64 of heads of up to 128)", me, rows_per_group);
   const int rows = max_q_len * p.group, mt = rows_per_group / 16, waves = gqa::few_waves(rows_per_group, dim, es) ? 4 : 8;
@@ -899,6 +889,18 @@ extern "C" int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_st
   const int row_groups = (rows + 16 * mt - 1) / (16 * mt);
   MLA_REQUIRE((int64_t)p.head_groups * row_groups <= 65535, MLA_ERR_SHAPE, "%s: %d head groups x %d row groups", me, p.head_groups, row_groups);
   const unsigned x = (unsigned)(num_chunks > 0 ? num_chunks : batch);
+  MLA_REQUIRE((int64_t)x * waves * 64 < (1ll << 32), MLA_ERR_SHAPE, "%s: %d chunks are more than a launch takes", me, num_chunks);
+  // (last: a caller that keeps scratch memory asks for it when all else has been found right)
+  const size_t need = mlahip_gqa_decode_workspace_bytes(batch, max_q_len, q_heads, dim, num_chunks);
+  MLA_REQUIRE(num_chunks == 0 || (workspace && (uintptr_t)workspace % 16 == 0 && workspace_bytes >= need), MLA_ERR_WORKSPACE,
+              "%s: workspace of %zu bytes, %zu are needed", me, workspace ? workspace_bytes : 0, need);
+  if (num_chunks > 0) {
+    char* ws = (char*)workspace;
+    const int64_t n = gqa::slots(batch, num_chunks) * max_q_len * q_heads;
+    p.seg_ids = (int32_t*)ws;
+    p.part_lse = (float*)(ws + gqa::align256((int64_t)batch * 8));
+    p.part_acc = (float*)((char*)p.part_lse + gqa::align256(n * 4));
+  }
   return dtype == 0 ? gqa::pick<__bf16>(p, dim, cache_dtype == 3, mt, row_groups, x, stream)
                     : gqa::pick<_Float16>(p, dim, cache_dtype == 3, mt, row_groups, x, stream);
 }

@@ -39,6 +39,8 @@ constexpr int64_t kVupMaxTokens = 1024;      // kernels.VUP_MAX_TOKENS: beyond, 
 constexpr int64_t kVupOnlyTokens = 256;      // kernels._VUP_ONLY_TOKENS
 constexpr int64_t kSparseWorkspaceCap = 256 << 20;   // kernels.SPARSE_WORKSPACE_CAP
 
+constexpr int kNoWorkspace = -4;              // the library's code for scratch memory that is too small, or none
+
 void check(int rc, const char* what) {
   if (rc != 0) throw std::runtime_error(std::string(what) + " failed with code " + std::to_string(rc) + ": " + mlahip_last_error_string());
 }
@@ -65,6 +67,10 @@ Tensor& scratch(const Tensor& like, Stream stream, int64_t bytes, int tag) {
   Tensor& t = g_scratch[{like.get_device(), stream, tag}];
   if (!t.defined() || t.numel() < bytes) t = py::cast<Tensor>(py::handle(g_workspace)(like.device(), bytes, names[tag]));
   return t;
+}
+bool has_scratch(const Tensor& like, Stream stream, int64_t bytes, int tag) {
+  const auto it = g_scratch.find({like.get_device(), stream, tag});
+  return it != g_scratch.end() && it->second.numel() >= bytes;
 }
 
 int64_t div_up(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -705,16 +711,22 @@ bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, c
   const int chunks = (int)num_chunks.value_or(by_rule);
   Stream st = stream_of(q);
   const int64_t need = (int64_t)mlahip_gqa_decode_workspace_bytes((int)b, (int)q_len, (int)hq, (int)d, chunks);
-  Tensor* ws = need ? &scratch(q, st, need, 3) : nullptr;
-  return done(mlahip_gqa_decode(q.data_ptr(), q.stride(0), q.stride(1), t, k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-                          v_cache.data_ptr(), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2), k_cache.size(0), (int)k_cache.size(1),
-                          (const int32_t*)block_table.data_ptr(), block_table.stride(0), (int)block_table.size(1),
-                          (const int32_t*)seq_lens.data_ptr(), (const int32_t*)data_of(qsl), (int)b, (int)q_len, (int)hq, (int)hk, (int)d,
-                          type_code(dt), type_code(k_cache.scalar_type()), (const float*)data_of(k_scale), (const float*)data_of(v_scale),
-                          (float)scale, (int)window, out.data_ptr(), out.stride(0), out.stride(1), (float*)data_of(lse),
-                          ws ? ws->data_ptr() : nullptr, ws ? (size_t)ws->numel() : 0, chunks, (int)heads_per_group.value_or(heads),
-                          (int)rows_per_group.value_or(rows), st),
-              "mlahip_gqa_decode");
+  const auto launch = [&](const Tensor* ws) {
+    return mlahip_gqa_decode(q.data_ptr(), q.stride(0), q.stride(1), t, k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
+                             v_cache.data_ptr(), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2), k_cache.size(0), (int)k_cache.size(1),
+                             (const int32_t*)block_table.data_ptr(), block_table.stride(0), (int)block_table.size(1),
+                             (const int32_t*)seq_lens.data_ptr(), (const int32_t*)data_of(qsl), (int)b, (int)q_len, (int)hq, (int)hk, (int)d,
+                             type_code(dt), type_code(k_cache.scalar_type()), (const float*)data_of(k_scale), (const float*)data_of(v_scale),
+                             (float)scale, (int)window, out.data_ptr(), out.stride(0), out.stride(1), (float*)data_of(lse),
+                             ws ? ws->data_ptr() : nullptr, ws ? (size_t)ws->numel() : 0, chunks, (int)heads_per_group.value_or(heads),
+                             (int)rows_per_group.value_or(rows), st);
+  };
+  // More scratch memory than there is, which is kept, is asked for when nothing but it is missing.
+  if (need && !has_scratch(q, st, need, 3)) {
+    const int rc = launch(nullptr);
+    if (rc != kNoWorkspace) return done(rc, "mlahip_gqa_decode");
+  }
+  return done(launch(need ? &scratch(q, st, need, 3) : nullptr), "mlahip_gqa_decode");
 }
 
 // kernels.copy_pages

@@ -1603,16 +1603,16 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
         chunks, heads, rows = gqa_plan(b, q_len, hq, hk, d, k_cache.element_size(), longest)
         num_chunks = chunks if num_chunks is None else num_chunks
         need = lib.mlahip_gqa_decode_workspace_bytes(b, q_len, hq, d, num_chunks)
-        ws = workspace
-        if ws is None and need:
-            ws = _workspace(dev, need, "gqa")
-        rc = lib.mlahip_gqa_decode(
+        launch = lambda ws: lib.mlahip_gqa_decode(
             q.data_ptr(), q.stride(0), q.stride(1), t, k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(), *v_cache.stride()[:3],
             k_cache.shape[0], k_cache.shape[1], block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
             query_start_loc.data_ptr() if query_start_loc is not None else None, b, q_len, hq, hk, d, _HEAD_DT[q.dtype], code, *scales,
             float(scale), min(window or 0, 0x7fffffff), out.data_ptr(), out.stride(0), out.stride(1), lse_out.data_ptr() if lse_out is not None else None,
             ws.data_ptr() if ws is not None else None, ws.numel() * ws.element_size() if ws is not None else 0, num_chunks,
             heads if heads_per_group is None else heads_per_group, rows if rows_per_group is None else rows_per_group, _stream(q))
+        rc = launch(workspace)
+        if rc == _lib.ERR_WORKSPACE and workspace is None:     # (nothing but it is missing: a call that is refused takes none)
+            rc = launch(_workspace(dev, need, "gqa"))
     _lib.check(rc, "mlahip_gqa_decode")
     return out
 

@@ -1,0 +1,59 @@
+"""Scratch memory of the attention over ordinary heads, which is kept until the process ends: refused calls take none."""
+import pytest
+import torch
+
+from tests.test_gqa_decode_gpu import call, check, make
+
+pytestmark = pytest.mark.gpu
+
+
+def _args(dev, b=2, hq=8, hk=2, d=128, page=32):
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=dev)
+    i = lambda *s: torch.ones(*s, dtype=torch.int32, device=dev)
+    return [z(b, hq, d), z(4, page, hk, d), z(4, page, hk, d), i(b, 100), i(b), 0.1, z(b, hq, d)]
+
+
+@pytest.mark.parametrize("form", [dict(d=96), dict(d=16), dict(b=65536), dict(page=24), dict(page=8)], ids=str)
+@pytest.mark.parametrize("chunks", [None, 8])
+def test_what_the_shapes_refuse(dev, form, chunks):
+    _refused(dev, _args(dev, **form), num_chunks=chunks)
+
+
+@pytest.mark.parametrize("kw", [dict(num_chunks=1 << 24), dict(num_chunks=(1 << 24) - 1), dict(num_chunks=8, heads_per_group=3),
+                                dict(num_chunks=8, heads_per_group=8), dict(num_chunks=8, rows_per_group=48), dict(num_chunks=8, rows_per_group=0)], ids=str)
+def test_what_the_launch_refuses(dev, kw):
+    _refused(dev, _args(dev), **kw)
+
+
+def test_what_addresses_and_strides_refuse(dev):
+    args = _args(dev)
+    odd = torch.zeros(2 * 8 * 128 + 1, dtype=torch.bfloat16, device=dev)[1:].view(2, 8, 128)
+    _refused(dev, [odd] + args[1:], num_chunks=8)
+    _refused(dev, args[:3] + [args[3][:1].expand(2, 100)] + args[4:], num_chunks=8)       # (rows that share their memory)
+
+
+def _refused(dev, args, **kw):
+    from omni_npu_amd import kernels as K
+    side = torch.cuda.Stream()                                 # (no scratch memory yet)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        before = K.retained_workspace_bytes()
+        with pytest.raises(K._lib.MlaHipError):
+            K.gqa_decode(*args, **kw)
+        assert K.retained_workspace_bytes() == before
+    torch.cuda.synchronize()
+
+
+def test_scratch_is_taken_as_it_is_needed_and_kept(dev):
+    """By the native side and by the general one (which another number of pieces than a 16-bit one goes to): what there is serves smaller calls."""
+    from omni_npu_amd import kernels as K
+    c = make(dev, [300, 700, 64], hq=8, hk=2, seed=1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        held = [K.retained_workspace_bytes()]
+        for chunks in (9, 5, (1 << 16) + 5, 40, 9):
+            check(c, *call(dev, c, 1, num_chunks=chunks))
+            held.append(K.retained_workspace_bytes())
+    need = lambda n: K._lib.load().mlahip_gqa_decode_workspace_bytes(3, 1, 8, 128, n)
+    assert [b - a for a, b in zip(held, held[1:])] == [need(9), 0, need((1 << 16) + 5), 0, 0]
