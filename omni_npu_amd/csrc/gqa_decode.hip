@@ -818,7 +818,8 @@ int pick(const Params& p, int dim, bool fp8, int mt, int row_groups, unsigned x,
                                                                              : pick<T, 256>(p, fp8, mt, row_groups, x, st);
 }
 
-int64_t slots(int64_t batch, int64_t chunks) { return chunks > 0 ? batch + chunks : 0; }
+// Partial results that there may be: of one piece none, no request is cut.
+int64_t slots(int64_t batch, int64_t chunks) { return chunks > 1 ? batch + chunks : 0; }
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
 }  // namespace gqa

@@ -57,3 +57,17 @@ def test_scratch_is_taken_as_it_is_needed_and_kept(dev):
             held.append(K.retained_workspace_bytes())
     need = lambda n: K._lib.load().mlahip_gqa_decode_workspace_bytes(3, 1, 8, 128, n)
     assert [b - a for a, b in zip(held, held[1:])] == [need(9), 0, need((1 << 16) + 5), 0, 0]
+
+
+@pytest.mark.parametrize("lens,counts", [([500], [200]), ([500, 301, 0, 77], [150, 301, 0, 1]), ([90] * 70, [3] * 70)], ids=["one", "some", "many"])
+def test_one_piece_has_no_partial_results(dev, lens, counts):
+    """However many tokens and heads: its scratch memory goes by the requests, and nothing behind it is touched."""
+    from omni_npu_amd import kernels as K
+    need = K._lib.load().mlahip_gqa_decode_workspace_bytes
+    assert need(len(lens), 1 << 14, 64, 128, 1) == need(len(lens), 1, 1, 64, 1) <= 8 * len(lens) + 256
+    c = make(dev, lens, q_lens=counts, hq=6, hk=2, d=64, page=16, seed=4)
+    n = need(len(lens), max(counts), 6, 64, 1)
+    memory = torch.full((n + (1 << 20),), 77, dtype=torch.uint8, device=dev)
+    for window in (None, 60):
+        check(c, *call(dev, c, max(counts), varlen=True, num_chunks=1, window=window, workspace=memory[:n]), window=window)
+    assert (memory[n:] == 77).all()
