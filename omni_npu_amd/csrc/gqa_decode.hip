@@ -855,6 +855,8 @@ extern "C" int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_st
               "%s: %d pages of %d tokens a request (pages of a multiple of 16, at most 2^30 tokens)", me, max_blocks, page_size);
   MLA_REQUIRE((int64_t)batch * max_blocks * page_size < (1ll << 35) && num_chunks < (1 << 24), MLA_ERR_SHAPE,
               "%s: %d requests of up to %lld tokens in %d chunks are more than the plan counts", me, batch, (long long)max_blocks * page_size, num_chunks);
+  MLA_REQUIRE(query_start_loc || (int64_t)batch * max_q_len <= 0x7fffffff, MLA_ERR_SHAPE, "%s: %d requests of %d tokens: more than 2^31 - 1 rows", me,
+              batch, max_q_len);
   const int es = cache_dtype == 3 ? 1 : 2, unit = 16 / es;
   const int64_t c_strides = kc_page_stride | kc_row_stride | kc_head_stride | vc_page_stride | vc_row_stride | vc_head_stride;
   MLA_REQUIRE((q_stride_t | q_stride_h) % 8 == 0 && c_strides % unit == 0 && (out_stride_t | out_stride_h) % 4 == 0 &&
