@@ -602,7 +602,8 @@ int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, int
 /* ---- pages of a cache, any cache -------------------------------------------------------------
  * cache[dst[i], r] = cache[src[i], r] for r < rows[i] (rows = NULL: whole pages) in every cache of the list, in as few launches as
  * hold their arguments.  caches, src, dst and rows are HOST arrays, read before the call returns (a captured graph keeps the pairs of its
- * capture).  A destination named twice, or one that is a source too, is refused: the copies have no order.
+ * capture).  A destination named twice, or one that is a source too, is refused: the copies have no order.  So is a cache whose
+ * pages or rows share memory (rows lie inside pages, or pages inside rows).
  * block_table (device, int32, may be NULL; not beside rows): entries that name a source name its destination afterwards; a source named
  * twice is refused then. */
 typedef struct {

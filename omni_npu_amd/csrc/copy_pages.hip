@@ -132,6 +132,11 @@ extern "C" int mlahip_copy_pages(const mlahip_page_cache* caches, int32_t num_ca
                     c.row_bytes * page_size < (1ll << 31) && c.page_stride_bytes >= c.row_bytes,
                 MLA_ERR_SHAPE, "%s: cache %d: rows of %lld bytes, %lld apart, pages %lld apart", me, i, (long long)c.row_bytes,
                 (long long)c.row_stride_bytes, (long long)c.page_stride_bytes);
+    // rows inside pages, or pages inside rows
+    MLA_REQUIRE(num_pages == 1 || (page_size - 1) * c.row_stride_bytes + c.row_bytes <= c.page_stride_bytes ||
+                    (c.page_stride_bytes < c.row_stride_bytes && (num_pages - 1) * c.page_stride_bytes + c.row_bytes <= c.row_stride_bytes),
+                MLA_ERR_SHAPE, "%s: cache %d: pages that share memory: rows of %lld bytes, %lld apart, %d to a page, pages %lld apart", me, i,
+                (long long)c.row_bytes, (long long)c.row_stride_bytes, page_size, (long long)c.page_stride_bytes);
   }
   for (int32_t i = 0; i < num_pairs; i++) {
     MLA_REQUIRE(src[i] >= 0 && src[i] < num_pages && dst[i] >= 0 && dst[i] < num_pages, MLA_ERR_SHAPE,

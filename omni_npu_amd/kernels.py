@@ -1647,7 +1647,9 @@ def copy_pages(caches, src, dst, rows=None, block_table: Optional[torch.Tensor] 
     for c in caches:
         if c.dim() < 2 or c.shape[:2] != (pages, page) or pages < 1 or page < 1 or c[0, 0].numel() < 1 or not c[0, 0].is_contiguous():
             raise ValueError(f"{what}: caches must be [pages, page, ...] of the same pages with contiguous rows, got {tuple(c.shape)}")
-        if c.stride(0) < 1 and pages > 1 or c.stride(1) < 1 and page > 1:
+        width, (apart, rows_apart) = c[0, 0].numel(), c.stride()[:2]   # (rows inside pages, or pages inside rows)
+        if page > 1 and rows_apart < width or pages > 1 and (apart < width or apart < (page - 1) * rows_apart + width and
+                                                             rows_apart < (pages - 1) * apart + width):
             raise ValueError(f"{what}: a cache whose pages or rows share memory")
     for i, (a, z) in enumerate(zip(src, dst)):
         if not (0 <= a < pages and 0 <= z < pages):
