@@ -7,6 +7,12 @@ from tests.test_gqa_decode_gpu import call, check, make
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(scope="module")
+def side(dev):
+    """A stream without scratch memory; one for all, as torch hands out 32 in turn and other tests count on new ones too."""
+    return torch.cuda.Stream(dev)
+
+
 def _args(dev, b=2, hq=8, hk=2, d=128, page=32):
     z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16, device=dev)
     i = lambda *s: torch.ones(*s, dtype=torch.int32, device=dev)
@@ -15,26 +21,25 @@ def _args(dev, b=2, hq=8, hk=2, d=128, page=32):
 
 @pytest.mark.parametrize("form", [dict(d=96), dict(d=16), dict(b=65536), dict(page=24), dict(page=8)], ids=str)
 @pytest.mark.parametrize("chunks", [None, 8])
-def test_what_the_shapes_refuse(dev, form, chunks):
-    _refused(dev, _args(dev, **form), num_chunks=chunks)
+def test_what_the_shapes_refuse(dev, side, form, chunks):
+    _refused(dev, side, _args(dev, **form), num_chunks=chunks)
 
 
 @pytest.mark.parametrize("kw", [dict(num_chunks=1 << 24), dict(num_chunks=(1 << 24) - 1), dict(num_chunks=8, heads_per_group=3),
                                 dict(num_chunks=8, heads_per_group=8), dict(num_chunks=8, rows_per_group=48), dict(num_chunks=8, rows_per_group=0)], ids=str)
-def test_what_the_launch_refuses(dev, kw):
-    _refused(dev, _args(dev), **kw)
+def test_what_the_launch_refuses(dev, side, kw):
+    _refused(dev, side, _args(dev), **kw)
 
 
-def test_what_addresses_and_strides_refuse(dev):
+def test_what_addresses_and_strides_refuse(dev, side):
     args = _args(dev)
     odd = torch.zeros(2 * 8 * 128 + 1, dtype=torch.bfloat16, device=dev)[1:].view(2, 8, 128)
-    _refused(dev, [odd] + args[1:], num_chunks=8)
-    _refused(dev, args[:3] + [args[3][:1].expand(2, 100)] + args[4:], num_chunks=8)       # (rows that share their memory)
+    _refused(dev, side, [odd] + args[1:], num_chunks=8)
+    _refused(dev, side, args[:3] + [args[3][:1].expand(2, 100)] + args[4:], num_chunks=8)       # (rows that share their memory)
 
 
-def _refused(dev, args, **kw):
+def _refused(dev, side, args, **kw):
     from omni_npu_amd import kernels as K
-    side = torch.cuda.Stream()                                 # (no scratch memory yet)
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         before = K.retained_workspace_bytes()
@@ -44,11 +49,10 @@ def _refused(dev, args, **kw):
     torch.cuda.synchronize()
 
 
-def test_scratch_is_taken_as_it_is_needed_and_kept(dev):
+def test_scratch_is_taken_as_it_is_needed_and_kept(dev, side):
     """By the native side and by the general one (which another number of pieces than a 16-bit one goes to): what there is serves smaller calls."""
     from omni_npu_amd import kernels as K
     c = make(dev, [300, 700, 64], hq=8, hk=2, seed=1)
-    side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(side):
         held = [K.retained_workspace_bytes()]
