@@ -19,10 +19,10 @@
 //               neighbouring dims, even and odd ones into products of their own
 //   join        wavefronts of a head through LDS, then chunks of a sequence through the workspace, by a second launch
 //
-// Measured, split and join together: 64 requests x 4096-8192 keys x 32/8 heads of 128 (1630 MB) 250 us, 6.5 TB/s; one of 131 072 x 64/8 90 us,
-// 5.9; 128 x 2 tokens x 2048-16 384 keys x 64/8 over the 8-bit cache (2440 MB) 396 us, 6.15; 33 requests x the newest 1024 keys x 16/4 heads of
+// Measured, split and join together: 64 requests x 4096-8192 keys x 32/8 heads of 128 (1630 MB) 251 us, 6.5 TB/s; one of 131 072 x 64/8 90 us,
+// 5.9; 128 x 2 tokens x 2048-16 384 keys x 64/8 over the 8-bit cache (2440 MB) 397 us, 6.1; 33 requests x the newest 1024 keys x 16/4 heads of
 // 256, pages of 16 (137 MB) 34 us, 4.0: four wavefronts to a CU (a wavefront's sums, keys and values take 300 registers, a second workgroup would
-// not fit), five tiles each, and most chunks begin a second sequence.  One request x 1021 keys x 4/1 heads 8.4 us: 6.2 of the split, whose loads
+// not fit), five tiles each, and most chunks begin a second sequence.  One request x 1021 keys x 4/1 heads 8.7 us: 6.5 of the split, whose loads
 // hang on one another (length, page, keys and values, partial results), 2.2 of the join.
 #include <type_traits>
 
@@ -72,8 +72,9 @@ template <> struct Types<__bf16> {
     return __builtin_bit_cast(uint32_t, hi ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, true) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, false));
   }
   static constexpr uint32_t kOnes = 0x3f803f80u;
-  // log2 units: how far a row's reference is set below its largest score, and how far above that a later one may lie before it is set anew
-  static constexpr float kBelow = 0.f, kOutgrown = 8.f;
+  // log2 units: how far a row's reference is set below its largest score, and how far above that a later one may lie before it is set anew.
+  // Above it here, so that the largest scores' probabilities are 2^-24 to 2^-16: sums over values of any size stay finite.
+  static constexpr float kBelow = -24.f, kOutgrown = 8.f;
   static constexpr uint32_t kExp = 0x7f807f80u, kLow = 0x00800080u;   // a number's exponent bits and the lowest of them
 };
 template <> struct Types<_Float16> {
@@ -693,6 +694,8 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
 // several partials at once.  A wavefront goes by its own partials' largest log-sum-exp, so that all it reads of them is asked for together.
 // They are kept in log2 units: behind a product the compiler would subtract from the unrounded one, which is far off beyond 2^32.
 // Bound by the launch and two dependent reads: 2.2 us for 4 rows of 32 partials, 4.4 for 64 x 32 rows of 2 to 4, 8.4 for 128 x 128 of them, 45 MB.
+// A weight is at most 2^-24 (kFar), so that sums over results of any size stay finite.
+constexpr float kFar = 24.f;
 template <typename T, int D, int kWaves>
 __global__ __launch_bounds__(256) void gqa_join_kernel(const Params p) {
   __shared__ float part[4][D], stat[4][2];
@@ -721,14 +724,14 @@ __global__ __launch_bounds__(256) void gqa_join_kernel(const Params p) {
     }
 #pragma unroll
     for (int k = 0; k < 4; k++) next = fmaxf(next, l[k]);
-    const float ref = next == -INFINITY ? 0.f : next, f = fast_exp2(most - ref);   // (nothing so far: zeros)
+    const float ref = next == -INFINITY ? 0.f : next, f = fast_exp2(most - ref), far = ref + kFar;   // (nothing so far: zeros)
     sum *= f;
 #pragma unroll
     for (int e = 0; e < 4; e++) acc[e] *= f;
     most = next;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      const float wt = fast_exp2(l[k] - ref);
+      const float wt = fast_exp2(l[k] - far);
       sum += wt;
 #pragma unroll
       for (int e = 0; e < 4; e++) acc[e] += wt == 0.f ? 0.f : wt * a[k][e];
@@ -780,7 +783,7 @@ __global__ __launch_bounds__(256) void gqa_join_kernel(const Params p) {
 #pragma unroll
   for (int e = 0; e < 4; e++) y[e] = (T)(sum == 0.f ? 0.f : acc[e] / sum);
   *(typename Types<T>::v4*)(p.out + t * p.o_st + (int64_t)qh * p.o_sh + gi * 8) = y;
-  if (p.lse && gi == 0) p.lse[t * (p.kv_heads * p.group) + qh] = sum == 0.f ? -INFINITY : (top + fast_log2(sum)) * kLn2;
+  if (p.lse && gi == 0) p.lse[t * (p.kv_heads * p.group) + qh] = sum == 0.f ? -INFINITY : (top + (fast_log2(sum) + kFar)) * kLn2;
 }
 
 template <typename T, int D, bool kFp8, int MT>

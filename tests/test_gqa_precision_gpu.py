@@ -125,3 +125,17 @@ def test_pieces_with_scores_whose_steps_are_large(dev, dtype, scale, requests, c
     out, lse = call(dev, c, 1, num_chunks=chunks)
     assert torch.equal(out, c["v"][page, row].repeat_interleave(2, 1))
     assert torch.allclose(lse.double(), torch.tensor(32768.0 * 200 * scale, dtype=torch.float64), rtol=2.0 ** -21)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
+@pytest.mark.parametrize("lens,chunks", [([1, 2, 40, 700], 0), ([1, 2, 40, 700], 9), ([5000], 1), ([5000], 40), ([5000, 3000, 20], 30)])
+@pytest.mark.parametrize("d", [64, 256])
+def test_values_of_the_largest_size(dev, dtype, lens, chunks, d):
+    """All values are the type's largest, of one sign for a dim: so are the results, however many are summed and joined."""
+    c = make(dev, lens, hq=6, hk=2, d=d, dtype=dtype, page=16, seed=7)
+    sign = 1.0 - 2.0 * (torch.arange(d) % 2)
+    c["v"][...] = (sign * torch.finfo(dtype).max).to(dtype)
+    out, lse = call(dev, c, 1, num_chunks=chunks)
+    assert torch.equal(out, c["v"][0, 0, 0].expand_as(out))
+    o, l, weight, reach = H.gqa(c["q"], c["k"], torch.zeros_like(c["v"]), c["table"], c["lens"], c["scale"], c["start"])
+    assert ((lse.double() - l).abs() <= 1.01 * LEFT[dtype] + 5000 * 2.0 ** -24 + (d + 4) * 2.0 ** -24 * reach + 2.0 ** -18 * (1 + l.abs())).all()
