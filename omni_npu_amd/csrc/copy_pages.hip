@@ -7,7 +7,7 @@
 // the order of the copies does not matter.  Where a table follows, a source is named once too: a page moves to one place.
 //
 // What bounds it is memory, each byte read and written once; a workgroup copies a piece of one pair's page in one cache.  A launch of 32 MB or
-// more goes past the caches, which would give up other lines for it, in pieces of 4 KB: together in flight they are neighbours in memory.  us
+// more, filled rows counted as whole pages, goes past the caches, which would give up other lines for it, in pieces of 4 KB: together in flight they are neighbours in memory.  us
 // through the caches / past them, pieces of 4 KB / 32 KB, behind 2 GB of other writes: 63 MB (7 pairs x 34 caches) 37 / 27, 42 / 29; 418 MB 170 / 140, 185 /
 // 162; 2.5 GB 922 / 826, 1044 / 977.  Where the same pages are copied again and again, 47 MB 17.8 / 19.2, 105 MB 47 / 41, 2.5 GB 904 / 819 (6.1 TB/s read
 // and written; a plain copy of 2 GiB 4.9).  Smaller launches go through the caches, in pieces of 8 KB: 12 MB 5.6, past them 9.9.

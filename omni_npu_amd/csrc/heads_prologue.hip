@@ -15,7 +15,7 @@
 //
 // What bounds it is memory, every value read and written once: 16 384 tokens x 64 + 2 x 8 heads of 128 into the 8-bit cache (646 MB) take
 // 115 us, 5.6 TB/s (a copy of 2 GiB on this card: 4.94).  2999 tokens x 16 + 2 x 4 heads of 64 (19 MB) take 6.6 us, and 1 token 2.7, 64 tokens 2.8 in
-// a graph, which is a launch and three dependent reads (slot and position, table row, values).  Without the next head's values on their
+// a graph, which is a launch and two reads one behind the other (slot and position; then table row and values).  Without the next head's values on their
 // way 10 786 tokens x 8 + 2 x 8 heads of 256 took 72 us in place of 53; with the first key and value head of a group asked for in front of its queries
 // (80 registers in place of 60) 16 384 x 32 + 2 x 8 of 128 took 81 in place of 78.
 #include <type_traits>

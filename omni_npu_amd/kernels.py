@@ -1489,7 +1489,7 @@ def qk_norm_rope_cache(q: torch.Tensor, k: Optional[torch.Tensor], v: Optional[t
 def gqa_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, dim: int, element_bytes: int, max_seq_len: int):
     """(pieces that gqa_decode cuts the cached keys of a step into, key heads of a workgroup, rows of a workgroup); 0 pieces: a request to a
     workgroup, one launch.  The fastest by an estimate in us of what was measured (13 200 launches, 1-128 requests of 64-20 000 keys, heads
-    of 64-256 values, 1-8 of them, 1-64 rows; the estimate's choice is 1.1 % slower than the best one on average, 31 % at worst):
+    of 64-256 values, 1-8 of them, 1-64 rows; the estimate's choice is 1.1 % slower than the best one on average, 34 % at worst):
     a wavefront's step of 32 keys x 512 bytes takes 2.2, 15 % more with more than 16 rows, and a CU takes 31 KB per us from the memory (short
     contexts are bound by these: few heads to a workgroup, so that its wavefronts share their keys, and few rows, each workgroup reading the
     keys again); the cache stream 7.1 MB per us, 5 % less for each halving of a key's heads of a workgroup below 2 KB, a quarter longer for each
@@ -1544,8 +1544,8 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
     q [T,Hq,D] bf16 or fp16, D 64, 128 or 256; caches [pages, page, Hk, D] of its type or float8_e4m3fn (times ``k_scale`` /
     ``v_scale`` fp32 [Hk]), page a multiple of 16, any page / row / head strides of 16-byte multiples; query head h reads key head
     h // (Hq // Hk).  block_table int32 [B,maxblk], seq_lens int32 [B] on the device, the newest tokens included.  Sequence b owns
-    query tokens [b*q_len, (b+1)*q_len), or with query_start_loc (int32 [B+1], device) those, at most q_len of them; token i of s
-    sees keys [0, L - s + i], with ``window`` only the newest ``window`` of these.  ``out`` [T,Hq,D] like q; ``lse_out`` fp32
+    query tokens [b*q_len, (b+1)*q_len), or with query_start_loc (int32 [B+1], device) those, of which the first q_len are done; token i
+    of s sees keys [0, L - s + i], with ``window`` only the newest ``window`` of these.  ``out`` [T,Hq,D] like q; ``lse_out`` fp32
     [T,Hq].  A row without keys gives zeros and -inf; rows behind the last request stay as they were.  ``max_seq_len``: no request is
     longer (it shapes the launch; results are right without); under capture the table's room counts, as a graph is replayed over
     others.  Scratch memory is kept per stream: graphs captured on one stream share it and are replayed one after the other, or get a
