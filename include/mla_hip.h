@@ -599,6 +599,41 @@ int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, int
                       void* workspace, size_t workspace_bytes, int32_t num_chunks, int32_t heads_per_group,
                       int32_t rows_per_group, mlahip_stream_t stream);
 
+/* The same for tokens drafted as a tree: a request's newest s keys are its own tokens', and token i sees the context, j < seq_lens[b] - s, and of
+ * these keys the k-th where bit k % 64 of visible[t * visible_stride + k / 64] is set, k < 64 * words (1 to 8 words; bits past the request's own
+ * tokens are not looked at); with window > 0 only the newest ``window`` of all these keys.  A token's own key is one of its bits.  A request has as many
+ * tokens as are in the batch for it: max_q_len, or what query_start_loc says.  All else as above, the workspace's size too. */
+int mlahip_gqa_tree_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t num_tokens, const void* k_cache,
+                           int64_t kc_page_stride, int64_t kc_row_stride, int64_t kc_head_stride, const void* v_cache,
+                           int64_t vc_page_stride, int64_t vc_row_stride, int64_t vc_head_stride, int64_t num_pages,
+                           int32_t page_size, const int32_t* block_table, int64_t bt_stride, int32_t max_blocks,
+                           const int32_t* seq_lens, const int32_t* query_start_loc /* may be NULL */, const uint64_t* visible,
+                           int64_t visible_stride, int32_t words, int32_t batch, int32_t max_q_len, int32_t q_heads, int32_t kv_heads,
+                           int32_t dim, int32_t dtype, int32_t cache_dtype, const float* k_scale, const float* v_scale, float scale,
+                           int32_t window, void* out, int64_t out_stride_t, int64_t out_stride_h, float* lse_out, void* workspace,
+                           size_t workspace_bytes, int32_t num_chunks, int32_t heads_per_group, int32_t rows_per_group,
+                           mlahip_stream_t stream);
+
+/* ---- a step's tables, from its requests' lengths --------------------------------------------
+ * Request b has context_lens[b] cached tokens (negative: an idle place of the batch) and n new ones: q_len, or with query_start_loc [batch + 1] those
+ * from query_start_loc[b] to query_start_loc[b + 1].  All arrays on the device; one launch, or two.
+ * With num_blocks [batch], free_pages [capacity] and num_free [1] (all or none) the block tables [batch, max_blocks] follow the lengths: num_blocks[b] of a
+ * row's entries are the request's pages, free_pages[0 .. num_free) the list of free ones.  First pages that a request no longer needs (context + n tokens
+ * fit fewer; an idle place needs none) go back behind the list's end, the last one named first, so that they would be taken again in the order in which they
+ * were held; then pages are taken from the list's end, in the order of the requests.  A request whose table has no room, or for whom and those
+ * in front of it the list is too short, gets no page: its length stays context_lens[b] and its tokens get no slots.  A list without room for what
+ * comes back takes none of it from that request on.  Entries behind a request's pages are left as they were.
+ * seq_lens [batch]: context + n (idle: 0).  positions, slot_mapping [num_tokens] int64: token i's position context + i, and the cache row of place
+ * context + i by the block table, -1 where the table ends or names no page; rows behind the last request and an idle place's get 0 and -1.
+ * With parents [num_tokens] (a token's parent among its request's tokens, in front of it; anything else: it follows the context) positions are context +
+ * depth, and visible [num_tokens, words] (rows visible_stride apart) gets a bit for the token itself and for each of its ancestors, bit k % 64 of word k / 64
+ * for token k < 64 * words: mlahip_gqa_tree_decode's.  No result may share memory with another array of the call. */
+int mlahip_step_tables(const int32_t* context_lens, const int32_t* query_start_loc /* may be NULL */, int32_t batch, int32_t q_len,
+                       int32_t* block_table, int64_t bt_stride, int32_t max_blocks, int32_t page_size, int32_t* seq_lens,
+                       int64_t* positions, int64_t* slot_mapping, int64_t num_tokens, const int32_t* parents /* may be NULL */,
+                       uint64_t* visible, int64_t visible_stride, int32_t words, int32_t* num_blocks /* may be NULL */,
+                       int32_t* free_pages, int32_t* num_free, int32_t capacity, mlahip_stream_t stream);
+
 /* ---- pages of a cache, any cache -------------------------------------------------------------
  * cache[dst[i], r] = cache[src[i], r] for r < rows[i] (rows = NULL: whole pages) in every cache of the list, in as few launches as
  * hold their arguments.  caches, src, dst and rows are HOST arrays, read before the call returns (a captured graph keeps the pairs of its
@@ -613,6 +648,17 @@ typedef struct {
 int mlahip_copy_pages(const mlahip_page_cache* caches, int32_t num_caches, const int32_t* src, const int32_t* dst,
                       const int32_t* rows /* may be NULL */, int32_t num_pairs, int64_t num_pages, int32_t page_size,
                       int32_t* block_table, int64_t bt_stride, int32_t bt_rows, int32_t bt_cols, mlahip_stream_t stream);
+
+/* The rows of an accepted path moved up behind the context, in every cache of the list (HOST array, as above): row(context_lens[b] + d) =
+ * row(context_lens[b] + accepted[b][d]) for the first num_accepted[b] entries, at most max_accepted, of a row of accepted [batch, max_accepted] (rows
+ * accepted_stride apart), and kept_lens[b] = context_lens[b] + their number.  A path is numbers of the request's new tokens, each larger than the one before:
+ * it ends at its first entry that is not, that is no token of the request (context_lens[b] + it >= seq_lens[b]) or whose page, or the place's that it would
+ * go to, is not in the table or the cache.  Idle places (negative context) keep their length.  All but ``caches`` on the device; kept_lens shares
+ * no memory with what is read.  Requests must not share the pages that their new tokens lie in.  Rows of at most 2 MB. */
+int mlahip_keep_rows(const mlahip_page_cache* caches, int32_t num_caches, int64_t num_pages, int32_t page_size, const int32_t* block_table,
+                     int64_t bt_stride, int32_t max_blocks, const int32_t* context_lens, const int32_t* seq_lens, int32_t batch,
+                     const int32_t* accepted, int64_t accepted_stride, int32_t max_accepted, const int32_t* num_accepted, int32_t* kept_lens,
+                     mlahip_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -681,9 +681,9 @@ std::tuple<int, int, int> gqa_plan(int64_t batch, int64_t q_len, int64_t q_heads
   return {(int)std::get<1>(best), (int)std::get<2>(best), (int)std::get<3>(best)};
 }
 
-// kernels.gqa_decode
+// kernels.gqa_decode and, with bits, kernels.gqa_tree_decode
 using OptInt = std::optional<int64_t>;
-bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& seq_lens, double scale,
+bool gqa(const Tensor* bits, const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& seq_lens, double scale,
                 const Tensor& out, int64_t q_len, const OptTensor& qsl, OptInt window_keys, const OptTensor& k_scale, const OptTensor& v_scale,
                 const OptTensor& lse, OptInt num_chunks, OptInt max_seq_len, const OptTensor& workspace, OptInt heads_per_group, OptInt rows_per_group) {
   if (!current_gpu(q) || q.dim() != 3 || workspace || k_cache.dim() != 4) return false;
@@ -704,29 +704,76 @@ bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, c
     return false;
   const bool fp8 = k_cache.scalar_type() == at::kFloat8_e4m3fn;
   if (!head_scale(k_scale, fp8, hk, dev) || !head_scale(v_scale, fp8, hk, dev) || wants_grad({&q, &k_cache, &v_cache})) return false;
+  if (bits && !(bits->scalar_type() == at::kLong && bits->dim() == 2 && bits->device() == dev && bits->size(0) == t && bits->size(1) >= 1 &&
+                bits->size(1) <= 8 && (bits->size(1) == 1 || bits->stride(1) == 1) && q_len <= 64 * bits->size(1)))
+    return false;
   int64_t longest = block_table.size(1) * k_cache.size(1);
   if (max_seq_len && c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) longest = std::min(longest, *max_seq_len);
-  if (window > 0) longest = std::min(longest, window + q_len + 30);
+  if (window > 0) longest = std::min(longest, window + q_len + (bits ? 31 : 30));
   const auto [by_rule, heads, rows] = gqa_plan(b, q_len, hq, hk, d, k_cache.element_size(), longest);
   const int chunks = (int)num_chunks.value_or(by_rule);
   Stream st = stream_of(q);
+  const char* what = bits ? "mlahip_gqa_tree_decode" : "mlahip_gqa_decode";
   const int64_t need = (int64_t)mlahip_gqa_decode_workspace_bytes((int)b, (int)q_len, (int)hq, (int)d, chunks);
   const auto launch = [&](const Tensor* ws) {
-    return mlahip_gqa_decode(q.data_ptr(), q.stride(0), q.stride(1), t, k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2),
-                             v_cache.data_ptr(), v_cache.stride(0), v_cache.stride(1), v_cache.stride(2), k_cache.size(0), (int)k_cache.size(1),
-                             (const int32_t*)block_table.data_ptr(), block_table.stride(0), (int)block_table.size(1),
-                             (const int32_t*)seq_lens.data_ptr(), (const int32_t*)data_of(qsl), (int)b, (int)q_len, (int)hq, (int)hk, (int)d,
-                             type_code(dt), type_code(k_cache.scalar_type()), (const float*)data_of(k_scale), (const float*)data_of(v_scale),
-                             (float)scale, (int)window, out.data_ptr(), out.stride(0), out.stride(1), (float*)data_of(lse),
-                             ws ? ws->data_ptr() : nullptr, ws ? (size_t)ws->numel() : 0, chunks, (int)heads_per_group.value_or(heads),
-                             (int)rows_per_group.value_or(rows), st);
+    const auto run = [&](auto fn, auto... words) {
+      return fn(q.data_ptr(), q.stride(0), q.stride(1), t, k_cache.data_ptr(), k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), v_cache.data_ptr(),
+                v_cache.stride(0), v_cache.stride(1), v_cache.stride(2), k_cache.size(0), (int)k_cache.size(1), (const int32_t*)block_table.data_ptr(),
+                block_table.stride(0), (int)block_table.size(1), (const int32_t*)seq_lens.data_ptr(), (const int32_t*)data_of(qsl), words..., (int)b,
+                (int)q_len, (int)hq, (int)hk, (int)d, type_code(dt), type_code(k_cache.scalar_type()), (const float*)data_of(k_scale),
+                (const float*)data_of(v_scale), (float)scale, (int)window, out.data_ptr(), out.stride(0), out.stride(1), (float*)data_of(lse),
+                ws ? ws->data_ptr() : nullptr, ws ? (size_t)ws->numel() : 0, chunks, (int)heads_per_group.value_or(heads),
+                (int)rows_per_group.value_or(rows), st);
+    };
+    return bits ? run(mlahip_gqa_tree_decode, (const uint64_t*)bits->data_ptr(), bits->stride(0), (int)bits->size(1)) : run(mlahip_gqa_decode);
   };
   // More scratch memory than there is, which is kept, is asked for when nothing but it is missing.
   if (need && !has_scratch(q, st, need, 3)) {
     const int rc = launch(nullptr);
-    if (rc != kNoWorkspace) return done(rc, "mlahip_gqa_decode");
+    if (rc != kNoWorkspace) return done(rc, what);
   }
-  return done(launch(need ? &scratch(q, st, need, 3) : nullptr), "mlahip_gqa_decode");
+  return done(launch(need ? &scratch(q, st, need, 3) : nullptr), what);
+}
+bool gqa_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& seq_lens, double scale,
+                const Tensor& out, int64_t q_len, const OptTensor& qsl, OptInt window, const OptTensor& k_scale, const OptTensor& v_scale,
+                const OptTensor& lse, OptInt num_chunks, OptInt max_seq_len, const OptTensor& workspace, OptInt heads_per_group, OptInt rows_per_group) {
+  return gqa(nullptr, q, k_cache, v_cache, block_table, seq_lens, scale, out, q_len, qsl, window, k_scale, v_scale, lse, num_chunks, max_seq_len, workspace,
+             heads_per_group, rows_per_group);
+}
+bool gqa_tree_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& block_table, const Tensor& seq_lens,
+                     const Tensor& visible, double scale, const Tensor& out, int64_t q_len, const OptTensor& qsl, OptInt window, const OptTensor& k_scale,
+                     const OptTensor& v_scale, const OptTensor& lse, OptInt num_chunks, OptInt max_seq_len, const OptTensor& workspace,
+                     OptInt heads_per_group, OptInt rows_per_group) {
+  return gqa(&visible, q, k_cache, v_cache, block_table, seq_lens, scale, out, q_len, qsl, window, k_scale, v_scale, lse, num_chunks, max_seq_len, workspace,
+             heads_per_group, rows_per_group);
+}
+
+// kernels.step_tables
+bool step_tables(const Tensor& context, const Tensor& table, int64_t page_size, const Tensor& lens, const Tensor& positions, const Tensor& slots,
+                 int64_t q_len, const OptTensor& qsl, const OptTensor& parents, const OptTensor& visible, const OptTensor& num_blocks,
+                 const OptTensor& free_pages, const OptTensor& num_free) {
+  if (!current_gpu(context)) return false;
+  const at::Device dev = context.device();
+  const int64_t b = context.numel(), t = slots.numel();
+  const auto row = [&](const Tensor& x, at::ScalarType type, int64_t n) {
+    return x.scalar_type() == type && x.dim() == 1 && x.numel() == n && x.is_contiguous() && x.device() == dev;
+  };
+  if (page_size < 1 || page_size > 0x7fffffff || q_len < 1 || q_len > 0x7fffffff || !row(context, at::kInt, b) || !row(lens, at::kInt, b) ||
+      !row(positions, at::kLong, t) || !row(slots, at::kLong, t) || (qsl && !row(*qsl, at::kInt, b + 1)) || (parents && !row(*parents, at::kInt, t)) ||
+      (num_blocks && !row(*num_blocks, at::kInt, b)) || (num_free && !row(*num_free, at::kInt, 1)) ||
+      (free_pages && !row(*free_pages, at::kInt, free_pages->numel())) || !is_i32(table, 2, dev) || table.size(0) < b || table.size(1) < 1 ||
+      parents.has_value() != visible.has_value() || num_blocks.has_value() != free_pages.has_value() || num_blocks.has_value() != num_free.has_value())
+    return false;
+  const bool bits = visible.has_value();
+  if (bits && !(visible->scalar_type() == at::kLong && visible->dim() == 2 && visible->device() == dev && visible->size(0) == t && visible->size(1) >= 1 &&
+                visible->size(1) <= 0x7fffffff && (visible->size(1) == 1 || visible->stride(1) == 1)))
+    return false;
+  if (b > 0x7fffffff || t > 0x7fffffff || table.size(1) > 0x7fffffff || (free_pages && free_pages->numel() > 0x7fffffff)) return false;
+  return done(mlahip_step_tables((const int32_t*)context.data_ptr(), (const int32_t*)data_of(qsl), (int)b, (int)q_len, (int32_t*)table.data_ptr(),
+                                 table.stride(0), (int)table.size(1), (int)page_size, (int32_t*)lens.data_ptr(), (int64_t*)positions.data_ptr(),
+                                 (int64_t*)slots.data_ptr(), t, (const int32_t*)data_of(parents), (uint64_t*)data_of(visible), bits ? visible->stride(0) : 0,
+                                 bits ? (int)visible->size(1) : 0, (int32_t*)data_of(num_blocks), (int32_t*)data_of(free_pages), (int32_t*)data_of(num_free),
+                                 free_pages ? (int)free_pages->numel() : 0, stream_of(context)), "mlahip_step_tables");
 }
 
 // kernels.copy_pages
@@ -744,15 +791,40 @@ bool whole_numbers(py::handle list, std::vector<int32_t>& to) {
   }
   return true;
 }
-bool copy_pages(py::handle cache_list, py::handle src_list, py::handle dst_list, py::handle rows_list, const OptTensor& table) {
+// The caches of a list as the library takes them; empty where they are not what it knows.
+struct Caches { std::vector<mlahip_page_cache> list; const Tensor* first = nullptr; };
+Caches page_caches(py::handle cache_list) {
+  Caches to;
   // (the list's own tensors: a vector of them would count references up and down)
-  if (!PyList_CheckExact(cache_list.ptr())) return false;
+  if (!PyList_CheckExact(cache_list.ptr())) return to;
   const Py_ssize_t num = PyList_GET_SIZE(cache_list.ptr());
   for (Py_ssize_t i = 0; i < num; i++)
-    if (!THPVariable_Check(PyList_GET_ITEM(cache_list.ptr(), i))) return false;
+    if (!THPVariable_Check(PyList_GET_ITEM(cache_list.ptr(), i))) return to;
   auto cache = [&](Py_ssize_t i) -> const Tensor& { return THPVariable_Unpack(PyList_GET_ITEM(cache_list.ptr(), i)); };
-  if (num == 0 || !current_gpu(cache(0))) return false;
+  if (num == 0 || !current_gpu(cache(0))) return to;
   const Tensor& first = cache(0);
+  to.list.reserve(num);
+  for (Py_ssize_t k = 0; k < num; k++) {
+    const Tensor& c = cache(k);
+    if (c.dim() < 2 || c.device() != first.device() || c.size(0) < 1 || c.size(1) < 1 || c.size(0) != first.size(0) || c.size(1) != first.size(1) ||
+        wants_grad({&c}))
+      return Caches{};
+    int64_t width = 1;
+    for (int64_t i = c.dim() - 1; i >= 2; i--) {               // (rows of contiguous elements)
+      if (c.size(i) != 1 && c.stride(i) != width) return Caches{};
+      width *= c.size(i);
+    }
+    // (the stride of a dim of one entry says nothing)
+    const int64_t es = c.element_size(), row = width * es, row_stride = c.size(1) > 1 ? c.stride(1) * es : row;
+    to.list.push_back({c.data_ptr(), c.size(0) > 1 ? c.stride(0) * es : row_stride * c.size(1), row_stride, row});
+  }
+  to.first = &first;
+  return to;
+}
+bool copy_pages(py::handle cache_list, py::handle src_list, py::handle dst_list, py::handle rows_list, const OptTensor& table) {
+  const Caches caches = page_caches(cache_list);
+  if (!caches.first) return false;
+  const Tensor& first = *caches.first;
   const at::Device dev = first.device();
   std::vector<int32_t> src, dst, rows;
   const bool part = !rows_list.is_none();
@@ -762,26 +834,29 @@ bool copy_pages(py::handle cache_list, py::handle src_list, py::handle dst_list,
   if (table && (table->scalar_type() != at::kInt || table->dim() != 2 || table->device() != dev || (table->size(1) > 1 && table->stride(1) != 1) ||
                 (table->size(0) > 1 && table->stride(0) < table->size(1))))
     return false;
-  std::vector<mlahip_page_cache> list;
-  list.reserve(num);
-  for (Py_ssize_t k = 0; k < num; k++) {
-    const Tensor& c = cache(k);
-    if (c.dim() < 2 || c.device() != dev || c.size(0) < 1 || c.size(1) < 1 || c.size(0) != first.size(0) || c.size(1) != first.size(1) ||
-        wants_grad({&c}))
-      return false;
-    int64_t width = 1;
-    for (int64_t i = c.dim() - 1; i >= 2; i--) {               // (rows of contiguous elements)
-      if (c.size(i) != 1 && c.stride(i) != width) return false;
-      width *= c.size(i);
-    }
-    // (the stride of a dim of one entry says nothing)
-    const int64_t es = c.element_size(), row = width * es, row_stride = c.size(1) > 1 ? c.stride(1) * es : row;
-    list.push_back({c.data_ptr(), c.size(0) > 1 ? c.stride(0) * es : row_stride * c.size(1), row_stride, row});
-  }
-  return done(mlahip_copy_pages(list.data(), (int)list.size(), src.data(), dst.data(), part ? rows.data() : nullptr, (int)src.size(),
+  return done(mlahip_copy_pages(caches.list.data(), (int)caches.list.size(), src.data(), dst.data(), part ? rows.data() : nullptr, (int)src.size(),
                                 first.size(0), (int)first.size(1), table ? (int32_t*)table->data_ptr() : nullptr,
                                 table ? (table->size(0) > 1 ? table->stride(0) : table->size(1)) : 0, table ? (int)table->size(0) : 0,
                                 table ? (int)table->size(1) : 0, stream_of(first)), "mlahip_copy_pages");
+}
+
+// kernels.keep_rows
+bool keep_rows(py::handle cache_list, const Tensor& table, const Tensor& context, const Tensor& lens, const Tensor& accepted, const Tensor& num,
+               const Tensor& kept) {
+  const Caches caches = page_caches(cache_list);
+  if (!caches.first) return false;
+  const Tensor& first = *caches.first;
+  const at::Device dev = first.device();
+  const int64_t b = context.numel();
+  for (const Tensor* x : {&context, &lens, &num, &kept})
+    if (!is_i32(*x, 1, dev) || x->numel() != b || !x->is_contiguous()) return false;
+  if (!is_i32(table, 2, dev) || table.size(0) < b || table.size(1) < 1 || !is_i32(accepted, 2, dev) || accepted.size(0) < b || b > 0x7fffffff ||
+      table.size(1) > 0x7fffffff || accepted.size(1) > 0x7fffffff)
+    return false;
+  return done(mlahip_keep_rows(caches.list.data(), (int)caches.list.size(), first.size(0), (int)first.size(1), (const int32_t*)table.data_ptr(),
+                               table.stride(0), (int)table.size(1), (const int32_t*)context.data_ptr(), (const int32_t*)lens.data_ptr(), (int)b,
+                               (const int32_t*)accepted.data_ptr(), accepted.stride(0), (int)accepted.size(1), (const int32_t*)num.data_ptr(),
+                               (int32_t*)kept.data_ptr(), stream_of(first)), "mlahip_keep_rows");
 }
 
 }  // namespace
@@ -798,7 +873,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("dsa_select_prompts", &dsa_select_prompts);
   m.def("qk_norm_rope_cache", &qk_norm_rope_cache);
   m.def("gqa_decode", &gqa_decode);
+  m.def("gqa_tree_decode", &gqa_tree_decode);
+  m.def("step_tables", &step_tables);
   m.def("copy_pages", &copy_pages);
+  m.def("keep_rows", &keep_rows);
   // (what this file has a copy of, for a test to hold against kernels.py)
   m.def("launch_splits", &launch_splits, py::arg("batch"), py::arg("q_len"), py::arg("heads"), py::arg("max_seq_len"), py::arg("full") = false);
   m.def("gqa_plan", &gqa_plan);

@@ -1550,11 +1550,37 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
     longer (it shapes the launch; results are right without); under capture the table's room counts, as a graph is replayed over
     others.  Scratch memory is kept per stream: graphs captured on one stream share it and are replayed one after the other, or get a
     ``workspace`` each (mlahip_gqa_decode_workspace_bytes)."""
-    what = "gqa_decode"
-    if _host.load().gqa_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out, q_len, query_start_loc,
-                               window, k_scale, v_scale, lse_out, num_chunks, max_seq_len, workspace, heads_per_group, rows_per_group):
-        return out
-    dev = _one_device(what, q, k_cache, v_cache, block_table, seq_lens, out, query_start_loc, k_scale, v_scale, lse_out, workspace)
+    if not _host.load().gqa_decode(q, k_cache, v_cache, block_table, seq_lens, scale, out, q_len, query_start_loc,
+                                   window, k_scale, v_scale, lse_out, num_chunks, max_seq_len, workspace, heads_per_group, rows_per_group):
+        _gqa("gqa_decode", q, k_cache, v_cache, block_table, seq_lens, None, scale, out, q_len, query_start_loc, window, k_scale, v_scale,
+             lse_out, num_chunks, max_seq_len, workspace, heads_per_group, rows_per_group)
+    return out
+
+
+def gqa_tree_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                    visible: torch.Tensor, scale: float, out: torch.Tensor, q_len: int = 1, query_start_loc: Optional[torch.Tensor] = None,
+                    window: Optional[int] = None, k_scale: Optional[torch.Tensor] = None, v_scale: Optional[torch.Tensor] = None,
+                    lse_out: Optional[torch.Tensor] = None, num_chunks: Optional[int] = None, max_seq_len: Optional[int] = None,
+                    workspace: Optional[torch.Tensor] = None, heads_per_group: Optional[int] = None,
+                    rows_per_group: Optional[int] = None) -> torch.Tensor:
+    """gqa_decode for tokens drafted as a tree: each sees the whole context and, of its request's own tokens, those that its bits name.
+
+    Arguments as gqa_decode's, and ``visible`` int64 [T,W], W 1 to 8 with contiguous rows: bit k % 64 of visible[t, k // 64] is set where token t
+    sees the request's k-th new token, its own key among them (step_tables makes them of the tokens' parents).  A request of s tokens has
+    its context in the places [0, L - s) and its tokens' keys behind it, in their order; at most 64 W tokens.  With ``window`` a token sees
+    the newest ``window`` of its keys: the bits' first, then the context's."""
+    if not _host.load().gqa_tree_decode(q, k_cache, v_cache, block_table, seq_lens, visible, scale, out, q_len, query_start_loc,
+                                        window, k_scale, v_scale, lse_out, num_chunks, max_seq_len, workspace, heads_per_group, rows_per_group):
+        _gqa("gqa_tree_decode", q, k_cache, v_cache, block_table, seq_lens, visible, scale, out, q_len, query_start_loc, window, k_scale, v_scale,
+             lse_out, num_chunks, max_seq_len, workspace, heads_per_group, rows_per_group)
+    return out
+
+
+def _gqa(what, q, k_cache, v_cache, block_table, seq_lens, visible, scale, out, q_len, query_start_loc, window, k_scale, v_scale, lse_out,
+         num_chunks, max_seq_len, workspace, heads_per_group, rows_per_group) -> None:
+    """The general path of both: every check by name, then the library."""
+    tree = what == "gqa_tree_decode"
+    dev = _one_device(what, q, k_cache, v_cache, block_table, seq_lens, out, query_start_loc, k_scale, v_scale, lse_out, workspace, visible)
     _no_grad(what, q, k_cache, v_cache)
     if q.dim() != 3 or q.dtype not in _HEAD_DT or q.stride(2) != 1 or out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1:
         raise ValueError(f"{what}: q and out must be bf16 or fp16 [T, Hq, D] with contiguous last dims, got {q.dtype} {tuple(q.shape)}, "
@@ -1590,31 +1616,112 @@ def gqa_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, bl
         raise ValueError(f"{what}: query_start_loc must be contiguous int32 [{b + 1}]")
     if lse_out is not None and (lse_out.dtype != torch.float32 or lse_out.shape != (t, hq) or not lse_out.is_contiguous()):
         raise ValueError(f"{what}: lse_out must be contiguous fp32 [{t}, {hq}]")
+    if tree and (visible is None or visible.dtype != torch.int64 or visible.dim() != 2 or visible.shape[0] != t or
+                 not 1 <= visible.shape[1] <= 8 or visible.stride(1) != 1 and visible.shape[1] > 1):
+        raise ValueError(f"{what}: visible must be int64 [{t}, W] with 1 to 8 words in contiguous rows"
+                         + ("" if visible is None else f", got {visible.dtype} {tuple(visible.shape)}"))
+    if tree and q_len > 64 * visible.shape[1]:
+        raise ValueError(f"{what}: {visible.shape[1]} words hold no bits for {q_len} tokens")
     scales = _head_scales(what, code == _E4M3, hk, k_scale=k_scale, v_scale=v_scale)
     if t == 0 or b == 0:
-        return out
+        return
     lib = _lib.load()
+    entry = lib.mlahip_gqa_tree_decode if tree else lib.mlahip_gqa_decode
+    bits = (visible.data_ptr(), visible.stride(0), visible.shape[1]) if tree else ()
     with torch.cuda.device(dev):
         longest = block_table.shape[1] * k_cache.shape[1]
         if max_seq_len is not None and not torch.cuda.is_current_stream_capturing():
             longest = min(longest, max_seq_len)
         if window is not None:
-            longest = min(longest, window + q_len + 30)
+            longest = min(longest, window + q_len + 30 + tree)
         chunks, heads, rows = gqa_plan(b, q_len, hq, hk, d, k_cache.element_size(), longest)
         num_chunks = chunks if num_chunks is None else num_chunks
         need = lib.mlahip_gqa_decode_workspace_bytes(b, q_len, hq, d, num_chunks)
-        launch = lambda ws: lib.mlahip_gqa_decode(
+        launch = lambda ws: entry(
             q.data_ptr(), q.stride(0), q.stride(1), t, k_cache.data_ptr(), *k_cache.stride()[:3], v_cache.data_ptr(), *v_cache.stride()[:3],
             k_cache.shape[0], k_cache.shape[1], block_table.data_ptr(), block_table.stride(0), block_table.shape[1], seq_lens.data_ptr(),
-            query_start_loc.data_ptr() if query_start_loc is not None else None, b, q_len, hq, hk, d, _HEAD_DT[q.dtype], code, *scales,
+            query_start_loc.data_ptr() if query_start_loc is not None else None, *bits, b, q_len, hq, hk, d, _HEAD_DT[q.dtype], code, *scales,
             float(scale), min(window or 0, 0x7fffffff), out.data_ptr(), out.stride(0), out.stride(1), lse_out.data_ptr() if lse_out is not None else None,
             ws.data_ptr() if ws is not None else None, ws.numel() * ws.element_size() if ws is not None else 0, num_chunks,
             heads if heads_per_group is None else heads_per_group, rows if rows_per_group is None else rows_per_group, _stream(q))
         rc = launch(workspace)
         if rc == _lib.ERR_WORKSPACE and workspace is None:     # (nothing but it is missing: a call that is refused takes none)
             rc = launch(_workspace(dev, need, "gqa"))
-    _lib.check(rc, "mlahip_gqa_decode")
-    return out
+    _lib.check(rc, "mlahip_" + what)
+
+
+def step_tables(context_lens: torch.Tensor, block_table: torch.Tensor, page_size: int, seq_lens: torch.Tensor, positions: torch.Tensor,
+                slot_mapping: torch.Tensor, q_len: int = 1, query_start_loc: Optional[torch.Tensor] = None,
+                parents: Optional[torch.Tensor] = None, visible: Optional[torch.Tensor] = None, num_blocks: Optional[torch.Tensor] = None,
+                free_pages: Optional[torch.Tensor] = None, num_free: Optional[torch.Tensor] = None) -> None:
+    """What a step reads besides its queries, made on the GPU from its requests' lengths: no host in between, so steps can follow each other in a graph.
+
+    Request b has context_lens[b] cached tokens (int32 [B]; negative: an idle place) and q_len new ones, or those of ``query_start_loc``
+    (int32 [B+1]).  Written: ``seq_lens`` int32 [B], context and new tokens; ``positions`` and ``slot_mapping`` int64 [T], what
+    qk_norm_rope_cache and cache_write take: 0 and -1 for rows behind the last request and of idle places, -1 for places that the
+    ``block_table`` (int32 [>= B, blocks], pages of ``page_size`` tokens) has no page for.
+    With ``num_blocks`` int32 [B], ``free_pages`` int32 [pages] and ``num_free`` int32 [1] the block table is kept as well: pages that a request
+    needs are taken from the end of free_pages[:num_free], in the order of the requests, those that it needs no more go back there first, so that they
+    would come out again in their order.  A request that the table or the list has too few pages for keeps the length of its context and gets no slots, and
+    so does every one behind it that needs pages, where the list is short.
+    With ``parents`` int32 [T], a token's parent among its request's tokens (in front of it; anything else: the token follows the context),
+    positions go by the depth, and ``visible`` int64 [T,W] gets the bits of the token and its ancestors, for gqa_tree_decode."""
+    what = "step_tables"
+    if _host.load().step_tables(context_lens, block_table, page_size, seq_lens, positions, slot_mapping, q_len, query_start_loc, parents, visible,
+                                num_blocks, free_pages, num_free):
+        return
+    dev = _one_device(what, context_lens, block_table, seq_lens, positions, slot_mapping, query_start_loc, parents, visible, num_blocks, free_pages,
+                      num_free)
+    b, t = context_lens.numel(), slot_mapping.numel()
+    if not 1 <= page_size <= 0x7fffffff or not 1 <= q_len <= 0x7fffffff:
+        raise ValueError(f"{what}: pages of {page_size}, {q_len} tokens a request")
+    for name, x, dtype, n in (("context_lens", context_lens, torch.int32, b), ("seq_lens", seq_lens, torch.int32, b),
+                              ("positions", positions, torch.int64, t), ("slot_mapping", slot_mapping, torch.int64, t),
+                              ("query_start_loc", query_start_loc, torch.int32, b + 1), ("parents", parents, torch.int32, t),
+                              ("num_blocks", num_blocks, torch.int32, b), ("num_free", num_free, torch.int32, 1),
+                              ("free_pages", free_pages, torch.int32, 0 if free_pages is None else free_pages.numel())):
+        if x is not None and (x.dtype != dtype or x.dim() != 1 or x.numel() != n or not x.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be contiguous {dtype} [{n}], got {x.dtype} {tuple(x.shape)}")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] < b or block_table.shape[1] < 1 or \
+            block_table.stride(1) != 1 and block_table.shape[1] > 1:
+        raise ValueError(f"{what}: block_table must be int32 [>= {b}, blocks] with contiguous rows")
+    if (parents is None) != (visible is None):
+        raise ValueError(f"{what}: parents and visible go together")
+    if (num_blocks is None) != (free_pages is None) or (num_blocks is None) != (num_free is None):
+        raise ValueError(f"{what}: num_blocks, free_pages and num_free go together")
+    if visible is not None and (visible.dtype != torch.int64 or visible.dim() != 2 or visible.shape[0] != t or visible.shape[1] < 1 or
+                                visible.stride(1) != 1 and visible.shape[1] > 1):
+        raise ValueError(f"{what}: visible must be int64 [{t}, words] with contiguous rows, got {visible.dtype} {tuple(visible.shape)}")
+    if query_start_loc is None and t < b * q_len:
+        raise ValueError(f"{what}: {t} places for {b} requests of {q_len} tokens")
+    if visible is not None and query_start_loc is None and q_len > 64 * visible.shape[1]:
+        raise ValueError(f"{what}: {visible.shape[1]} words hold no bits for {q_len} tokens")
+    ptr = lambda x: x.data_ptr() if x is not None else None
+    with torch.cuda.device(dev):
+        rc = _lib.load().mlahip_step_tables(
+            context_lens.data_ptr(), ptr(query_start_loc), b, q_len, block_table.data_ptr(), block_table.stride(0), block_table.shape[1], page_size,
+            seq_lens.data_ptr(), positions.data_ptr(), slot_mapping.data_ptr(), t, ptr(parents), ptr(visible),
+            visible.stride(0) if visible is not None else 0, visible.shape[1] if visible is not None else 0, ptr(num_blocks), ptr(free_pages),
+            ptr(num_free), free_pages.numel() if free_pages is not None else 0, _stream(context_lens))
+    _lib.check(rc, "mlahip_step_tables")
+
+
+def _page_caches(what: str, caches: list):
+    """The list as the library takes it, checked, and the caches' pages and tokens of a page."""
+    _no_grad(what, *caches)
+    pages, page = caches[0].shape[:2] if caches[0].dim() >= 2 else (0, 0)
+    for c in caches:
+        if c.dim() < 2 or c.shape[:2] != (pages, page) or pages < 1 or page < 1 or c[0, 0].numel() < 1 or not c[0, 0].is_contiguous():
+            raise ValueError(f"{what}: caches must be [pages, page, ...] of the same pages with contiguous rows, got {tuple(c.shape)}")
+        width, (apart, rows_apart) = c[0, 0].numel(), c.stride()[:2]   # (rows inside pages, or pages inside rows)
+        if page > 1 and rows_apart < width or pages > 1 and (apart < width or apart < (page - 1) * rows_apart + width and
+                                                             rows_apart < (pages - 1) * apart + width):
+            raise ValueError(f"{what}: a cache whose pages or rows share memory")
+    row_bytes = [math.prod(c.shape[2:]) * c.element_size() for c in caches]
+    geometry = [(c.stride(0) * c.element_size() if pages > 1 else w * page, c.stride(1) * c.element_size() if page > 1 else w, w)
+                for c, w in zip(caches, row_bytes)]
+    words = (ctypes.c_int64 * (4 * len(caches)))(*(x for c, geo in zip(caches, geometry) for x in (c.data_ptr(), *geo)))
+    return words, pages, page
 
 
 def copy_pages(caches, src, dst, rows=None, block_table: Optional[torch.Tensor] = None) -> None:
@@ -1642,15 +1749,7 @@ def copy_pages(caches, src, dst, rows=None, block_table: Optional[torch.Tensor] 
         raise ValueError(f"{what}: {len(caches)} caches, {len(src)} sources, {len(dst)} destinations"
                          + (f", {len(rows)} row counts" if rows is not None else ""))
     dev = _one_device(what, *caches, block_table)
-    _no_grad(what, *caches)
-    pages, page = caches[0].shape[:2] if caches[0].dim() >= 2 else (0, 0)
-    for c in caches:
-        if c.dim() < 2 or c.shape[:2] != (pages, page) or pages < 1 or page < 1 or c[0, 0].numel() < 1 or not c[0, 0].is_contiguous():
-            raise ValueError(f"{what}: caches must be [pages, page, ...] of the same pages with contiguous rows, got {tuple(c.shape)}")
-        width, (apart, rows_apart) = c[0, 0].numel(), c.stride()[:2]   # (rows inside pages, or pages inside rows)
-        if page > 1 and rows_apart < width or pages > 1 and (apart < width or apart < (page - 1) * rows_apart + width and
-                                                             rows_apart < (pages - 1) * apart + width):
-            raise ValueError(f"{what}: a cache whose pages or rows share memory")
+    words, pages, page = _page_caches(what, caches)
     for i, (a, z) in enumerate(zip(src, dst)):
         if not (0 <= a < pages and 0 <= z < pages):
             raise ValueError(f"{what}: pair {i} copies page {a} to {z} of {pages}")
@@ -1668,12 +1767,43 @@ def copy_pages(caches, src, dst, rows=None, block_table: Optional[torch.Tensor] 
             raise ValueError(f"{what}: block_table must be int32 [requests, blocks] with contiguous rows")
     if not src:
         return
-    row_bytes = [math.prod(c.shape[2:]) * c.element_size() for c in caches]
-    geometry = [(c.stride(0) * c.element_size() if pages > 1 else w * page, c.stride(1) * c.element_size() if page > 1 else w, w)
-                for c, w in zip(caches, row_bytes)]
-    words = (ctypes.c_int64 * (4 * len(caches)))(*(x for c, geo in zip(caches, geometry) for x in (c.data_ptr(), *geo)))
     ints = lambda x: None if x is None else (ctypes.c_int32 * len(x))(*x)
     table = (None, 0, 0, 0) if block_table is None else (block_table.data_ptr(), max(block_table.stride(0), block_table.shape[1]), *block_table.shape)
     with torch.cuda.device(dev):
         rc = _lib.load().mlahip_copy_pages(words, len(caches), ints(src), ints(dst), ints(rows), len(src), pages, page, *table, _stream(caches[0]))
     _lib.check(rc, "mlahip_copy_pages")
+
+
+def keep_rows(caches, block_table: torch.Tensor, context_lens: torch.Tensor, seq_lens: torch.Tensor, accepted: torch.Tensor,
+              num_accepted: torch.Tensor, kept_lens: torch.Tensor) -> None:
+    """The rows of an accepted path moved up behind the context, in every cache of the list (all layers', as copy_pages takes them):
+    row(context_lens[b] + d) = row(context_lens[b] + accepted[b, d]) for d < num_accepted[b], and kept_lens[b] = context_lens[b] + their number, the
+    next step's context.
+
+    All of it lies on the device: ``block_table`` int32 [>= B, blocks], ``context_lens`` and ``seq_lens`` int32 [B] as step_tables has them, ``accepted``
+    int32 [B,A] (numbers of a request's new tokens, each larger than the one before, as a path down a tree is), ``num_accepted`` and ``kept_lens``
+    int32 [B].  A path ends at its first entry that is not larger, that is no token of its request, or whose rows are not in the table or the
+    caches.  Idle places keep their negative length.  Requests must not share the pages that their new tokens lie in."""
+    what = "keep_rows"
+    native = _host.load().keep_rows
+    if native(caches, block_table, context_lens, seq_lens, accepted, num_accepted, kept_lens):     # (a list of tensors)
+        return
+    caches = [caches] if torch.is_tensor(caches) else list(caches)
+    if native(caches, block_table, context_lens, seq_lens, accepted, num_accepted, kept_lens):
+        return
+    if not caches:
+        raise ValueError(f"{what}: no caches")
+    dev = _one_device(what, *caches, block_table, context_lens, seq_lens, accepted, num_accepted, kept_lens)
+    words, pages, page = _page_caches(what, caches)
+    b = context_lens.numel()
+    for name, x in (("context_lens", context_lens), ("seq_lens", seq_lens), ("num_accepted", num_accepted), ("kept_lens", kept_lens)):
+        if x.dtype != torch.int32 or x.dim() != 1 or x.numel() != b or not x.is_contiguous():
+            raise ValueError(f"{what}: {name} must be contiguous int32 [{b}], got {x.dtype} {tuple(x.shape)}")
+    for name, x, most in (("block_table", block_table, 1), ("accepted", accepted, 0)):
+        if x.dtype != torch.int32 or x.dim() != 2 or x.shape[0] < b or x.shape[1] < most or x.stride(1) != 1 and x.shape[1] > 1:
+            raise ValueError(f"{what}: {name} must be int32 [>= {b}, n] with contiguous rows, got {x.dtype} {tuple(x.shape)}")
+    with torch.cuda.device(dev):
+        rc = _lib.load().mlahip_keep_rows(words, len(caches), pages, page, block_table.data_ptr(), block_table.stride(0), block_table.shape[1],
+                                          context_lens.data_ptr(), seq_lens.data_ptr(), b, accepted.data_ptr(), accepted.stride(0), accepted.shape[1],
+                                          num_accepted.data_ptr(), kept_lens.data_ptr(), _stream(caches[0]))
+    _lib.check(rc, "mlahip_keep_rows")
