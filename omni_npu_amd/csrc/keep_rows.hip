@@ -5,8 +5,12 @@
 //   before it, places of the request (c + accepted[d] < seq_lens[b]), and in pages that there are
 // A path goes down a tree whose tokens stand behind their parents, so accepted[d] >= d, and a row that is overwritten is no later one's source.
 //
-// What bounds it: few rows of each request, read and written once, behind two dependent reads (the path, its pages).  A lane takes a granule's column of
-// one request in one cache, in all its rows: reads in front of writes without a wait for anyone else.
+// What bounds it: few rows of each request, read and written once, behind two dependent reads (the path, its pages).  A wavefront looks a request's path up,
+// an entry to a lane, and moves 64 granules of its rows in one cache: as many rows at once as their granules leave lanes for.  A row is read in front of its
+// own write; rows that are read later lie behind all places that have been written by then.
+// us: 64 requests x 54 caches of 1024 and 128 bytes, 4 rows of 5 (8 MB read and written) 5.4; 256 requests x 64 caches x 4 rows of 2 KB (270 MB) 58, 4.6 TB/s.
+// By a lane that looked its request's path up for itself 8.1 and 117; a wavefront for four caches one after the other, the path looked up once, 5.4 and 68
+// (one takes up what another waits for); pieces of a row in neighbouring wavefronts 5.3 and 59.
 #include "mla_common.hpp"
 #include "../../include/mla_hip.h"
 #include <string.h>
@@ -24,59 +28,80 @@ struct Params {
   const int32_t* table; int64_t table_stride; int32_t cols, page_size, page_shift, num_pages;
   const int32_t *context, *lens, *accepted, *num; int64_t accepted_stride; int32_t most;
   int32_t* kept;                                             // or null
-  int32_t batch, lanes_shift;                                // log2 of the lanes that a request's row takes in a wavefront
+  int32_t batch;
 };
+typedef const __attribute__((address_space(4))) int32_t* ConstPtr;
 
-template <typename V>
+// kNt: past the caches.  Launches of 128 MB or more, every path counted as a whole one, go there: 270 MB moved 58 us, 62.5 through the caches; 77 MB at
+// most 21.7 and 20.0; 8 MB 6.6 and 5.4.
+template <typename V, bool kNt>
 __global__ __launch_bounds__(256) void keep_rows_kernel(const Params p) {
-  constexpr int kAtOnce = 8;
-  const int lane = threadIdx.x & ((1 << p.lanes_shift) - 1);
-  const int64_t b = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> p.lanes_shift;
+  struct Move { int32_t from_page, from_row, to_page, to_row; };
+  __shared__ Move list[4][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int b = blockIdx.x * 4 + wave;
   if (b >= p.batch) return;
-  const Cache c = p.caches[blockIdx.y];
-  const uint32_t at = (blockIdx.z << p.lanes_shift) + lane;  // the lane's granule of a row
-  const bool mine = at < c.row_bytes / sizeof(V), tells = p.kept && blockIdx.y == 0 && at == 0;
-  if (!mine && !tells) return;
-  const int ctx = p.context[b], len = p.lens[b];
-  int n = p.num[b];
-  n = ctx < 0 || n < 0 ? 0 : n < p.most ? n : p.most;
+  const int ctx = ((ConstPtr)p.context)[b], len = ((ConstPtr)p.lens)[b], num = ((ConstPtr)p.num)[b];
+  const int n = ctx < 0 || num < 0 ? 0 : num < p.most ? num : p.most;
+  Move* moves = list[wave];
   int last = -1, kept = 0;
-  GLOBAL char* column = (GLOBAL char*)c.base + (int64_t)at * sizeof(V);
-  struct Row { bool there; int64_t at; };
-  auto row = [&](int64_t place) {
-    const int64_t pi = p.page_shift >= 0 ? place >> p.page_shift : place / p.page_size;
-    if (place < 0 || pi >= p.cols) return Row{false, 0};
-    const int32_t page = p.table[b * p.table_stride + pi];
-    return Row{page >= 0 && page < p.num_pages, page * c.page_stride + (place - pi * p.page_size) * (int64_t)c.row_stride};
-  };
-  for (int d0 = 0; d0 < n; d0 += kAtOnce) {
-    int from[kAtOnce];
-#pragma unroll
-    for (int k = 0; k < kAtOnce; k++) from[k] = d0 + k < n ? p.accepted[b * p.accepted_stride + d0 + k] : -1;
-    Row src[kAtOnce], dst[kAtOnce];
-    V v[kAtOnce];
-#pragma unroll
-    for (int k = 0; k < kAtOnce; k++) {
-      const int64_t place = (int64_t)ctx + from[k];
-      src[k] = row(from[k] >= 0 && place < len ? place : -1);
-      dst[k] = row((int64_t)ctx + d0 + k);
+  for (int d0 = 0; d0 < p.most; d0 += 64) {                  // (the first entries asked for together with the numbers above)
+    const int d = d0 + lane;
+    const int from = d < p.most ? p.accepted[b * p.accepted_stride + d] : -1;
+    if (d0 >= n) break;
+    int before = __builtin_amdgcn_update_dpp(last, from, 0x138, 0xf, 0xf, false);   // (of the lane below; the first one's: the last of the 64 before)
+    struct Place { int32_t page, row; };
+    auto place = [&](int64_t x) {
+      if (x >= (int64_t)p.cols * p.page_size) return Place{-1, 0};
+      const uint32_t at = (uint32_t)x, pi = p.page_shift >= 0 ? at >> p.page_shift : at / (uint32_t)p.page_size;
+      return Place{p.table[b * p.table_stride + pi], (int32_t)(at - pi * (uint32_t)p.page_size)};
+    };
+    Place src{-1, 0}, dst{-1, 0};
+    const bool inside = d < n && from > before && (int64_t)ctx + from < len;
+    if (inside) {
+      src = place((int64_t)ctx + from);
+      dst = place((int64_t)ctx + d);
     }
-    bool good = true;
+    const bool good = inside && src.page >= 0 && src.page < p.num_pages && dst.page >= 0 && dst.page < p.num_pages;
+    const uint64_t bad = ~__builtin_amdgcn_ballot_w64(good);
+    const int run = bad ? __builtin_ctzll(bad) : 64;         // entries up to the first that ends the path
+    kept += run;
+    const bool moved = lane < run && from != d;
+    const uint64_t all = __builtin_amdgcn_ballot_w64(moved);
+    const int count = __builtin_popcountll(all);
+    if (moved) moves[__builtin_popcountll(all & ((1ull << lane) - 1))] = Move{src.page, src.row, dst.page, dst.row};
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const Cache c = p.caches[blockIdx.y];
+    const uint32_t granules = c.row_bytes / sizeof(V);
+    const int shift = granules > 32 ? 6 : granules > 1 ? 32 - __builtin_clz(granules - 1) : 0, rows = 64 >> shift;
+    const uint32_t at = (blockIdx.z << shift) + (lane & ((1 << shift) - 1));
+    GLOBAL char* column = (GLOBAL char*)c.base + (int64_t)at * sizeof(V);
+    auto spot = [&](int32_t page, int32_t row) { return (GLOBAL V*)(column + (page * c.page_stride + (int64_t)row * c.row_stride)); };
+    constexpr int kAtOnce = 4;
+    for (int m0 = at < granules ? lane >> shift : count; m0 < count; m0 += rows * kAtOnce) {
+      V v[kAtOnce];
 #pragma unroll
-    for (int k = 0; k < kAtOnce; k++) {
-      good = good && from[k] > last && src[k].there && dst[k].there;
-      last = from[k];
-      kept += good;
-      if (from[k] == d0 + k) src[k].there = false;           // (there already)
-      else src[k].there = good;
-      if (mine && src[k].there) v[k] = *(const GLOBAL V*)(column + src[k].at);
+      for (int k = 0; k < kAtOnce; k++) {
+        const int m = m0 + k * rows;
+        if (m >= count) continue;
+        const GLOBAL V* x = spot(moves[m].from_page, moves[m].from_row);
+        if constexpr (kNt) v[k] = __builtin_nontemporal_load(x);
+        else v[k] = *x;
+      }
+#pragma unroll
+      for (int k = 0; k < kAtOnce; k++) {
+        const int m = m0 + k * rows;
+        if (m >= count) continue;
+        GLOBAL V* x = spot(moves[m].to_page, moves[m].to_row);
+        if constexpr (kNt) __builtin_nontemporal_store(v[k], x);
+        else *x = v[k];
+      }
     }
-#pragma unroll
-    for (int k = 0; k < kAtOnce; k++)
-      if (mine && src[k].there) *(GLOBAL V*)(column + dst[k].at) = v[k];
-    if (!good) break;
+    if (run < 64) break;
+    last = __builtin_amdgcn_readlane(from, 63);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
-  if (tells) p.kept[b] = ctx < 0 ? ctx : ctx + kept;
+  if (p.kept && blockIdx.y == 0 && blockIdx.z == 0 && lane == 0) p.kept[b] = ctx < 0 ? ctx : ctx + kept;
 }
 
 }  // namespace keep
@@ -126,22 +151,21 @@ extern "C" int mlahip_keep_rows(const mlahip_page_cache* caches, int32_t num_cac
     int32_t next = 0;
     while (next < num_caches) {
       int32_t m = 0;
-      int64_t most = 1;
+      int64_t most = 1, total = 0;
       for (; next < num_caches && m < keep::kCaches; next++) {
         const mlahip_page_cache& c = caches[next];
         const uint64_t bits = (uint64_t)(uintptr_t)c.base | (uint64_t)c.page_stride_bytes | (uint64_t)c.row_stride_bytes | (uint64_t)c.row_bytes;
         if ((bits & 15 ? bits & 3 ? 1 : 4 : 16) != unit) continue;
         p.caches[m++] = keep::Cache{(char*)c.base, c.page_stride_bytes, (uint32_t)c.row_bytes, (uint32_t)c.row_stride_bytes};
         most = c.row_bytes / unit > most ? c.row_bytes / unit : most;
+        total += c.row_bytes;
       }
       if (m == 0) break;
-      p.lanes_shift = 0;
-      while (p.lanes_shift < 6 && (1 << p.lanes_shift) < most) p.lanes_shift++;
-      const int64_t groups = (((int64_t)batch << p.lanes_shift) + 255) / 256, pieces = (most + (1 << p.lanes_shift) - 1) >> p.lanes_shift;
-      const dim3 grid((unsigned)groups, (unsigned)m, (unsigned)pieces);
-      if (unit == 16) hipLaunchKernelGGL((keep::keep_rows_kernel<u32x4>), grid, dim3(256), 0, stream, p);
-      else if (unit == 4) hipLaunchKernelGGL((keep::keep_rows_kernel<uint32_t>), grid, dim3(256), 0, stream, p);
-      else hipLaunchKernelGGL((keep::keep_rows_kernel<uint8_t>), grid, dim3(256), 0, stream, p);
+      const dim3 grid((unsigned)((batch + 3) / 4), (unsigned)m, (unsigned)((most + 63) / 64));
+      if (unit == 16 && (double)total * batch * max_accepted >= 0x1p27) hipLaunchKernelGGL((keep::keep_rows_kernel<u32x4, true>), grid, dim3(256), 0, stream, p);
+      else if (unit == 16) hipLaunchKernelGGL((keep::keep_rows_kernel<u32x4, false>), grid, dim3(256), 0, stream, p);
+      else if (unit == 4) hipLaunchKernelGGL((keep::keep_rows_kernel<uint32_t, false>), grid, dim3(256), 0, stream, p);
+      else hipLaunchKernelGGL((keep::keep_rows_kernel<uint8_t, false>), grid, dim3(256), 0, stream, p);
       if (int e = check_launch(me)) return e;
       p.kept = nullptr;
     }
