@@ -422,7 +422,14 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
       const int t0 = only < 0 ? tok_first : only, t1 = only < 0 ? tok_last : only;
       // (a tree's: the context that every token sees, and the keys that there are)
       const int all_hi = sq.key_0 + (kTree ? 0 : t0), any_hi = kTree ? sq.len : sq.key_0 + t1;
-      const int all_lo = p.window > 0 ? (kTree ? any_hi : sq.key_0 + t1) - p.window : 0, any_lo = p.window > 0 ? all_hi - p.window : 0;
+      const int all_lo = p.window > 0 ? (kTree ? any_hi : sq.key_0 + t1) - p.window : 0;
+      int any_lo = p.window > 0 ? all_hi - p.window : 0;
+      if constexpr (kTree) {
+        if (p.window > 0 && t0 == t1) {                      // (one token's: where its own window begins)
+          const int left = window_left(visible_of(t0));
+          any_lo = sq.key_0 - (left > 0 ? left : 0);
+        }
+      }
       uint32_t odd = 0;
       const float scale_log2 = first->scale_log2 * (kFp8 && first->k_scale ? ((const GLOBAL float*)first->k_scale)[head] : 1.f);
 
@@ -868,6 +875,14 @@ __global__ __launch_bounds__(256) void gqa_join_kernel(const Params p) {
   if (p.lse && gi == 0) p.lse[t * (p.kv_heads * p.group) + qh] = sum == 0.f ? -INFINITY : (top + (fast_log2(sum) + kFar)) * kLn2;
 }
 
+template <bool kTree, typename T, int D>
+int launch_join(const char* me, const Params& p, hipStream_t st) {
+  // a wavefront for a row where the chunks leave a few partials to a request, four where they leave many
+  const int items = p.kv_heads * p.max_q_len * p.group;
+  if (p.num_chunks > 8 * p.batch) hipLaunchKernelGGL((gqa_join_kernel<kTree, T, D, 4>), dim3((unsigned)items, (unsigned)p.batch), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((gqa_join_kernel<kTree, T, D, 1>), dim3((unsigned)((items + 3) / 4), (unsigned)p.batch), dim3(256), 0, st, p);
+  return check_launch(me);
+}
 template <bool kTree, typename T, int D, bool kFp8, int MT>
 int launch(const char* me, const Params& p, int row_groups, unsigned x, hipStream_t st) {
   typedef Shape<T, D, kFp8, MT> Sh;
@@ -876,14 +891,7 @@ int launch(const char* me, const Params& p, int row_groups, unsigned x, hipStrea
   if (rc != MLA_OK) return rc;
   hipLaunchKernelGGL((gqa_split_kernel<kTree, T, D, kFp8, MT>), dim3(x, (unsigned)(p.head_groups * row_groups)), dim3(Sh::waves * 64), bytes, st, p);
   if (int e = check_launch(me)) return e;
-  if (p.num_chunks > 0) {
-    // a wavefront for a row where the chunks leave a few partials to a request, four where they leave many
-    const int items = p.kv_heads * p.max_q_len * p.group;
-    if (p.num_chunks > 8 * p.batch) hipLaunchKernelGGL((gqa_join_kernel<kTree, T, D, 4>), dim3((unsigned)items, (unsigned)p.batch), dim3(256), 0, st, p);
-    else hipLaunchKernelGGL((gqa_join_kernel<kTree, T, D, 1>), dim3((unsigned)((items + 3) / 4), (unsigned)p.batch), dim3(256), 0, st, p);
-    return check_launch(me);
-  }
-  return MLA_OK;
+  return p.num_chunks > 0 ? launch_join<kTree, T, D>(me, p, st) : MLA_OK;
 }
 // 64 rows to a wavefront are for heads of up to 128: wider ones' sums of as many rows do not fit its registers.
 template <bool kTree, typename T, int D, bool kFp8>
@@ -911,6 +919,9 @@ inline size_t workspace_need(int32_t batch, int32_t max_q_len, int32_t q_heads, 
   const int64_t n = slots(batch, num_chunks) * max_q_len * q_heads;
   return (size_t)(align256((int64_t)batch * 8) + align256(n * 4) + n * dim * 4);
 }
+
+// gqa_wide.hip: 128 rows to a workgroup.
+int launch_wide_rows(const char* me, const Params& p, int dtype, int dim, bool fp8, unsigned x, hipStream_t st);
 
 // The checks and the launches of both entry points.
 template <bool kTree>
@@ -963,8 +974,10 @@ int run(const char* me, const void* q, int64_t q_stride_t, int64_t q_stride_h, i
   p.visible = visible; p.visible_stride = visible_stride; p.words = words;
   p.scale_log2 = scale * kLog2e;
   p.out = (char*)out; p.o_st = out_stride_t * 2; p.o_sh = out_stride_h * 2; p.lse = lse_out;
-  MLA_REQUIRE(rows_per_group == 16 || rows_per_group == 32 || (rows_per_group == 64 && dim < 256), MLA_ERR_SHAPE,
-              "%s: %d rows to a workgroup (16, 32, or 64 of heads of up to 128)", me, rows_per_group);
+  const bool wide = kTree && rows_per_group == 128;
+  MLA_REQUIRE(rows_per_group == 16 || rows_per_group == 32 || ((rows_per_group == 64 || wide) && dim < 256), MLA_ERR_SHAPE,
+              "%s: %d rows to a workgroup (16, 32, or of heads of up to 128 %s)", me, rows_per_group, kTree ? "64 and 128" : "64");
+  MLA_REQUIRE(!wide || heads_per_group == 1, MLA_ERR_SHAPE, "%s: %d key heads to a workgroup of %d rows", me, heads_per_group, rows_per_group);
   const int rows = max_q_len * p.group, mt = rows_per_group / 16, waves = few_waves(rows_per_group, dim, es) ? 4 : 8;
   MLA_REQUIRE(heads_per_group >= 1 && heads_per_group <= waves && (heads_per_group & (heads_per_group - 1)) == 0 && kv_heads % heads_per_group == 0,
               MLA_ERR_SHAPE, "%s: %d of %d key heads to a workgroup of %d wavefronts (a power of two that divides both)", me, heads_per_group,
@@ -989,6 +1002,7 @@ int run(const char* me, const void* q, int64_t q_stride_t, int64_t q_stride_h, i
     p.part_lse = (float*)(ws + align256((int64_t)batch * 8));
     p.part_acc = (float*)((char*)p.part_lse + align256(n * 4));
   }
+  if (wide) return launch_wide_rows(me, p, dtype, dim, cache_dtype == 3, x, stream);
   return dtype == 0 ? pick<kTree, __bf16>(me, p, dim, cache_dtype == 3, mt, row_groups, x, stream)
                     : pick<kTree, _Float16>(me, p, dim, cache_dtype == 3, mt, row_groups, x, stream);
 }

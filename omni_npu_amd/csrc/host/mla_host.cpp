@@ -645,15 +645,16 @@ bool qk_norm_rope_cache(const Tensor& q, const OptTensor& k, const OptTensor& v,
             ko ? ko->data_ptr() : nullptr, ko ? ko->stride(0) : 0, ko ? ko->stride(1) : 0, stream_of(q)), "mlahip_qk_norm_rope_cache");
 }
 
-// kernels.gqa_plan
-std::tuple<int, int, int> gqa_plan(int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t element_bytes,
-                                   int64_t max_seq_len) {
+// kernels.gqa_plan: its estimate, and what it chose
+typedef std::tuple<double, int64_t, int64_t, int64_t> GqaBest;
+GqaBest gqa_best(int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t element_bytes,
+                 int64_t max_seq_len) {
   if (batch < 1 || q_len < 1 || kv_heads < 1 || dim < 1 || element_bytes < 1 || q_heads < kv_heads)
     throw std::invalid_argument("gqa_plan: " + std::to_string(batch) + " requests of " + std::to_string(q_len) + " tokens, " + std::to_string(q_heads) +
                                 " query and " + std::to_string(kv_heads) + " key heads of " + std::to_string(dim) + " values, " +
                                 std::to_string(element_bytes) + " bytes each");
   const int64_t rows = q_len * q_heads / kv_heads, key = 2 * dim * element_bytes, units = batch * div_up(max_seq_len, 32);
-  std::tuple<double, int64_t, int64_t, int64_t> best{INFINITY, 1, 1, 16};
+  GqaBest best{INFINITY, 1, 1, 16};
   for (int64_t tile = 16; tile <= 64; tile *= 2) {
     if ((tile > 16 && tile / 2 >= rows) || (tile == 64 && dim == 256)) break;
     const bool few = dim == 256 || tile == 64 || (tile == 32 && dim == 128 && element_bytes == 2);
@@ -678,7 +679,36 @@ std::tuple<int, int, int> gqa_plan(int64_t batch, int64_t q_len, int64_t q_heads
       best = std::min(best, {6.8 + more + parts + std::max(walk(std::min(size, batch * max_seq_len)), stream) + joins, chunks, heads, tile});
     }
   }
-  return {(int)std::get<1>(best), (int)std::get<2>(best), (int)std::get<3>(best)};
+  return best;
+}
+std::tuple<int, int, int> plan_of(const GqaBest& best) { return {(int)std::get<1>(best), (int)std::get<2>(best), (int)std::get<3>(best)}; }
+std::tuple<int, int, int> gqa_plan(int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t element_bytes,
+                                   int64_t max_seq_len) {
+  return plan_of(gqa_best(batch, q_len, q_heads, kv_heads, dim, element_bytes, max_seq_len));
+}
+// kernels.gqa_tree_plan
+std::tuple<int, int, int> gqa_tree_plan(int64_t batch, int64_t q_len, int64_t q_heads, int64_t kv_heads, int64_t dim, int64_t element_bytes,
+                                        int64_t max_seq_len) {
+  GqaBest best = gqa_best(batch, q_len, q_heads, kv_heads, dim, element_bytes, max_seq_len);
+  const int64_t rows = q_len * q_heads / kv_heads, tile = std::get<3>(best);
+  if (rows <= 32 || dim > 128) return plan_of(best);
+  std::get<0>(best) = std::max(std::get<0>(best), 9.3 + (double)(batch * max_seq_len * kv_heads * div_up(rows, tile) * tile * dim) / 1e9 *
+                                                            (tile == 64 ? 10.9 : 17.0) * (dim == 64 ? 1.3 : 1.0));
+  const double step = dim == 128 ? 1.2 : 0.9;
+  const int64_t groups = div_up(rows, 128) * kv_heads;
+  const auto alone = [](int64_t workgroups) { return workgroups <= 256 ? 0.8 : 1.0; };
+  if (max_seq_len <= 2048) {
+    const int64_t workgroups = batch * groups;
+    best = std::min(best, {7.4 + (double)div_up(workgroups, 512) * ((double)div_up(max_seq_len, 32) * step * alone(workgroups) + 2.3), 0, 1, 128});
+  }
+  for (int64_t workgroups : {256, 512, 1024}) {
+    const int64_t chunks = std::max<int64_t>(1, std::min(batch * div_up(max_seq_len, 64), workgroups / groups));
+    const int64_t size = div_up(batch * div_up(max_seq_len, 32), chunks);
+    const double parts = std::min(1.0 + (double)chunks / (double)batch, (double)chunks) * (double)(batch * q_len * q_heads * dim) / 1e6;
+    best = std::min(best, {13.3 + (double)div_up(chunks * groups, 512) * ((double)size * step * alone(chunks * groups) +
+                                                                         2.3 * std::max(1.0, (double)batch / (double)chunks)) + 2.1 * parts, chunks, 1, 128});
+  }
+  return plan_of(best);
 }
 
 // kernels.gqa_decode and, with bits, kernels.gqa_tree_decode
@@ -690,7 +720,7 @@ bool gqa(const Tensor* bits, const Tensor& q, const Tensor& k_cache, const Tenso
   const int64_t window = std::min<int64_t>(window_keys.value_or(0), 0x7fffffff);
   auto off = [](OptInt x, int64_t lo, int64_t hi) { return x && (*x < lo || *x > hi); };
   if (q_len > (1 << 24) || off(window_keys, 1, INT64_MAX) || off(num_chunks, 0, 1 << 16) || off(max_seq_len, 1, INT64_MAX) || off(heads_per_group, 1, 8) ||
-      off(rows_per_group, 1, 64))
+      off(rows_per_group, 1, bits ? 128 : 64))
     return false;
   const at::Device dev = q.device();
   const at::ScalarType dt = q.scalar_type();
@@ -710,7 +740,7 @@ bool gqa(const Tensor* bits, const Tensor& q, const Tensor& k_cache, const Tenso
   int64_t longest = block_table.size(1) * k_cache.size(1);
   if (max_seq_len && c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) longest = std::min(longest, *max_seq_len);
   if (window > 0) longest = std::min(longest, window + q_len + (bits ? 31 : 30));
-  const auto [by_rule, heads, rows] = gqa_plan(b, q_len, hq, hk, d, k_cache.element_size(), longest);
+  const auto [by_rule, heads, rows] = (bits ? gqa_tree_plan : gqa_plan)(b, q_len, hq, hk, d, k_cache.element_size(), longest);
   const int chunks = (int)num_chunks.value_or(by_rule);
   Stream st = stream_of(q);
   const char* what = bits ? "mlahip_gqa_tree_decode" : "mlahip_gqa_decode";
@@ -880,6 +910,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   // (what this file has a copy of, for a test to hold against kernels.py)
   m.def("launch_splits", &launch_splits, py::arg("batch"), py::arg("q_len"), py::arg("heads"), py::arg("max_seq_len"), py::arg("full") = false);
   m.def("gqa_plan", &gqa_plan);
+  m.def("gqa_tree_plan", &gqa_tree_plan);
   m.def("prefill_long_rows", &prefill_long_rows);
   m.def("prefill_blocks", &prefill_blocks);
   m.def("prefill_pieces", &prefill_pieces);

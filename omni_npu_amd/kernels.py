@@ -1500,6 +1500,11 @@ def gqa_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, dim: int, elem
     own has more than 32 pieces only of two steps or more, as they are joined one after the other: 4/1 heads of 128, 5000 keys, 157 / 79
     pieces 11.3 / 9.9.  Beyond 2048 keys a request to a workgroup loses up to two thirds where lengths are ragged, which the host does not
     know."""
+    return _gqa_best(batch, q_len, q_heads, kv_heads, dim, element_bytes, max_seq_len)[1:]
+
+
+def _gqa_best(batch, q_len, q_heads, kv_heads, dim, element_bytes, max_seq_len):
+    """gqa_plan's estimate, and what it chose."""
     if min(batch, q_len, kv_heads, dim, element_bytes) < 1 or q_heads < kv_heads:
         raise ValueError(f"gqa_plan: {batch} requests of {q_len} tokens, {q_heads} query and {kv_heads} key heads of {dim} values, {element_bytes} bytes each")
     rows = q_len * q_heads // kv_heads
@@ -1530,6 +1535,37 @@ def gqa_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, dim: int, elem
             joins = 3.5 * max(1.0, batch / chunks) * -(-chunks * groups // 256)
             best = min(best, (6.8 + more + parts + max(walk(min(size, batch * max_seq_len)), stream) + joins, chunks, heads, tile))
             heads *= 2
+    return best
+
+
+def gqa_tree_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, dim: int, element_bytes: int, max_seq_len: int):
+    """gqa_plan for gqa_tree_decode, whose workgroups have 128 rows that share a head's keys as well: the faster by an estimate in us.
+
+    Of 14 000 measured launches (1-64 requests of 64-32 000 keys, 1-8 key heads of 64 or 128 values, 24-2000 rows) its choice is 1.7 % slower than the
+    best one on average, 15 % in one of twenty; gqa_plan's is 9 % and 59 %.  gqa_plan's own estimate is of the cache's reads; many rows are
+    bound by products: 9.3 and, for 1e9 times (row, key, value of a head), 10.9 with 64 rows to a workgroup, 17 with fewer, a third more for
+    heads of 64.  128 rows: a workgroup's step of 32 keys takes 1.2, heads of 64 0.9, four fifths of that where it has a CU to itself (256
+    workgroups and fewer; 512 run at once), 2.3 for each piece of a sequence; 7.4 for one launch, 13.3 for two, 2.1 for a million values of
+    partial results.  us, 64 / 128 rows: 26 requests of 14 500 keys, 126 rows, 8 key heads of 128, 417 / 261; 3 of 7500, 544 rows, 2 key heads,
+    52 / 49; one of 4096, 240 rows, 8 key heads, 27 / 31; 24-32 rows are a quarter slower with 128."""
+    estimate, chunks, heads, tile = _gqa_best(batch, q_len, q_heads, kv_heads, dim, element_bytes, max_seq_len)
+    rows = q_len * q_heads // kv_heads
+    if rows <= 32 or dim > 128:
+        return chunks, heads, tile
+    estimate = max(estimate, 9.3 + batch * max_seq_len * kv_heads * -(-rows // tile) * tile * dim / 1e9 * (10.9 if tile == 64 else 17.0) * (1.3 if dim == 64 else 1.0))
+    best = (estimate, chunks, heads, tile)
+    step = 1.2 if dim == 128 else 0.9
+    groups = -(-rows // 128) * kv_heads
+    alone = lambda workgroups: 0.8 if workgroups <= 256 else 1.0
+    if max_seq_len <= 2048:
+        workgroups = batch * groups
+        best = min(best, (7.4 + -(-workgroups // 512) * (-(-max_seq_len // 32) * step * alone(workgroups) + 2.3), 0, 1, 128))
+    for workgroups in (256, 512, 1024):
+        chunks = max(1, min(batch * -(-max_seq_len // 64), workgroups // groups))
+        size = -(-batch * -(-max_seq_len // 32) // chunks)
+        parts = min(1.0 + chunks / batch, float(chunks)) * (batch * q_len * q_heads * dim) / 1e6
+        best = min(best, (13.3 + -(-chunks * groups // 512) * (size * step * alone(chunks * groups) + 2.3 * max(1.0, batch / chunks)) + 2.1 * parts,
+                          chunks, 1, 128))
     return best[1:]
 
 
@@ -1600,7 +1636,7 @@ def _gqa(what, q, k_cache, v_cache, block_table, seq_lens, visible, scale, out, 
         raise ValueError(f"{what}: a window of {window} keys")
     if not 1 <= q_len <= 1 << 24:
         raise ValueError(f"{what}: q_len {q_len}")
-    for name, x, most in (("num_chunks", num_chunks, 1 << 24), ("heads_per_group", heads_per_group, 8), ("rows_per_group", rows_per_group, 64)):
+    for name, x, most in (("num_chunks", num_chunks, 1 << 24), ("heads_per_group", heads_per_group, 8), ("rows_per_group", rows_per_group, 128 if tree else 64)):
         if x is not None and not 0 <= x <= most:
             raise ValueError(f"{what}: {name} {x}")
     if max_seq_len is not None and max_seq_len < 1:
@@ -1634,7 +1670,7 @@ def _gqa(what, q, k_cache, v_cache, block_table, seq_lens, visible, scale, out, 
             longest = min(longest, max_seq_len)
         if window is not None:
             longest = min(longest, window + q_len + 30 + tree)
-        chunks, heads, rows = gqa_plan(b, q_len, hq, hk, d, k_cache.element_size(), longest)
+        chunks, heads, rows = (gqa_tree_plan if tree else gqa_plan)(b, q_len, hq, hk, d, k_cache.element_size(), longest)
         num_chunks = chunks if num_chunks is None else num_chunks
         need = lib.mlahip_gqa_decode_workspace_bytes(b, q_len, hq, d, num_chunks)
         launch = lambda ws: entry(

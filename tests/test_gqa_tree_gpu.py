@@ -72,12 +72,12 @@ def test_types_and_head_layouts(dev, d, dtype, fp8, q_len, hq, hk):
     check(c, *call(dev, c, q_len))
 
 
-@pytest.mark.parametrize("rows", [16, 32, 64])
+@pytest.mark.parametrize("rows", [16, 32, 64, 128])
 @pytest.mark.parametrize("q_len,hq,hk", [(1, 8, 2), (17, 2, 2), (40, 12, 3), (64, 16, 2)])
 @pytest.mark.parametrize("chunks", [0, 5])
 def test_rows_of_a_workgroup(dev, rows, q_len, hq, hk, chunks):
     c = tree(make(dev, [q_len, 300, 64 + q_len - 1, q_len + 1], q_len=q_len, hq=hq, hk=hk, page=48, seed=q_len), seed=rows)
-    check(c, *call(dev, c, q_len, num_chunks=chunks, rows_per_group=rows))
+    check(c, *call(dev, c, q_len, num_chunks=chunks, rows_per_group=rows, heads_per_group=1))
 
 
 @pytest.mark.parametrize("q_len,words", [(64, 2), (65, 2), (100, 2), (129, 3), (300, 5), (512, 8)])

@@ -34,10 +34,36 @@ def test_tree_decode_codes():
     assert rc(_26=96) == -3 and rc(_27=1) == -3
     assert rc(_13=24) == -2 and rc(_25=3) == -2 and rc(_32=-1) == -2
     assert rc(_37=None) == -4 and rc(_38=100) == -4
-    assert rc(_40=3) == -2 and rc(_41=48) == -2
+    assert rc(_40=3) == -2 and rc(_41=48) == -2 and rc(_41=256) == -2
+    assert rc(_41=128) == -2                                   # two key heads to a workgroup of 128 rows
+    assert rc(_41=128, _40=1, _26=256) == -2                   # heads of 256
     assert rc(_22=0) == 0 and rc(_3=0) == 0                    # nothing to do
     assert "gqa_tree_decode" in (rc(_41=48), lib.mlahip_last_error_string().decode())[1]
     del raw
+
+
+def test_tree_plan():
+    """Both sides choose alike, what the entry point takes; gqa_decode's choices stay its own."""
+    from omni_npu_amd import _host
+    host, seen = _host.load(), set()
+    for batch in (1, 3, 32, 500):
+        for q_len in (1, 5, 26, 60, 512):
+            for hq, hk in ((8, 8), (32, 8), (64, 4), (6, 3), (1, 1)):
+                for d in (64, 128, 256):
+                    for es in (1, 2):
+                        for longest in (1, 64, 1280, 2049, 16384, 1 << 30):
+                            chunks, heads, rows = K.gqa_tree_plan(batch, q_len, hq, hk, d, es, longest)
+                            assert (chunks, heads, rows) == tuple(host.gqa_tree_plan(batch, q_len, hq, hk, d, es, longest))
+                            seen.add(rows)
+                            assert 0 <= chunks <= 1 << 16 and hk % heads == 0
+                            if rows == 128:
+                                assert heads == 1 and d < 256 and q_len * hq // hk > 32
+                            else:
+                                assert (chunks, heads, rows) == K.gqa_plan(batch, q_len, hq, hk, d, es, longest)
+    assert seen == {16, 32, 64, 128}
+    for plan in (K.gqa_tree_plan, host.gqa_tree_plan):
+        with pytest.raises(ValueError, match="gqa_plan"):
+            plan(0, 1, 8, 2, 128, 2, 100)
 
 
 def test_step_tables_codes():
