@@ -9,6 +9,12 @@
 //
 // A list's order hangs on all requests in front of one: sums over the requests, by one workgroup, which changes the list, the tables and the counts.  The
 // tokens of larger steps follow in a launch of their own, when these stand.
+//
+// A few KB: what takes time is what waits for something else.  A launch of this takes 3.3 us when it does nothing for tokens, of which one is the first
+// loads' way; so all of a request's numbers are asked for at once, one scan adds up what is given back and what is needed (the others only where a
+// list is too short), what tokens look up lies in LDS, parents too (a tree ten deep is ten loads behind each other), and a token's page is under way
+// meanwhile.  us: one token 4.1, 67 requests of 26 tokens as trees 6.2, 500 of up to 64 8.4 (pages 3.3, tokens 5), 16 000 tokens of prompts 6.3; loads
+// where they are used: 4.5, 9.0, 9.3, 6.9.
 #include "mla_common.hpp"
 #include "../../include/mla_hip.h"
 
@@ -26,6 +32,7 @@ struct Params {
   int32_t *held, *free_pages, *num_free; int32_t capacity;   // or null
 };
 
+typedef const __attribute__((address_space(1))) int32_t* Ints;
 constexpr int kThreads = 1024, kSamples = 4096;
 
 // Tokens of request b, however its entries lie: at least none.
@@ -50,201 +57,261 @@ __device__ __forceinline__ int held_of(const Params& p, int b) {
   return h < 0 ? 0 : h < p.cols ? h : p.cols;
 }
 
-// The tokens t of a workgroup's threads; samples: every ``apart``th entry of qsl.
-__device__ __forceinline__ void token(const Params& p, int64_t t, const int32_t* samples, int apart) {
+// What a workgroup's tokens look up, in LDS: the beginnings of the requests, every ``apart``th of them where they are many, contexts and lengths of up to
+// kFew requests, and the parents of its tokens and of up to kBack in front of them (a tree's, whose bits there are words for).
+constexpr int kFew = kThreads, kBack = 512;
+template <int kTokens> struct Known {
+  int32_t begin[kSamples], ctx[kFew], len[kFew], up[kTokens + kBack];
+};
+__device__ __forceinline__ int apart_of(const Params& p) { return p.batch / kSamples + 1; }
+template <int kTokens> __device__ __forceinline__ void know(const Params& p, Known<kTokens>& known, int64_t first, bool lengths, int threads) {
+  if (p.qsl) {
+    const int apart = apart_of(p);
+    for (int i = threadIdx.x; i * apart <= p.batch; i += threads) known.begin[i] = p.qsl[i * apart];
+  }
+  if (lengths && p.batch <= kFew) {
+    for (int i = threadIdx.x; i < p.batch; i += threads) {
+      known.ctx[i] = p.context[i];
+      if (p.held) known.len[i] = p.seq_lens[i];
+    }
+  }
+  if (p.parents) {
+    const int64_t from = first > kBack ? first - kBack : 0, most = p.num_tokens - from;
+    for (int i = threadIdx.x; i < kTokens + kBack && i < most; i += threads) known.up[i] = p.parents[from + i];
+  }
+}
+
+// Token t, of a workgroup's kTokens from ``first`` on.
+template <int kTokens> __device__ __forceinline__ void token(const Params& p, const Known<kTokens>& known, int64_t first, int64_t t) {
   int b = 0;
   int64_t begin = 0, n = 0;
   if (p.batch > 0) {
     if (p.qsl) {                                             // the last request that begins at or in front of t
+      const int apart = apart_of(p);
       int lo = 0, hi = (p.batch - 1) / apart;
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (samples[mid] <= t) lo = mid;
+        if (known.begin[mid] <= t) lo = mid;
         else hi = mid - 1;
       }
-      lo *= apart;
-      hi = lo + apart - 1 < p.batch - 1 ? lo + apart - 1 : p.batch - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (p.qsl[mid] <= t) lo = mid;
-        else hi = mid - 1;
+      if (apart == 1) {
+        begin = known.begin[lo];
+        n = known.begin[lo + 1] - begin;
+      } else {
+        lo *= apart;
+        hi = lo + apart - 1 < p.batch - 1 ? lo + apart - 1 : p.batch - 1;
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (p.qsl[mid] <= t) lo = mid;
+          else hi = mid - 1;
+        }
+        begin = p.qsl[lo];
+        n = p.qsl[lo + 1] - begin;
       }
       b = lo;
-      begin = p.qsl[b];
-      n = tokens_of(p, b);
     } else {
-      const int64_t at = t / p.q_len;
-      b = at < p.batch ? (int)at : p.batch - 1;
+      const uint32_t at = (uint32_t)t / (uint32_t)p.q_len;   // (there are fewer than 2^31 tokens)
+      b = at < (uint32_t)p.batch ? (int)at : p.batch - 1;
       begin = (int64_t)b * p.q_len;
       n = p.q_len;
     }
   }
   const int64_t i = t - begin;
-  int64_t position = 0, slot = -1;
-  const bool there = n > 0 && i >= 0 && i < n && begin >= 0 && p.context[b] >= 0;
+  int32_t ctx = -1;
+  if (n > 0 && i >= 0 && i < n && begin >= 0) ctx = p.batch <= kFew ? known.ctx[b] : ((Ints)p.context)[b];
+  // (its page is under way while the parents are followed)
+  int32_t page = -1;
+  uint32_t row = 0;
+  if (ctx >= 0) {                                            // (idle places and rows behind the last request: none)
+    const uint32_t place = (uint32_t)ctx + (uint32_t)i, col = page_of(p, place);
+    const int64_t len = ctx + n;
+    const bool fits = !p.held || (p.batch <= kFew ? known.len[b] : ((Ints)p.seq_lens)[b]) == (len < 0x7fffffff ? len : 0x7fffffff);
+    if (col < (uint32_t)p.cols && fits) page = p.table[b * p.table_stride + col];
+    row = place - col * (uint32_t)p.page_size;
+  }
   int64_t depth = i;
   if (p.parents) {
-    uint64_t* row = p.visible + t * p.visible_stride;
-    if (there) {
-      // up the parents, whose numbers fall: words from the last one on
-      const int32_t* up = p.parents + begin;
-      int64_t at = i;
-      uint64_t bits = 0;
-      int w = p.words - 1;
-      depth = -1;
-      while (true) {
-        if (at >> 6 < p.words) {
-          for (; w > (int)(at >> 6); w--) {
-            row[w] = bits;
-            bits = 0;
+    uint64_t* out = p.visible + t * p.visible_stride;
+    const int64_t from = first > kBack ? first - kBack : 0;
+    uint64_t bits = 0;
+    int w = p.words - 1;
+    if (ctx >= 0) {
+      // up the parents, whose numbers fall
+      int32_t at = (int32_t)i;
+      if (p.words == 1 && n <= 64 && begin >= from) {
+        const int32_t* up = known.up + (begin - from);
+        depth = -1;
+        int32_t next = at;
+        do {
+          at = next;
+          bits |= 1ull << at;
+          depth++;
+          next = up[at];
+        } while (next >= 0 && next < at);
+      } else {                                               // words from the last one on
+        const int32_t apart = (int32_t)(begin - from);
+        depth = -1;
+        while (true) {
+          if (at >> 6 < p.words) {
+            for (; w > at >> 6; w--) {
+              out[w] = bits;
+              bits = 0;
+            }
+            bits |= 1ull << (at & 63);
           }
-          bits |= 1ull << (at & 63);
+          depth++;
+          const int32_t next = apart + at >= 0 ? known.up[apart + at] : ((Ints)p.parents)[begin + at];
+          if (next < 0 || next >= at) break;
+          at = next;
         }
-        depth++;
-        const int64_t next = up[at];
-        if (next < 0 || next >= at) break;
-        at = next;
       }
-      for (; w >= 0; w--) {
-        row[w] = bits;
-        bits = 0;
-      }
-    } else {
-      for (int w = 0; w < p.words; w++) row[w] = 0;
+    }
+    for (; w >= 0; w--) {
+      out[w] = bits;
+      bits = 0;
     }
   }
-  if (there) {
-    const Length x = length_of(p, b);
-    position = x.ctx + depth;
-    const uint32_t place = (uint32_t)x.ctx + (uint32_t)i, col = page_of(p, place);
-    if (col < (uint32_t)p.cols && (!p.held || p.seq_lens[b] == x.len)) {
-      const int32_t page = p.table[b * p.table_stride + col];
-      if (page >= 0) slot = (int64_t)page * p.page_size + (place - col * (uint32_t)p.page_size);
-    }
-  }
-  p.positions[t] = position;
-  p.slots[t] = slot;
+  p.positions[t] = ctx >= 0 ? ctx + depth : 0;
+  p.slots[t] = page >= 0 ? (int64_t)page * p.page_size + row : -1;
 }
 
-__device__ __forceinline__ int apart_of(const Params& p) { return p.batch > kSamples ? (p.batch + kSamples - 1) / kSamples : 1; }
-__device__ __forceinline__ void take_samples(const Params& p, int32_t* samples, int threads) {
-  if (!p.qsl) return;
-  const int apart = apart_of(p);
-  for (int i = threadIdx.x; i * apart < p.batch; i += threads) samples[i] = p.qsl[i * apart];
-}
-
-// Inclusive sums over a workgroup's threads, and the whole one.
-struct Sum { int upto, all; };
-__device__ __forceinline__ Sum scan(int v, int* parts) {
+// Sums over a workgroup's threads of two values, up to each thread's and whole.
+struct Sums { int a, b, all_a, all_b; };
+__device__ __forceinline__ Sums scan(int a, int b, int2* parts) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int mine = wave_incl_scan_dpp(v);
-  if (lane == 63) parts[wave] = mine;
+  a = wave_incl_scan_dpp(a);
+  b = wave_incl_scan_dpp(b);
+  if (lane == 63) parts[wave] = int2{a, b};
   __syncthreads();
-  int before = 0, all = 0;
+  int all_a = 0, all_b = 0;
 #pragma unroll
   for (int w = 0; w < kThreads / 64; w++) {
-    before += w < wave ? parts[w] : 0;
-    all += parts[w];
+    const int2 x = parts[w];
+    a += w < wave ? x.x : 0;
+    b += w < wave ? x.y : 0;
+    all_a += x.x;
+    all_b += x.y;
   }
   __syncthreads();
-  return {before + mine, all};
+  return {a, b, all_a, all_b};
 }
 
-// Pages: every request's, by one workgroup.
-__device__ void pages(const Params& p, int* parts, int* upto) {
+// Pages: every request's, by one workgroup, kThreads of them at a time; a thread's own stays in registers where that is all there are.
+struct Room { int2 parts[kThreads / 64]; int upto[kThreads], end[kThreads]; };
+__device__ void pages(const Params& p, Room& room, int32_t* ctx, int32_t* len) {
   const int tid = threadIdx.x;
   const int there = *p.num_free;
+  struct { Length x; int t, h, give, need; } m;
+  Sums s;                                                    // of pages given back and needed
+  auto look = [&](int base) {
+    m = {{0, 0}, 0, 0, 0, 0};
+    if (base + tid < p.batch) {
+      m.x = length_of(p, base + tid);
+      m.t = pages_of(p, m.x.len);
+      m.h = held_of(p, base + tid);
+      m.give = m.h > m.t ? m.h - m.t : 0;                    // (t < h: it fits the table)
+      m.need = m.t > m.h && m.t <= p.cols ? m.t - m.h : 0;
+    }
+    s = scan(m.give, m.need, room.parts);
+  };
+  auto each = [&](auto f) {
+    for (int base = 0; base < p.batch; base += kThreads) {
+      if (p.batch > kThreads) look(base);
+      f(base);
+    }
+  };
+  if (p.batch <= kThreads) look(0);
   int free = there < 0 ? 0 : there < p.capacity ? there : p.capacity;
   // pages that go back: how many in all, then each to its place
-  int back = 0;
-  auto gives = [&](int b) {
-    if (b >= p.batch) return 0;
-    const int t = pages_of(p, length_of(p, b).len), h = held_of(p, b);
-    return h > t ? h - t : 0;                                // (t < h: it fits the table)
-  };
-  int before = 0;
-  for (int base = 0; base < p.batch; base += kThreads) {
-    const int n = gives(base + tid);
-    const Sum s = scan(n, parts);
-    back += scan(before + s.upto + free <= p.capacity ? n : 0, parts).all;
-    before += s.all;
-  }
-  if (before > 0) {
+  int back = 0, before = 0;
+  each([&](int) { back += s.all_a; });
+  if (free + back > p.capacity) {
+    back = 0;
+    each([&](int) {
+      back += scan(before + s.a + free <= p.capacity ? m.give : 0, 0, room.parts).all_a;
+      before += s.all_a;
+    });
     before = 0;
-    for (int base = 0; base < p.batch; base += kThreads) {
-      const int b = base + tid, n = gives(b);
-      const Sum s = scan(n, parts);
-      if (n > 0 && before + s.upto + free <= p.capacity) {
-        const int t = held_of(p, b) - n, first = free + back - 1 - (before + s.upto - n);
-        for (int k = 0; k < n; k++) p.free_pages[first - k] = p.table[b * p.table_stride + t + k];
-        p.held[b] = t;
+  }
+  if (back > 0) {
+    each([&](int base) {
+      if (m.give > 0 && before + s.a + free <= p.capacity) {
+        const int32_t* row = p.table + (base + tid) * p.table_stride + m.t;
+        const int first = free + back - 1 - (before + s.a - m.give);
+        for (int k = 0; k < m.give; k++) p.free_pages[first - k] = row[k];
+        p.held[base + tid] = m.t;
       }
-      before += s.all;
-    }
+      before += s.all_a;
+    });
     free += back;
     __syncthreads();
   }
   // pages that are taken
   int taken = 0;
   before = 0;
-  for (int base = 0; base < p.batch; base += kThreads) {
-    const int b = base + tid;
-    int need = 0, t = 0, h = 0;
-    Length x{0, 0};
-    if (b < p.batch) {
-      x = length_of(p, b);
-      t = pages_of(p, x.len);
-      h = held_of(p, b);
-      need = t > h && t <= p.cols ? t - h : 0;
-    }
-    const Sum s = scan(need, parts);
-    const bool got = need == 0 || before + s.upto <= free;
-    if (b < p.batch) {
-      p.seq_lens[b] = t <= p.cols && got ? x.len : x.ctx;
-      if (need > 0 && got) p.held[b] = t;
-    }
-    taken += scan(need > 0 && got ? need : 0, parts).all;
-    if (s.all > 0) {
-      // a page to a thread: the request that it is for by its sum
-      upto[tid] = s.upto;
-      __syncthreads();
-      const int rows = p.batch - base < kThreads ? p.batch - base : kThreads;
-      for (int k = tid; k < s.all; k += kThreads) {
-        int lo = 0, hi = rows - 1;
-        while (lo < hi) {                                    // the first whose sum is above k
-          const int mid = (lo + hi) >> 1;
-          if (upto[mid] > k) hi = mid;
-          else lo = mid + 1;
-        }
-        if (before + upto[lo] > free) continue;
-        const int first = lo > 0 ? upto[lo - 1] : 0, n = upto[lo] - first;
-        const Length y = length_of(p, base + lo);
-        p.table[(base + lo) * p.table_stride + pages_of(p, y.len) - n + (k - first)] = p.free_pages[free - 1 - before - k];
+  each([&](int base) {
+    const bool got = m.need == 0 || before + s.b <= free;
+    if (base + tid < p.batch) {
+      const int32_t now = m.t <= p.cols && got ? m.x.len : m.x.ctx;
+      p.seq_lens[base + tid] = now;
+      if (p.batch <= kFew) {
+        ctx[tid] = m.x.ctx;
+        len[tid] = now;
       }
+      if (m.need > 0 && got) p.held[base + tid] = m.t;
+    }
+    if (s.all_b > 0) {
+      // A page or a few to a request: by its thread.  More: a page to a thread, which finds the request by its sum.
+      constexpr int kOwn = 2;
+      room.upto[tid] = s.b;
+      room.end[tid] = m.t;
+      const int all = s.all_b;
+      if (__syncthreads_or(m.need > kOwn)) {
+        const int rows = p.batch - base < kThreads ? p.batch - base : kThreads;
+        for (int k = tid; k < all; k += kThreads) {
+          int lo = 0, hi = rows - 1;
+          while (lo < hi) {                                  // the first whose sum is above k
+            const int mid = (lo + hi) >> 1;
+            if (room.upto[mid] > k) hi = mid;
+            else lo = mid + 1;
+          }
+          if (before + room.upto[lo] <= free)
+            p.table[(base + lo) * p.table_stride + room.end[lo] - (room.upto[lo] - k)] = p.free_pages[free - 1 - before - k];
+        }
+      } else if (got) {
+#pragma unroll
+        for (int k = 0; k < kOwn; k++)
+          if (k < m.need) p.table[(base + tid) * p.table_stride + m.h + k] = p.free_pages[free - 1 - before - (s.b - m.need) - k];
+      }
+      taken += before + all <= free ? all : scan(got ? m.need : 0, 0, room.parts).all_a;
+      before += all;
       __syncthreads();
     }
-    before += s.all;
-  }
+  });
   if (tid == 0) *p.num_free = free - taken;
 }
 
+// Tokens that the workgroup of the pages does as well.  us, together / in a launch of their own: 1500 tokens in trees 6.0 / 6.8, 2000 6.7 / 7.0, 3000
+// 7.9 / 7.0; 2000 tokens of four requests 5.0 / 7.0, 4000 6.1 / 7.0; of as many requests 3000 11.2 / 10.3.
+constexpr int kTogether = 2048, kBlock = 256;
+
 __global__ __launch_bounds__(kThreads) void step_pages_kernel(const Params p, int with_tokens) {
-  __shared__ int parts[kThreads / 64], upto[kThreads];
-  __shared__ int32_t samples[kSamples];
-  if (with_tokens) take_samples(p, samples, kThreads);
-  pages(p, parts, upto);
+  __shared__ Room room;
+  __shared__ Known<kTogether> known;
+  if (with_tokens) know(p, known, 0, false, kThreads);
+  pages(p, room, known.ctx, known.len);
   if (!with_tokens) return;
   __syncthreads();
-  for (int64_t t = threadIdx.x; t < p.num_tokens; t += kThreads) token(p, t, samples, apart_of(p));
+  for (int64_t t = threadIdx.x; t < p.num_tokens; t += kThreads) token(p, known, 0, t);
 }
 
-__global__ __launch_bounds__(256) void step_tokens_kernel(const Params p) {
-  __shared__ int32_t samples[kSamples];
-  take_samples(p, samples, 256);
+__global__ __launch_bounds__(kBlock) void step_tokens_kernel(const Params p) {
+  __shared__ Known<kBlock> known;
+  const int64_t first = (int64_t)blockIdx.x * kBlock, t = first + threadIdx.x;
+  know(p, known, first, true, kBlock);
   __syncthreads();
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (!p.held && t < p.batch) p.seq_lens[t] = length_of(p, (int)t).len;
-  if (t < p.num_tokens) token(p, t, samples, apart_of(p));
+  if (t < p.num_tokens) token(p, known, first, t);
 }
 
 struct Range { const char *begin, *end; };
@@ -298,13 +365,13 @@ extern "C" int mlahip_step_tables(const int32_t* context_lens, const int32_t* qu
   p.seq_lens = seq_lens; p.positions = positions; p.slots = slot_mapping; p.num_tokens = num_tokens;
   p.parents = num_tokens > 0 ? parents : nullptr; p.visible = visible; p.visible_stride = visible_stride; p.words = words;
   p.held = pages ? num_blocks : nullptr; p.free_pages = free_pages; p.num_free = num_free; p.capacity = capacity;
-  const bool together = num_tokens <= 2048;
+  const bool together = num_tokens <= tables::kTogether;
   if (pages) {
     hipLaunchKernelGGL(tables::step_pages_kernel, dim3(1), dim3(tables::kThreads), 0, stream, p, (int)together);
     if (int e = check_launch(me)) return e;
     if (together) return MLA_OK;
   }
   const int64_t n = num_tokens > batch ? num_tokens : batch;
-  hipLaunchKernelGGL(tables::step_tokens_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL(tables::step_tokens_kernel, dim3((unsigned)((n + tables::kBlock - 1) / tables::kBlock)), dim3(tables::kBlock), 0, stream, p);
   return check_launch(me);
 }
