@@ -20,6 +20,11 @@
 //               neighbouring dims, even and odd ones into products of their own
 //   join        wavefronts of a head through LDS, then chunks of a sequence through the workspace, by a second launch
 //
+// A wait counts loads in their order, so the keys of a tile may be waited for only where it is known what was asked for behind them on every way there:
+// each wavefront asks for a first tile, the last tile is a step of its own, and the rare load of page numbers is waited for in its branch.  With
+// loads that some ways had and others not, a step waited for its values with its keys: 64 requests x 2000-6000 keys x 8 tokens x 32/8 heads 199 us
+// against 193, 4096-8192 keys and trees of 8 tokens 289 against 280; 16 x 3 tokens x 48/3 26.4 against 24.8.
+//
 // Measured, split and join together: 64 requests x 4096-8192 keys x 32/8 heads of 128 (1630 MB) 251 us, 6.5 TB/s; one of 131 072 x 64/8 90 us,
 // 5.9; 128 x 2 tokens x 2048-16 384 keys x 64/8 over the 8-bit cache (2440 MB) 397 us, 6.1; 33 requests x the newest 1024 keys x 16/4 heads of
 // 256, pages of 16 (137 MB) 34 us, 4.0: four wavefronts to a CU (a wavefront's sums, keys and values take 300 registers, a second workgroup would
@@ -140,8 +145,8 @@ __device__ __forceinline__ int chunk_units(int tot, int n) {
 }
 
 // A page as a buffer, and 16 bytes out of it that are read once: at the lane's offset and a scalar one.  (Host: no page takes 2^31 bytes.)
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_at(const char* base, int page, int64_t stride) {
-  return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)page * stride), 0, 0x7fffffff, 0x00027000);
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_at(const char* base, int page, int64_t stride, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(base + (int64_t)page * stride), 0, bytes, 0x00027000);
 }
 __device__ __forceinline__ u32x4 load_nt(__amdgpu_buffer_rsrc_t from, int lane_offset, int offset) {
   return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(from, lane_offset, offset, 2));
@@ -180,26 +185,29 @@ __device__ __forceinline__ ParamsPtr reload() {
 // What a tree's tokens see of tiles that hold keys of the request's own tokens, kept in LDS as a word of 32 keys for each tile and token.
 constexpr int kMostWords = 8, kTreeTiles = 2 * kMostWords + 1;
 __device__ __forceinline__ uint32_t bits_to(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
-// How many of a token's first n bits are set (n: at most 64 * words).
-__device__ __forceinline__ int bits_below(const GLOBAL uint64_t* row, int n) {
+// How many of a token's first n bits are set (n: at most 64 * words); word: its words, by their number.
+template <typename F> __device__ __forceinline__ int bits_below(F word, int n) {
   int sum = 0;
   for (int w = 0; w * 64 < n; w++) {
-    const uint64_t x = row[w];
+    const uint64_t x = word(w);
     sum += __builtin_popcountll(n - w * 64 < 64 ? x & ((1ull << (n - w * 64)) - 1) : x);
   }
   return sum;
 }
+__device__ __forceinline__ int bits_below(const GLOBAL uint64_t* row, int n) {
+  return bits_below([&](int w) { return row[w]; }, n);
+}
 // The 32 keys from key0 on (key0 + 32 > ctx): the context's, below ctx, and those of the token's bits that are keys of the request's, below len; of
 // the bits the lowest ``drop`` ones are in front of the window.
-__device__ __forceinline__ uint32_t tree_word(const GLOBAL uint64_t* row, int words, int key0, int ctx, int len, int drop) {
+template <typename F> __device__ __forceinline__ uint32_t tree_word(F word, int words, int key0, int ctx, int len, int drop) {
   const int j = key0 > ctx ? key0 - ctx : 0, w = j >> 6, r = j & 63;
   uint32_t x = 0;
   if (w < words) {
-    uint64_t y = row[w] >> r;
-    if (r > 32 && w + 1 < words) y |= row[w + 1] << (64 - r);
+    uint64_t y = word(w) >> r;
+    if (r > 32 && w + 1 < words) y |= word(w + 1) << (64 - r);
     x = (uint32_t)y;
     if (drop > 0)
-      for (int n = drop - bits_below(row, j); n > 0 && x; n--) x &= x - 1;
+      for (int n = drop - bits_below(word, j); n > 0 && x; n--) x &= x - 1;
   }
   if (ctx > key0) x = x << (ctx - key0) | bits_to(ctx - key0);
   return x & bits_to(len - key0);
@@ -322,7 +330,10 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
       struct Place { int page, row; };
       auto place_of = [&](int key) {                         // (sixteen keys from a multiple of sixteen on: one page)
         const int pi = page_of(key);
-        if ((uint32_t)(pi - have0) > 63u) pages_from(b, pi);   // (in front of them where a piece is begun again)
+        if ((uint32_t)(pi - have0) > 63u) {                  // (in front of them where a piece is begun again)
+          pages_from(b, pi);
+          asm volatile("" : "+v"(have));                     // (waited for here: behind the branch it would be with every tile, and so all loads)
+        }
         const int pg = __builtin_amdgcn_readlane(have, pi - have0);
         return Place{pg < 0 ? 0 : pg < p.num_pages ? pg : p.num_pages - 1, key - pi * p.page_size};
       };
@@ -333,13 +344,16 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
       const int k_off = l16 * p.k_sr + g * 16, v_off = lk * p.v_sr + lp * 16;
       u32x4 kr[2][Sh::gran], vr[Sh::v_loads];
       Place at[2];
+      // (Loads that some wavefronts make and some do not would be waited for with all that follow them: one without tiles makes them too, of the first
+      // tile's place, in a buffer of no bytes.)
+      const int kw_from = mine > 0 ? kw : 0, readable = mine > 0 ? 0x7fffffff : 0;
       auto ask_keys = [&](int i) {
-        const int key = key0 + (kw + i * kws) * kTile;
+        const int key = key0 + (kw_from + i * kws) * kTile;
 #pragma unroll
         for (int s = 0; s < 2; s++) {
           // (a page of a multiple of 32 holds both sixteens)
           at[s] = s == 1 && (p.page_size & 16) == 0 ? Place{at[0].page, at[0].row + 16} : place_of(key + s * 16);
-          const __amdgpu_buffer_rsrc_t from = page_at(k_head, at[s].page, p.k_sp);
+          const __amdgpu_buffer_rsrc_t from = page_at(k_head, at[s].page, p.k_sp, readable);
 #pragma unroll
           for (int c = 0; c < Sh::gran; c++) kr[s][c] = load_nt(from, k_off + c * 64, at[s].row * p.k_sr);
         }
@@ -347,13 +361,12 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
       auto ask_values = [&]() {
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-          const __amdgpu_buffer_rsrc_t from = page_at(v_head, at[s].page, p.v_sp);
+          const __amdgpu_buffer_rsrc_t from = page_at(v_head, at[s].page, p.v_sp, readable);
 #pragma unroll
           for (int n = 0; n < Sh::v_loads / 2; n++)
             vr[s * (Sh::v_loads / 2) + n] = load_nt(from, v_off, (at[s].row + n * Sh::keys_per_load) * p.v_sr);
         }
       };
-      if (mine > 0 && (p.num_chunks == 0 ? p.window > 0 : p.batch > 1)) pages_from(b, page_of(key0 + kw * kTile));
 
       // the rows' tokens
       int tok_first = 0, tok_last = 0;
@@ -363,62 +376,84 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
       }
       uint32_t* tree_words = (uint32_t*)(stats + Sh::stat_floats);   // [token][tile]
       const int tree_tile0 = sq.key_0 & ~(kTile - 1);        // first key of the first tile that is not the context's alone
+      const int tree_row = 2 * p.words + 2;                  // its tiles, and how many keys of a window are left to the context
       auto visible_of = [&](int token) {
         const ParamsPtr at = reload();
         const int64_t t = (int64_t)sq.q0 + token;
         return (const GLOBAL uint64_t*)at->visible + (t >= 0 && t < at->num_tokens ? t : 0) * at->visible_stride;
       };
       // how many keys of a window are left to the context, below 0: how many bits are in front of the window
-      auto window_left = [&](const GLOBAL uint64_t* row) {
-        const int own = sq.len - sq.key_0;
-        return p.window - bits_below(row, own < 64 * p.words ? own : 64 * p.words);
-      };
-      if constexpr (kTree) {
-        if (key1 > sq.key_0) {                               // (the same for all of the workgroup)
-          for (int it = threadIdx.x; it < (tok_last - tok_first + 1) * kTreeTiles; it += Sh::waves * 64) {
-            const int k = it / kTreeTiles, n = it - k * kTreeTiles;
-            const GLOBAL uint64_t* row = visible_of(tok_first + k);
-            tree_words[it] = tree_word(row, p.words, tree_tile0 + n * kTile, sq.key_0, sq.len, p.window > 0 ? -window_left(row) : 0);
-          }
-          lds_barrier();
-        }
-      }
+      const int own = sq.len - sq.key_0;
+      auto window_left = [&](const GLOBAL uint64_t* row) { return p.window - bits_below(row, own < 64 * p.words ? own : 64 * p.words); };
       auto tile_bits = [&](int token, int tile_key) {        // without the window's begin
         const int n = (tile_key - tree_tile0) / kTile;       // (both multiples)
-        return tile_key < tree_tile0 ? 0xffffffffu : n < kTreeTiles ? tree_words[(token - tok_first) * kTreeTiles + n] : 0u;
+        return tile_key < tree_tile0 ? 0xffffffffu : n < tree_row - 1 ? tree_words[(token - tok_first) * tree_row + n] : 0u;
       };
 
       // ---- the query: row l16 of each row tile, eight dims a step; zeros in rows that do not exist ----
       u32x4 qf[MT][D / 32];
       int hi[MT], lo[MT], tok[MT];
+      auto load_queries = [&] {
 #pragma unroll
-      for (int m = 0; m < MT; m++) {
-        const int r = row0 + m * 16 + l16;
-        const bool there = r < rows;
-        const int rr = there ? r : 0;
-        tok[m] = p.max_q_len == 1 ? 0 : (int)((uint32_t)rr / (uint32_t)p.group);
-        const int64_t t = (int64_t)sq.q0 + tok[m];
-        const bool ok = there && t >= 0 && t < first->num_tokens;
-        const GLOBAL char* src = (const GLOBAL char*)first->q + (ok ? t : 0) * first->q_st + (int64_t)(head * p.group + (rr - tok[m] * p.group)) * first->q_sh;
+        for (int m = 0; m < MT; m++) {
+          const int r = row0 + m * 16 + l16;
+          const bool there = r < rows;
+          const int rr = there ? r : kTree ? row0 : 0;
+          tok[m] = p.max_q_len == 1 ? 0 : (int)((uint32_t)rr / (uint32_t)p.group);
+          const int64_t t = (int64_t)sq.q0 + tok[m];
+          const bool ok = there && t >= 0 && t < first->num_tokens;
+          const GLOBAL char* src = (const GLOBAL char*)first->q + (ok ? t : 0) * first->q_st + (int64_t)(head * p.group + (rr - tok[m] * p.group)) * first->q_sh;
 #pragma unroll
-        for (int s = 0; s < D / 32; s++) {
-          // (an 8-bit key's granule of 16 dims is two steps' operands)
-          const int dim = kFp8 ? (s >> 1) * 64 + g * 16 + (s & 1) * 8 : s * 32 + g * 8;
-          qf[m][s] = ok ? *(const GLOBAL u32x4*)(src + dim * 2) : u32x4{0u, 0u, 0u, 0u};
-        }
-        if constexpr (kTree) {
-          lo[m] = 0;
-          if (p.window > 0) {
-            const int left = window_left(visible_of(tok[m]));
-            lo[m] = sq.key_0 - (left > 0 ? left : 0);
+          for (int s = 0; s < D / 32; s++) {
+            // (an 8-bit key's granule of 16 dims is two steps' operands)
+            const int dim = kFp8 ? (s >> 1) * 64 + g * 16 + (s & 1) * 8 : s * 32 + g * 8;
+            qf[m][s] = ok ? *(const GLOBAL u32x4*)(src + dim * 2) : u32x4{0u, 0u, 0u, 0u};
           }
-        } else {
+        }
+      };
+      // A tree's bits are asked for with the table and the queries, in front of the first keys and values, and looked at while these are under way: a
+      // load that is waited for behind them waits for them as well.  One word: a thread's of all tiles that it is in.
+      uint64_t word = 0;
+      const int word_of = (int)threadIdx.x >> 2;
+      if (kTree && p.words == 1) word = *visible_of(tok_first + word_of <= tok_last ? tok_first + word_of : tok_last);
+      load_queries();
+      if (p.num_chunks == 0 ? p.window > 0 : p.batch > 1) pages_from(b, page_of(key0 + kw_from * kTile));
+      if constexpr (!kTree) {
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
           hi[m] = sq.key_0 + tok[m];
           lo[m] = p.window > 0 ? hi[m] - p.window : 0;
         }
       }
       int only = -1;                                         // the token that a pass is for, where the piece is done token by token
       while (true) {
+      if constexpr (kTree) asm volatile("" : "+v"(word), "+v"(have));   // (waited for here)
+      __builtin_amdgcn_sched_barrier(0);
+      ask_keys(0);
+      ask_values();
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (kTree) {
+        const int items = (tok_last - tok_first + 1) * tree_row;
+        if (only < 0 && p.words == 1) {
+          const int n = (int)threadIdx.x & 3, over = p.window > 0 ? bits_below([&](int) { return word; }, own < 64 ? own : 64) - p.window : 0;
+          const uint32_t bits = tree_word([&](int) { return word; }, 1, tree_tile0 + n * kTile, sq.key_0, sq.len, over);
+          if ((int)threadIdx.x < items) tree_words[threadIdx.x] = n == 3 ? (uint32_t)-over : bits;
+        } else if (only < 0) {
+          for (int it = threadIdx.x; it < items; it += Sh::waves * 64) {
+            const int k = it / tree_row, n = it - k * tree_row;
+            const GLOBAL uint64_t* row = visible_of(tok_first + k);
+            const int left = p.window > 0 ? window_left(row) : 0;
+            const uint32_t bits = tree_word([&](int w) { return row[w]; }, p.words, tree_tile0 + n * kTile, sq.key_0, sq.len, -left);
+            tree_words[it] = n == tree_row - 1 ? (uint32_t)left : bits;
+          }
+        }
+        lds_barrier();
+#pragma unroll
+        for (int m = 0; m < MT; m++) {
+          const int left = p.window > 0 ? (int)tree_words[(tok[m] - tok_first + 1) * tree_row - 1] : 0;
+          lo[m] = p.window > 0 ? sq.key_0 - (left > 0 ? left : 0) : 0;
+        }
+      }
       const int t0 = only < 0 ? tok_first : only, t1 = only < 0 ? tok_last : only;
       // (a tree's: the context that every token sees, and the keys that there are)
       const int all_hi = sq.key_0 + (kTree ? 0 : t0), any_hi = kTree ? sq.len : sq.key_0 + t1;
@@ -426,7 +461,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
       int any_lo = p.window > 0 ? all_hi - p.window : 0;
       if constexpr (kTree) {
         if (p.window > 0 && t0 == t1) {                      // (one token's: where its own window begins)
-          const int left = window_left(visible_of(t0));
+          const int left = (int)tree_words[(t0 - tok_first + 1) * tree_row - 1];
           any_lo = sq.key_0 - (left > 0 ? left : 0);
         }
       }
@@ -442,12 +477,8 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
 #pragma unroll
         for (int d = 0; d < D / 16; d++) acc[m][d] = f32x4{0.f, 0.f, 0.f, 0.f};
       }
-      if (mine > 0) {
-        ask_keys(0);
-        ask_values();
-      }
-
-      for (int i = 0; i < mine; i++) {
+      // (the last tile by itself: where the next one's loads may be missing the compiler waits for them with those that it means)
+      auto step = [&](int i, auto kMore) __attribute__((always_inline)) {
         const int tile_key = key0 + (kw + i * kws) * kTile;
         const bool partial = tile_key + kTile > all_hi || tile_key < all_lo;
         // ---- S^T ----
@@ -476,7 +507,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
         }
         // (the barriers for the scheduler keep the next tile's loads behind the last use of the registers they go to)
         __builtin_amdgcn_sched_barrier(0);
-        if (i + 1 < mine) ask_keys(i + 1);
+        if constexpr (kMore()) ask_keys(i + 1);
         __builtin_amdgcn_sched_barrier(0);
         // ---- probabilities against the rows' references ----
         u32x4 pf[MT], pl[MT];
@@ -573,7 +604,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
           *(u32x4*)(mine_lds + row * Sh::row_b + ((lp ^ Sh::swz(row & 15)) << 4)) = vr[n];
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (i + 1 < mine) ask_values();
+        if constexpr (kMore()) ask_values();
         __builtin_amdgcn_sched_barrier(0);
         // ---- O^T += V^T P^T ----
         const int v_row = 4 * g + (l16 >> 2), sw = Sh::swz(v_row);
@@ -610,7 +641,9 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
 #pragma unroll
             for (int m = 0; m < MT; m++) acc[m][d * Sh::ops + o] = Ty::mm(a[o], pl[m], acc[m][d * Sh::ops + o]);
         }
-      }
+      };
+      for (int i = 0; i + 1 < mine; i++) step(i, std::true_type{});
+      if (mine > 0) step(mine - 1, std::false_type{});
 
       // ---- join of the wavefronts of a head ----
       const bool several = only < 0 && tok_first != tok_last, again = several && __builtin_amdgcn_ballot_w64(odd != 0) != 0;
@@ -886,7 +919,7 @@ int launch_join(const char* me, const Params& p, hipStream_t st) {
 template <bool kTree, typename T, int D, bool kFp8, int MT>
 int launch(const char* me, const Params& p, int row_groups, unsigned x, hipStream_t st) {
   typedef Shape<T, D, kFp8, MT> Sh;
-  constexpr int bytes = Sh::lds_b + (kTree ? 16 * MT * kTreeTiles * 4 : 0);
+  constexpr int bytes = Sh::lds_b + (kTree ? 16 * MT * (kTreeTiles + 1) * 4 : 0);
   const int rc = ensure_dynamic_lds((const void*)gqa_split_kernel<kTree, T, D, kFp8, MT>, bytes, me);
   if (rc != MLA_OK) return rc;
   hipLaunchKernelGGL((gqa_split_kernel<kTree, T, D, kFp8, MT>), dim3(x, (unsigned)(p.head_groups * row_groups)), dim3(Sh::waves * 64), bytes, st, p);

@@ -227,7 +227,7 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), 2) void gqa_tree_wide_ker
         for (int it = threadIdx.x; it < (tok_last - tok_first + 1) * kTreeTiles; it += W::threads) {
           const int k = it / kTreeTiles, n = it - k * kTreeTiles;
           const GLOBAL uint64_t* row = visible_of(tok_first + k);
-          tree_words[it] = tree_word(row, p.words, tree_tile0 + n * 32, sq.key_0, sq.len, p.window > 0 ? -window_left(row) : 0);
+          tree_words[it] = tree_word([&](int w) { return row[w]; }, p.words, tree_tile0 + n * 32, sq.key_0, sq.len, p.window > 0 ? -window_left(row) : 0);
         }
       }
       if (threadIdx.x == 0) flags[0] = 0;
