@@ -601,7 +601,7 @@ int mlahip_gqa_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, int
 
 /* The same for tokens drafted as a tree: a request's newest s keys are its own tokens', and token i sees the context, j < seq_lens[b] - s, and of
  * these keys the k-th where bit k % 64 of visible[t * visible_stride + k / 64] is set, k < 64 * words (1 to 8 words; bits past the request's own
- * tokens are not looked at; rows_per_group may be 128 as well, of heads of up to 128, with one key head to a workgroup); with window > 0 only the newest ``window`` of all these keys.  A token's own key is one of its bits.  A request has as many
+ * tokens are not looked at; rows_per_group may be 128 as well, with one key head to a workgroup); with window > 0 only the newest ``window`` of all these keys.  A token's own key is one of its bits.  A request has as many
  * tokens as are in the batch for it: max_q_len, or what query_start_loc says.  All else as above, the workspace's size too. */
 int mlahip_gqa_tree_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t num_tokens, const void* k_cache,
                            int64_t kc_page_stride, int64_t kc_row_stride, int64_t kc_head_stride, const void* v_cache,

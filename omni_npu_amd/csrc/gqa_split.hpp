@@ -1008,8 +1008,8 @@ int run(const char* me, const void* q, int64_t q_stride_t, int64_t q_stride_h, i
   p.scale_log2 = scale * kLog2e;
   p.out = (char*)out; p.o_st = out_stride_t * 2; p.o_sh = out_stride_h * 2; p.lse = lse_out;
   const bool wide = kTree && rows_per_group == 128;
-  MLA_REQUIRE(rows_per_group == 16 || rows_per_group == 32 || ((rows_per_group == 64 || wide) && dim < 256), MLA_ERR_SHAPE,
-              "%s: %d rows to a workgroup (16, 32, or of heads of up to 128 %s)", me, rows_per_group, kTree ? "64 and 128" : "64");
+  MLA_REQUIRE(rows_per_group == 16 || rows_per_group == 32 || (rows_per_group == 64 && dim < 256) || wide, MLA_ERR_SHAPE,
+              "%s: %d rows to a workgroup (16, 32, 64 of heads of up to 128%s)", me, rows_per_group, kTree ? ", 128" : "");
   MLA_REQUIRE(!wide || heads_per_group == 1, MLA_ERR_SHAPE, "%s: %d key heads to a workgroup of %d rows", me, heads_per_group, rows_per_group);
   const int rows = max_q_len * p.group, mt = rows_per_group / 16, waves = few_waves(rows_per_group, dim, es) ? 4 : 8;
   MLA_REQUIRE(heads_per_group >= 1 && heads_per_group <= waves && (heads_per_group & (heads_per_group - 1)) == 0 && kv_heads % heads_per_group == 0,

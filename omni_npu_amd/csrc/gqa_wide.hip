@@ -3,7 +3,8 @@
 // The formulas, the plan's partial results and their join are gqa_split.hpp's.  There 64 rows are a wavefront's, which walks keys of its own: each group of
 // rows reads all keys again, a workgroup's wavefronts are joined at its end, and a SIMD has one wavefront, which does its products and its exponentials in
 // turn.  Here
-//   workgroup    one key head, 32 rows to each of four wavefronts, two workgroups to a CU; no joins inside it, as each wavefront has all keys for its rows
+//   workgroup    one key head, 32 rows to each of four wavefronts, two workgroups to a CU (one with heads of 256, whose sums alone are 128 registers of a
+//                lane and whose tiles 128 KB); no joins inside it, as each wavefront has all keys for its rows
 //   tile         32 keys and values in LDS, 16 bits whatever the cache holds (16-bit ones are copied there directly, three tiles ahead, 8-bit ones are
 //                converted once, two ahead), four buffers of each, one barrier to a tile
 //   products     S^T = K Q^T and O^T = V^T P^T of 32x32x16: a lane's 16 scores are of one row, and their probabilities lie as the second product wants them
@@ -12,8 +13,8 @@
 // The order inside a turn is written down (sched_barrier): left to the compiler, products and exponentials lie in blocks of their own.
 //
 // Both operands of the probabilities make 3 products where a rounded one takes 2.  us, rows of a workgroup 64 / here, 8 key heads of 128 where nothing else
-// is said: 8 requests of 480 rows, 2000-16 000 keys 363 / 265; 16 of 256, 1000-4000 keys 128 / 98; 8 of 256, 4 heads of 64, 109 / 73; but one of
-// 240, 4096 keys 27.2 / 30.9, and 32 of 32, 303 / 342.  That is 880 TFLOP/s of matrix products, with the card at 1370 of its 1400 W (zeros for data,
+// is said: 8 requests of 480 rows, 2000-16 000 keys 363 / 265; 16 of 256, 1000-4000 keys 128 / 98; 8 of 256, 4 heads of 64, 109 / 73;
+// 4 heads of 256, 8 requests of 480 rows, 2000-16 000 keys (32 rows there) 719 / 303; but one of 240, 4096 keys 27.2 / 30.9, and 32 of 32, 303 / 342.  That is 880 TFLOP/s of matrix products, with the card at 1370 of its 1400 W (zeros for data,
 // same instructions: 17 % less time).  Eight wavefronts and 256 rows to a workgroup: 2 % faster at the largest of these, 12 % slower on average; products
 // of 16x16x32, sums by dot products or by a column of ones, values one tile behind, other orders in a turn: all within 3 % or slower.
 #include <utility>
@@ -65,12 +66,13 @@ template <typename T> __device__ __forceinline__ uint32_t times(uint32_t x, floa
   return __builtin_bit_cast(uint32_t, typename Types<T>::v2{(T)((float)v[0] * f), (T)((float)v[1] * f)});
 }
 template <int n> __device__ __forceinline__ void wait_loads() {
-  static_assert(n <= 4, "the loads of a set");
+  static_assert(n <= 4 || n == 8, "the loads of a set");
   if constexpr (n == 0) MLA_WAIT_VMCNT(0);
   else if constexpr (n == 1) MLA_WAIT_VMCNT(1);
   else if constexpr (n == 2) MLA_WAIT_VMCNT(2);
   else if constexpr (n == 3) MLA_WAIT_VMCNT(3);
-  else MLA_WAIT_VMCNT(4);
+  else if constexpr (n == 4) MLA_WAIT_VMCNT(4);
+  else MLA_WAIT_VMCNT(8);
 }
 template <int n> using Int = std::integral_constant<int, n>;
 template <typename F, int... i> __device__ __forceinline__ void each_of(F f, std::integer_sequence<int, i...>) { (f(Int<i>{}), ...); }
@@ -78,7 +80,7 @@ template <int n, typename F> __device__ __forceinline__ void each(F f) { each_of
 constexpr int kNowhere = 0x7effffc0;                         // a key that no request has (they have at most 2^30, and 2^24 tokens in front of the first)
 
 template <typename T, int D, bool kFp8>
-__global__ __launch_bounds__((Wide<D, kFp8>::threads), 2) void gqa_tree_wide_kernel(const Params p, const int row_groups) {
+__global__ __launch_bounds__((Wide<D, kFp8>::threads), (D > 128 ? 1 : 2)) void gqa_tree_wide_kernel(const Params p, const int row_groups) {
   typedef Wide<D, kFp8> W;
   typedef Types<T> Ty;
   typedef Wider<T> Wd;
@@ -123,6 +125,7 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), 2) void gqa_tree_wide_ker
   // (16 bits: copies into LDS, where a lane's place is its number's: it fetches the granule that belongs there)
   const int k_swz = W::k_swz(wave * W::keys_per_load + lk), v_swz = W::v_swz(wave * W::keys_per_load + lk);
   const int k_off = lk * p.k_sr + (kFp8 ? lp : lp ^ k_swz) * 16, v_off = lk * p.v_sr + (kFp8 ? lp : lp ^ v_swz) * 16;
+  const int k_off8 = lk * p.k_sr + (lp ^ k_swz ^ 8) * 16;     // (of keys eight further, where a load is that far from the one before)
   do {
     if (b >= p.batch) break;
     const Seq sq = seq_at<true>(p, b);
@@ -197,7 +200,7 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), 2) void gqa_tree_wide_ker
 #pragma unroll
           for (int j = 0; j < W::loads; j++) {
             if constexpr (kFp8) in_k[j] = load(k_head + k_at[j], k_off);
-            else dma16_sv_m0add(k_head + k_at[j], k_off, k_to, j * kApart * W::row_b);
+            else dma16_sv_m0add(k_head + k_at[j], kApart % 16 * j % 16 ? k_off8 : k_off, k_to, j * kApart * W::row_b);
           }
         }
         if (i >= W::lag) {
@@ -380,7 +383,7 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), 2) void gqa_tree_wide_ker
         // D / 16 operands of values, each with the probabilities' first and second ones, h and l:
         //   D / 64 times  S h S h S l S l, with three quarters of the probabilities, then  D / 64 times  h h l l, with the others and the new scores' maximum
         auto turn = [&] {
-          constexpr int kBlocks = D / 64, kSlots = 12 * kBlocks, kA = 8 * kBlocks;
+          constexpr int kBlocks = D / 64, kSlots = 12 * kBlocks, kA = 8 * kBlocks, kParts = kBlocks > 1 ? 2 : 1;
           const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
           f32x16 sc;
           u32x4 k[3], v[4], pn[2], ln[2];
@@ -425,7 +428,9 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), 2) void gqa_tree_wide_ker
             // reads: an operand of scores four slots in front of its product, of values as their places get free
             if constexpr (i < kA && i % 2 == 0 && i / 2 + 2 < D / 16) k[(i / 2 + 2) % 3] = read_k(i / 2 + 2);
             each<D / 16 - 2>([&](auto n2) {
-              constexpr int n = n2() + 2, at = n < 4 ? 2 * n - 1 : n < 6 ? 2 * n + 1 : 2 * n + 2;   // (D 64: 3, 5; D 128: 3, 5, 9, 11, 14, 16)
+              // (operand n - 4, whose place it takes, is behind its products, of which the second phase's come four slots apart and not eight)
+              constexpr int n = n2() + 2, late = n - 2 * kBlocks;
+              constexpr int at = late < 0 ? n / 2 * 8 + n % 2 * 2 - 5 : late < 2 ? kA - 7 + 2 * late : late < 4 ? kA - 6 + 2 * late : kA + late / 2 * 4 - 5 + late % 2;
               if constexpr (at == i) v[n % 4] = read_v(n);
             });
             __builtin_amdgcn_sched_barrier(0);
@@ -438,9 +443,11 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), 2) void gqa_tree_wide_ker
             }
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (i < kA) {
-              pairs(Int<i % 8>{}, Int<8>{}, Int<i / 8 * 6 / kBlocks>{}, Int<6 / kBlocks>{});
+              constexpr int kOf = kA / kParts;
+              pairs(Int<i % kOf>{}, Int<kOf>{}, Int<i / kOf * (6 / kParts)>{}, Int<6 / kParts>{});
             } else {
-              pairs(Int<i % 4>{}, Int<4>{}, Int<6 + (i - kA) / 4>{}, Int<2 / kBlocks>{});
+              constexpr int kEach = 4 * kBlocks / kParts;
+              pairs(Int<(i - kA) % kEach>{}, Int<kEach>{}, Int<6 + (i - kA) / kEach * (2 / kParts)>{}, Int<2 / kParts>{});
               constexpr int f = i - kA - 1, kOf = 4 * kBlocks - 1;
               if constexpr (f >= 0) {
 #pragma unroll
@@ -557,6 +564,7 @@ int launch_wide(const char* me, const Params& p, unsigned x, hipStream_t st) {
 template <typename T>
 int pick_wide(const char* me, const Params& p, int dim, bool fp8, unsigned x, hipStream_t st) {
   if (dim == 64) return fp8 ? launch_wide<T, 64, true>(me, p, x, st) : launch_wide<T, 64, false>(me, p, x, st);
+  if (dim == 256) return fp8 ? launch_wide<T, 256, true>(me, p, x, st) : launch_wide<T, 256, false>(me, p, x, st);
   return fp8 ? launch_wide<T, 128, true>(me, p, x, st) : launch_wide<T, 128, false>(me, p, x, st);
 }
 int launch_wide_rows(const char* me, const Params& p, int dtype, int dim, bool fp8, unsigned x, hipStream_t st) {

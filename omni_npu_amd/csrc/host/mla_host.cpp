@@ -691,22 +691,23 @@ std::tuple<int, int, int> gqa_tree_plan(int64_t batch, int64_t q_len, int64_t q_
                                         int64_t max_seq_len) {
   GqaBest best = gqa_best(batch, q_len, q_heads, kv_heads, dim, element_bytes, max_seq_len);
   const int64_t rows = q_len * q_heads / kv_heads, tile = std::get<3>(best);
-  if (rows <= 32 || dim > 128) return plan_of(best);
-  std::get<0>(best) = std::max(std::get<0>(best), 9.3 + (double)(batch * max_seq_len * kv_heads * div_up(rows, tile) * tile * dim) / 1e9 *
-                                                            (tile == 64 ? 10.9 : 17.0) * (dim == 64 ? 1.3 : 1.0));
-  const double step = dim == 128 ? 1.2 : 0.9;
-  const int64_t groups = div_up(rows, 128) * kv_heads;
-  const auto alone = [](int64_t workgroups) { return workgroups <= 256 ? 0.8 : 1.0; };
+  if (rows <= 32) return plan_of(best);
+  const bool wide = dim > 128;
+  const double start = wide ? 12.7 : 9.3, rate = wide ? 10.0 : (tile == 64 ? 10.9 : 17.0) * (dim == 64 ? 1.3 : 1.0);
+  std::get<0>(best) = std::max(std::get<0>(best), start + (double)(batch * max_seq_len * kv_heads * div_up(rows, tile) * tile * dim) / 1e9 * rate);
+  const double step = wide ? 1.7 : dim == 128 ? 1.2 : 0.9, piece = wide ? 5.3 : 2.3, one = wide ? 10.2 : 7.4, two = wide ? 16.7 : 13.3, part = wide ? 1.7 : 2.1;
+  const int64_t groups = div_up(rows, 128) * kv_heads, slots = wide ? 256 : 512;
+  const auto alone = [&](int64_t workgroups) { return workgroups <= 256 && !wide ? 0.8 : 1.0; };
   if (max_seq_len <= 2048) {
     const int64_t workgroups = batch * groups;
-    best = std::min(best, {7.4 + (double)div_up(workgroups, 512) * ((double)div_up(max_seq_len, 32) * step * alone(workgroups) + 2.3), 0, 1, 128});
+    best = std::min(best, {one + (double)div_up(workgroups, slots) * ((double)div_up(max_seq_len, 32) * step * alone(workgroups) + piece), 0, 1, 128});
   }
-  for (int64_t workgroups : {256, 512, 1024}) {
+  for (int64_t workgroups : {slots / 2, slots, 2 * slots}) {
     const int64_t chunks = std::max<int64_t>(1, std::min(batch * div_up(max_seq_len, 64), workgroups / groups));
     const int64_t size = div_up(batch * div_up(max_seq_len, 32), chunks);
     const double parts = std::min(1.0 + (double)chunks / (double)batch, (double)chunks) * (double)(batch * q_len * q_heads * dim) / 1e6;
-    best = std::min(best, {13.3 + (double)div_up(chunks * groups, 512) * ((double)size * step * alone(chunks * groups) +
-                                                                         2.3 * std::max(1.0, (double)batch / (double)chunks)) + 2.1 * parts, chunks, 1, 128});
+    best = std::min(best, {two + (double)div_up(chunks * groups, slots) * ((double)size * step * alone(chunks * groups) +
+                                                                           piece * std::max(1.0, (double)batch / (double)chunks)) + part * parts, chunks, 1, 128});
   }
   return plan_of(best);
 }

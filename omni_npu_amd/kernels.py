@@ -1541,30 +1541,33 @@ def _gqa_best(batch, q_len, q_heads, kv_heads, dim, element_bytes, max_seq_len):
 def gqa_tree_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, dim: int, element_bytes: int, max_seq_len: int):
     """gqa_plan for gqa_tree_decode, whose workgroups have 128 rows that share a head's keys as well: the faster by an estimate in us.
 
-    Of 14 000 measured launches (1-64 requests of 64-32 000 keys, 1-8 key heads of 64 or 128 values, 24-2000 rows) its choice is 1.7 % slower than the
-    best one on average, 15 % in one of twenty; gqa_plan's is 9 % and 59 %.  gqa_plan's own estimate is of the cache's reads; many rows are
+    Of 23 000 measured cases (1-64 requests of 64-32 000 keys, 1-8 key heads of 64 to 256 values, 24-2000 rows) its choice is 1.7 % slower than the
+    best one on average, 15 % in one of twenty; gqa_plan's is 10 % and 65 %.  gqa_plan's own estimate is of the cache's reads; many rows are
     bound by products: 9.3 and, for 1e9 times (row, key, value of a head), 10.9 with 64 rows to a workgroup, 17 with fewer, a third more for
-    heads of 64.  128 rows: a workgroup's step of 32 keys takes 1.2, heads of 64 0.9, four fifths of that where it has a CU to itself (256
-    workgroups and fewer; 512 run at once), 2.3 for each piece of a sequence; 7.4 for one launch, 13.3 for two, 2.1 for a million values of
-    partial results.  us, 64 / 128 rows: 26 requests of 14 500 keys, 126 rows, 8 key heads of 128, 417 / 261; 3 of 7500, 544 rows, 2 key heads,
-    52 / 49; one of 4096, 240 rows, 8 key heads, 27 / 31; 24-32 rows are a quarter slower with 128."""
+    heads of 64; 12.7 and 10 for heads of 256.  128 rows: a workgroup's step of 32 keys takes 1.2, heads of 64 0.9, four fifths of that where it
+    has a CU to itself (256 workgroups and fewer; 512 run at once), heads of 256 1.7 (256 at once); 2.3 for each piece of a sequence, 5.3 with
+    heads of 256; 7.4 for one launch, 13.3 for two (10.2 and 16.7), 2.1 (1.7) for a million values of partial results.  us, without / with
+    128 rows: 26 requests of 14 500 keys, 126 rows, 8 key heads of 128, 417 / 261; 3 of 7500, 544 rows, 2 key heads, 52 / 49; one of 4096, 240
+    rows, 8 key heads, 27 / 31; 8 of 2000-16 000, 480 rows, 4 key heads of 256, 719 / 303; 16 of 1000-8000, 104 rows, 170 / 103; 24-32 rows are
+    a quarter slower."""
     estimate, chunks, heads, tile = _gqa_best(batch, q_len, q_heads, kv_heads, dim, element_bytes, max_seq_len)
     rows = q_len * q_heads // kv_heads
-    if rows <= 32 or dim > 128:
+    if rows <= 32:
         return chunks, heads, tile
-    estimate = max(estimate, 9.3 + batch * max_seq_len * kv_heads * -(-rows // tile) * tile * dim / 1e9 * (10.9 if tile == 64 else 17.0) * (1.3 if dim == 64 else 1.0))
-    best = (estimate, chunks, heads, tile)
-    step = 1.2 if dim == 128 else 0.9
+    wide = dim > 128
+    start, rate = (12.7, 10.0) if wide else (9.3, (10.9 if tile == 64 else 17.0) * (1.3 if dim == 64 else 1.0))
+    best = (max(estimate, start + batch * max_seq_len * kv_heads * -(-rows // tile) * tile * dim / 1e9 * rate), chunks, heads, tile)
+    step, piece, one, two, part, slots = (1.7, 5.3, 10.2, 16.7, 1.7, 256) if wide else (1.2 if dim == 128 else 0.9, 2.3, 7.4, 13.3, 2.1, 512)
     groups = -(-rows // 128) * kv_heads
-    alone = lambda workgroups: 0.8 if workgroups <= 256 else 1.0
+    alone = lambda workgroups: 0.8 if workgroups <= 256 and not wide else 1.0
     if max_seq_len <= 2048:
         workgroups = batch * groups
-        best = min(best, (7.4 + -(-workgroups // 512) * (-(-max_seq_len // 32) * step * alone(workgroups) + 2.3), 0, 1, 128))
-    for workgroups in (256, 512, 1024):
+        best = min(best, (one + -(-workgroups // slots) * (-(-max_seq_len // 32) * step * alone(workgroups) + piece), 0, 1, 128))
+    for workgroups in (slots // 2, slots, 2 * slots):
         chunks = max(1, min(batch * -(-max_seq_len // 64), workgroups // groups))
         size = -(-batch * -(-max_seq_len // 32) // chunks)
         parts = min(1.0 + chunks / batch, float(chunks)) * (batch * q_len * q_heads * dim) / 1e6
-        best = min(best, (13.3 + -(-chunks * groups // 512) * (size * step * alone(chunks * groups) + 2.3 * max(1.0, batch / chunks)) + 2.1 * parts,
+        best = min(best, (two + -(-chunks * groups // slots) * (size * step * alone(chunks * groups) + piece * max(1.0, batch / chunks)) + part * parts,
                           chunks, 1, 128))
     return best[1:]
 

@@ -20,7 +20,7 @@ def test_lengths_and_chunks(dev, lens, q_len, chunks):
     check(c, *call(dev, c, q_len, num_chunks=chunks, **WIDE))
 
 
-@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "fp16"])
 @pytest.mark.parametrize("fp8", [False, True], ids=["same", "e4m3"])
 @pytest.mark.parametrize("q_len,hq,hk,page", [(3, 4, 1, 16), (5, 8, 8, 64), (7, 6, 3, 48), (12, 32, 2, 128), (30, 40, 4, 80), (33, 5, 5, 32), (64, 28, 4, 16)])
@@ -45,7 +45,7 @@ def test_scores_that_grow(dev, dtype, gain):
 
 
 @pytest.mark.parametrize("q_len,words", [(64, 2), (65, 2), (129, 3), (300, 5), (512, 8)])
-@pytest.mark.parametrize("d,hq", [(64, 4), (128, 6)])
+@pytest.mark.parametrize("d,hq", [(64, 4), (128, 6), (256, 2)])
 def test_large_trees(dev, q_len, words, d, hq):
     """Several groups of rows, tokens that are shared by two, trees over many tiles."""
     c = tree(make(dev, [q_len, 700, q_len + 31], q_len=q_len, hq=hq, hk=2, d=d, page=16, seed=q_len), seed=1, words=words)
@@ -55,7 +55,7 @@ def test_large_trees(dev, q_len, words, d, hq):
 
 @pytest.mark.parametrize("window", [1, 2, 5, 15, 64, 100, 1000, 2 ** 31])
 @pytest.mark.parametrize("q_len,words", [(1, 1), (9, 1), (70, 2)])
-@pytest.mark.parametrize("d,page,fp8", [(64, 16, False), (128, 128, True), (128, 48, False)])
+@pytest.mark.parametrize("d,page,fp8", [(64, 16, False), (128, 128, True), (128, 48, False), (256, 16, False), (256, 64, True)])
 def test_windows(dev, window, q_len, words, d, page, fp8):
     c = tree(make(dev, [900, q_len, 64 + q_len, 257, 0], q_len=q_len, hq=8, hk=4, d=d, page=page, fp8=fp8, seed=window % 1001), seed=window % 1001, words=words)
     for chunks in (0, 7):
@@ -94,7 +94,7 @@ def test_more_tokens_than_keys(dev):
 
 @pytest.mark.parametrize("what,fp8", [(float("nan"), False), (float("inf"), False), (-float("inf"), False), (float("nan"), True)], ids=str)
 @pytest.mark.parametrize("chunks", [0, 6])
-@pytest.mark.parametrize("q_len,hq,hk,d", [(9, 8, 2, 64), (33, 16, 4, 128), (50, 32, 2, 64)])
+@pytest.mark.parametrize("q_len,hq,hk,d", [(9, 8, 2, 64), (33, 16, 4, 128), (50, 32, 2, 64), (20, 16, 2, 256)])
 def test_what_a_token_does_not_see_does_not_reach_it(dev, what, fp8, chunks, q_len, hq, hk, d):
     """Pages' free rows, and tokens that are not among a token's ancestors: their keys and values hold what is no number."""
     c = tree(make(dev, [q_len, 150, 64 + q_len], q_len=q_len, hq=hq, hk=hk, d=d, fp8=fp8, page=16, seed=q_len), seed=4)
@@ -203,7 +203,7 @@ def test_many_requests(dev, batch, chunks):
     check(c, *call(dev, c, 4, num_chunks=chunks, **WIDE))
 
 
-@pytest.mark.parametrize("lens,q_len,hq,hk,d", [([3000] * 6, 40, 32, 8, 128), ([9000, 20], 64, 32, 4, 64), ([1500] * 40, 20, 32, 4, 128)])
+@pytest.mark.parametrize("lens,q_len,hq,hk,d", [([3000] * 6, 40, 32, 8, 128), ([9000, 20], 64, 32, 4, 64), ([1500] * 40, 20, 32, 4, 128), ([2500] * 16, 26, 16, 4, 256)])
 def test_what_the_rule_chooses(dev, lens, q_len, hq, hk, d):
     """Work that it gives 128 rows to a workgroup."""
     from omni_npu_amd import kernels as K
