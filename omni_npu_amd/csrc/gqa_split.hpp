@@ -812,34 +812,42 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
   } while (v_cur < v_end);
 }
 
-// The partials of a sequence's chunks into its rows, by the weights exp2(lse_k - max lse): kWaves wavefronts for a row, lanes of 4 dims,
-// several partials at once.  A wavefront goes by its own partials' largest log-sum-exp, so that all it reads of them is asked for together.
+// The partials of a sequence's chunks into its rows, by the weights exp2(lse_k - max lse): lanes of 4 dims, kWaves wavefronts for a row, each with
+// several partials at once; or (0) the lanes of several rows in a wavefront, each of which goes through its partials, four at once.  Both go by their
+// own partials' largest log-sum-exp, so that all that is read of them is asked for together.
 // They are kept in log2 units: behind a product the compiler would subtract from the unrounded one, which is far off beyond 2^32.
-// Bound by the launch and two dependent reads: 2.2 us for 4 rows of 32 partials, 4.4 for 64 x 32 rows of 2 to 4, 8.4 for 128 x 128 of them, 45 MB.
-// A weight is at most 2^-24 (kFar), so that sums over results of any size stay finite.
+// Bound by the launch and two dependent reads: 2.2 us for 4 rows of 32 partials by four wavefronts; 64 requests x 256 rows of 128 dims of 2 partials 5.8,
+// 8 x 3840 of 3 10 (47 MB), where a wavefront for a row took 8.8 and 13; still ahead of it with 8 partials to a request, 194.8 / 195.2 with the
+// attention.  A weight is at most 2^-24 (kFar), so that sums over results of any size stay finite.
 constexpr float kFar = 24.f;
 template <bool kTree, typename T, int D, int kWaves>
 __global__ __launch_bounds__(256) void gqa_join_kernel(const Params p) {
   __shared__ float part[4][D], stat[4][2];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave % kWaves;
+  constexpr int kLanes = D / 4, kPer = 64 / kLanes;          // lanes of a partial; partials, or rows, of a wavefront at once
+  constexpr int kApart = kWaves == 0 ? 1 : kWaves * kPer;    // between a lane's partials
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / kLanes, gi = lane % kLanes;
   const int b = blockIdx.y, rows_max = p.max_q_len * p.group;
-  const int item = blockIdx.x * (4 / kWaves) + wave / kWaves;
+  int item, w = 0;
+  if constexpr (kWaves == 0) {
+    item = (blockIdx.x * 4 + wave) * kPer + sub;
+  } else {
+    item = blockIdx.x * (4 / kWaves) + wave / kWaves;
+    w = wave % kWaves * kPer + sub;
+  }
   const int first = ((ConstPtr)p.seg_ids)[2 * b], last = ((ConstPtr)p.seg_ids)[2 * b + 1];
   const Seq sq = seq_at<kTree>(p, b);
   if (first < 0) return;
   const int hd = (int)((uint32_t)item / (uint32_t)rows_max), r = item - hd * rows_max;
   const bool there = hd < p.kv_heads && r < sq.s * p.group;
-  constexpr int kLanes = D / 4, kPer = 64 / kLanes;          // lanes of a partial; partials of a wavefront at once
-  const int sub = lane / kLanes, gi = lane % kLanes;
   const int64_t stride = (int64_t)p.kv_heads * rows_max, base = there ? (int64_t)hd * rows_max + r : 0;
   float most = -INFINITY, sum = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = first + w * kPer + sub; s0 <= last; s0 += 4 * kWaves * kPer) {
+  for (int s0 = first + w; s0 <= last; s0 += 4 * kApart) {
     float l[4], next = most;
     f32x4 a[4];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      const int s = s0 + k * kWaves * kPer, at = s <= last ? s : last;
+      const int s = s0 + k * kApart, at = s <= last ? s : last;
       l[k] = p.part_lse[at * stride + base];
       a[k] = *(const f32x4*)(p.part_acc + (at * stride + base) * D + gi * 4);
       l[k] = s <= last ? l[k] : -INFINITY;
@@ -861,17 +869,19 @@ __global__ __launch_bounds__(256) void gqa_join_kernel(const Params p) {
   }
   // the wavefront's partials side by side, then the row's wavefronts
   float top = most;
+  if constexpr (kWaves > 0) {
 #pragma unroll
-  for (int o = kLanes; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-  const float f = fast_exp2(most - (top == -INFINITY ? 0.f : top));
-  sum *= f;
+    for (int o = kLanes; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    const float f = fast_exp2(most - (top == -INFINITY ? 0.f : top));
+    sum *= f;
 #pragma unroll
-  for (int e = 0; e < 4; e++) acc[e] *= f;
+    for (int e = 0; e < 4; e++) acc[e] *= f;
 #pragma unroll
-  for (int o = kLanes; o < 64; o <<= 1) {
-    sum += __shfl_xor(sum, o, 64);
+    for (int o = kLanes; o < 64; o <<= 1) {
+      sum += __shfl_xor(sum, o, 64);
 #pragma unroll
-    for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], o, 64);
+      for (int e = 0; e < 4; e++) acc[e] += __shfl_xor(acc[e], o, 64);
+    }
   }
   if constexpr (kWaves > 1) {
     if (sub == 0) {
@@ -896,7 +906,7 @@ __global__ __launch_bounds__(256) void gqa_join_kernel(const Params p) {
     }
     top = all;
   }
-  if (!there || sub != 0) return;
+  if (!there || (kWaves > 0 && sub != 0)) return;
   const int tk = p.max_q_len == 1 ? 0 : (int)((uint32_t)r / (uint32_t)p.group);
   const int64_t t = (int64_t)sq.q0 + tk;
   if (t < 0 || t >= p.num_tokens) return;
@@ -910,10 +920,10 @@ __global__ __launch_bounds__(256) void gqa_join_kernel(const Params p) {
 
 template <bool kTree, typename T, int D>
 int launch_join(const char* me, const Params& p, hipStream_t st) {
-  // a wavefront for a row where the chunks leave a few partials to a request, four where they leave many
+  // the rows of a wavefront side by side where the chunks leave a few partials to a request, four wavefronts to a row where they leave many
   const int items = p.kv_heads * p.max_q_len * p.group;
   if (p.num_chunks > 8 * p.batch) hipLaunchKernelGGL((gqa_join_kernel<kTree, T, D, 4>), dim3((unsigned)items, (unsigned)p.batch), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((gqa_join_kernel<kTree, T, D, 1>), dim3((unsigned)((items + 3) / 4), (unsigned)p.batch), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((gqa_join_kernel<kTree, T, D, 0>), dim3((unsigned)((items + 1024 / D - 1) / (1024 / D)), (unsigned)p.batch), dim3(256), 0, st, p);
   return check_launch(me);
 }
 template <bool kTree, typename T, int D, bool kFp8, int MT>
