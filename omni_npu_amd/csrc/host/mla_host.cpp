@@ -834,20 +834,23 @@ Caches page_caches(py::handle cache_list) {
   auto cache = [&](Py_ssize_t i) -> const Tensor& { return THPVariable_Unpack(PyList_GET_ITEM(cache_list.ptr(), i)); };
   if (num == 0 || !current_gpu(cache(0))) return to;
   const Tensor& first = cache(0);
+  const at::Device dev = first.device();
+  if (first.dim() < 2) return to;
+  const int64_t pages = first.size(0), page = first.size(1);
+  if (pages < 1 || page < 1) return to;
   to.list.reserve(num);
   for (Py_ssize_t k = 0; k < num; k++) {
     const Tensor& c = cache(k);
-    if (c.dim() < 2 || c.device() != first.device() || c.size(0) < 1 || c.size(1) < 1 || c.size(0) != first.size(0) || c.size(1) != first.size(1) ||
-        wants_grad({&c}))
-      return Caches{};
+    const c10::IntArrayRef sizes = c.sizes(), strides = c.strides();   // (looked up once: a call of copies may name a hundred caches)
+    if (sizes.size() < 2 || sizes[0] != pages || sizes[1] != page || c.device() != dev || wants_grad({&c})) return Caches{};
     int64_t width = 1;
-    for (int64_t i = c.dim() - 1; i >= 2; i--) {               // (rows of contiguous elements)
-      if (c.size(i) != 1 && c.stride(i) != width) return Caches{};
-      width *= c.size(i);
+    for (size_t i = sizes.size() - 1; i >= 2; i--) {           // (rows of contiguous elements)
+      if (sizes[i] != 1 && strides[i] != width) return Caches{};
+      width *= sizes[i];
     }
     // (the stride of a dim of one entry says nothing)
-    const int64_t es = c.element_size(), row = width * es, row_stride = c.size(1) > 1 ? c.stride(1) * es : row;
-    to.list.push_back({c.data_ptr(), c.size(0) > 1 ? c.stride(0) * es : row_stride * c.size(1), row_stride, row});
+    const int64_t es = c.element_size(), row = width * es, row_stride = page > 1 ? strides[1] * es : row;
+    to.list.push_back({c.data_ptr(), pages > 1 ? strides[0] * es : row_stride * page, row_stride, row});
   }
   to.first = &first;
   return to;
