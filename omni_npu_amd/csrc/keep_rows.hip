@@ -132,6 +132,15 @@ extern "C" int mlahip_keep_rows(const mlahip_page_cache* caches, int32_t num_cac
                 MLA_ERR_SHAPE, "%s: cache %d: pages that share memory: rows of %lld bytes, %lld apart, %d to a page, pages %lld apart", me, i,
                 (long long)c.row_bytes, (long long)c.row_stride_bytes, page_size, (long long)c.page_stride_bytes);
   }
+  // Two moves of the same rows would take each other's results for what they read.  (A bit for an address: looked at again where two have one.)
+  uint64_t bits[64] = {};
+  for (int32_t i = 0; i < num_caches; i++) {
+    const uint32_t at = (uint32_t)((uint64_t)(uintptr_t)caches[i].base * 0x9e3779b97f4a7c15ull >> 52);
+    const bool met = bits[at >> 6] >> (at & 63) & 1;
+    for (int32_t k = 0; met && k < i; k++)
+      MLA_REQUIRE(caches[k].base != caches[i].base, MLA_ERR_UNSUPPORTED, "%s: caches %d and %d are the same", me, k, i);
+    bits[at >> 6] |= 1ull << (at & 63);
+  }
   if (batch == 0) return MLA_OK;
   const char *out = (const char*)kept_lens, *out_end = out + batch * 4ll;
   const auto meets = [&](const void* at, int64_t bytes) { return at && (const char*)at < out_end && out < (const char*)at + bytes; };

@@ -99,6 +99,10 @@ def test_keep_rows_codes():
     assert rc(cache=(None, 1 << 24, 1 << 22, 1 << 22)) == -2   # rows of 4 MB
     assert rc(_14=at(2)) == -3 and rc(_14=at(3) + 8) == -3 and rc(_14=at(4) + 40) == -3 and rc(_14=at(5)) == -3 and rc(_14=at(1) + 64) == -3
     assert rc(_14=at(6) + 2) == -2
+    two = (ctypes.c_int64 * 8)(at(0), 64, 16, 16, at(0), 64, 16, 8)
+    assert rc(_0=two, _1=2) == -3                              # the same cache twice
+    two[4] += 512
+    assert rc(_0=two, _1=2, _9=0) == 0
     assert rc(_9=0) == 0
     del raw
 
