@@ -694,7 +694,7 @@ std::tuple<int, int, int> gqa_tree_plan(int64_t batch, int64_t q_len, int64_t q_
   if (rows <= 32) return plan_of(best);
   const bool wide = dim > 128;
   const double start = wide ? 12.7 : 9.3, rate = wide ? 10.0 : (tile == 64 ? 10.9 : 17.0) * (dim == 64 ? 1.3 : 1.0);
-  std::get<0>(best) = std::max(std::get<0>(best), start + (double)(batch * max_seq_len * kv_heads * div_up(rows, tile) * tile * dim) / 1e9 * rate);
+  std::get<0>(best) = std::max(std::get<0>(best), start + (double)batch * (double)max_seq_len * (double)kv_heads * (double)(div_up(rows, tile) * tile * dim) / 1e9 * rate);
   const double step = wide ? 1.7 : dim == 128 ? 1.2 : 0.9, piece = wide ? 5.3 : 2.3, one = wide ? 10.2 : 7.4, two = wide ? 16.7 : 13.3, part = wide ? 1.7 : 2.1;
   const int64_t groups = div_up(rows, 128) * kv_heads, slots = wide ? 256 : 512;
   const auto alone = [&](int64_t workgroups) { return workgroups <= 256 && !wide ? 0.8 : 1.0; };
@@ -741,7 +741,10 @@ bool gqa(const Tensor* bits, const Tensor& q, const Tensor& k_cache, const Tenso
   int64_t longest = block_table.size(1) * k_cache.size(1);
   if (max_seq_len && c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) longest = std::min(longest, *max_seq_len);
   if (window > 0) longest = std::min(longest, window + q_len + (bits ? 31 : 30));
-  const auto [by_rule, heads, rows] = (bits ? gqa_tree_plan : gqa_plan)(b, q_len, hq, hk, d, k_cache.element_size(), longest);
+  // (128 rows to a workgroup only where the caller's own choice, if there is one, leaves it)
+  const bool wide = bits && heads_per_group.value_or(1) == 1 && rows_per_group.value_or(128) == 128;
+  const auto [by_rule, by_heads, rows] = (wide ? gqa_tree_plan : gqa_plan)(b, q_len, hq, hk, d, k_cache.element_size(), longest);
+  const int heads = rows_per_group == 128 ? 1 : by_heads;
   const int chunks = (int)num_chunks.value_or(by_rule);
   Stream st = stream_of(q);
   const char* what = bits ? "mlahip_gqa_tree_decode" : "mlahip_gqa_decode";

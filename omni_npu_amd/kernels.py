@@ -1556,7 +1556,7 @@ def gqa_tree_plan(batch: int, q_len: int, q_heads: int, kv_heads: int, dim: int,
         return chunks, heads, tile
     wide = dim > 128
     start, rate = (12.7, 10.0) if wide else (9.3, (10.9 if tile == 64 else 17.0) * (1.3 if dim == 64 else 1.0))
-    best = (max(estimate, start + batch * max_seq_len * kv_heads * -(-rows // tile) * tile * dim / 1e9 * rate), chunks, heads, tile)
+    best = (max(estimate, start + float(batch) * max_seq_len * kv_heads * (-(-rows // tile) * tile * dim) / 1e9 * rate), chunks, heads, tile)
     step, piece, one, two, part, slots = (1.7, 5.3, 10.2, 16.7, 1.7, 256) if wide else (1.2 if dim == 128 else 0.9, 2.3, 7.4, 13.3, 2.1, 512)
     groups = -(-rows // 128) * kv_heads
     alone = lambda workgroups: 0.8 if workgroups <= 256 and not wide else 1.0
@@ -1673,7 +1673,10 @@ def _gqa(what, q, k_cache, v_cache, block_table, seq_lens, visible, scale, out, 
             longest = min(longest, max_seq_len)
         if window is not None:
             longest = min(longest, window + q_len + 30 + tree)
-        chunks, heads, rows = (gqa_tree_plan if tree else gqa_plan)(b, q_len, hq, hk, d, k_cache.element_size(), longest)
+        # (128 rows to a workgroup only where the caller's own choice, if there is one, leaves it)
+        plan = gqa_tree_plan if tree and heads_per_group in (None, 1) and rows_per_group in (None, 128) else gqa_plan
+        chunks, heads, rows = plan(b, q_len, hq, hk, d, k_cache.element_size(), longest)
+        heads = 1 if rows_per_group == 128 else heads
         num_chunks = chunks if num_chunks is None else num_chunks
         need = lib.mlahip_gqa_decode_workspace_bytes(b, q_len, hq, d, num_chunks)
         launch = lambda ws: entry(
@@ -1822,7 +1825,8 @@ def keep_rows(caches, block_table: torch.Tensor, context_lens: torch.Tensor, seq
     All of it lies on the device: ``block_table`` int32 [>= B, blocks], ``context_lens`` and ``seq_lens`` int32 [B] as step_tables has them, ``accepted``
     int32 [B,A] (numbers of a request's new tokens, each larger than the one before, as a path down a tree is), ``num_accepted`` and ``kept_lens``
     int32 [B].  A path ends at its first entry that is not larger, that is no token of its request, or whose rows are not in the table or the
-    caches.  Idle places keep their negative length.  Requests must not share the pages that their new tokens lie in."""
+    caches.  Idle places keep their negative length.  Requests must not share the pages that their new tokens lie in, nor caches memory (the same
+    one twice is refused)."""
     what = "keep_rows"
     native = _host.load().keep_rows
     if native(caches, block_table, context_lens, seq_lens, accepted, num_accepted, kept_lens):     # (a list of tensors)

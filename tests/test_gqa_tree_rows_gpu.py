@@ -252,3 +252,16 @@ def test_a_graph_over_other_requests(dev):
             run(**(kw or dict(max_seq_len=1280)))
             torch.cuda.synchronize()
             assert torch.allclose(got.float(), out.float(), rtol=2 ** -7, atol=1e-3)
+
+
+@pytest.mark.parametrize("kw", [dict(heads_per_group=2), dict(heads_per_group=4), dict(rows_per_group=16), dict(rows_per_group=128), dict(num_chunks=3),
+                                dict(heads_per_group=1)], ids=str)
+@pytest.mark.parametrize("path", ["native", "general"])
+def test_a_choice_of_the_callers_and_the_rules(dev, kw, path):
+    """Where the rule would choose 128 rows, which go with one key head alone: what the caller names holds, and the rest follows it."""
+    from omni_npu_amd import kernels as K
+    c = tree(make(dev, [3000] * 6, q_len=40, hq=32, hk=8, page=64, seed=1), seed=1)
+    assert K.gqa_tree_plan(6, 40, 32, 8, 128, 2, c["table"].shape[1] * 64)[2] == 128
+    if path == "general":
+        kw = dict(kw, workspace=torch.empty(1 << 28, dtype=torch.uint8, device=dev))
+    check(c, *call(dev, c, 40, **kw))
