@@ -1,4 +1,4 @@
-// The rows of an accepted path moved to the places behind the context, in all layers' caches at once, when a step's drafted tokens have been judged.
+// The rows of an accepted path moved to the places behind the context, in all layers' caches at once, when it is known which of a step's drafted tokens stay.
 //
 //   row(c + d) = row(c + accepted[d])   for d < kept, every cache of the list and every request b; its new length is c + kept
 //   row(x): the cache row of a request's place x by its block table;  kept: how many of the first num_accepted entries are each larger than the one
