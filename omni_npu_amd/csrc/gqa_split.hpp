@@ -27,7 +27,7 @@
 //
 // Measured, split and join together: 64 requests x 4096-8192 keys x 32/8 heads of 128 (1630 MB) 251 us, 6.5 TB/s; one of 131 072 x 64/8 90 us,
 // 5.9; 128 x 2 tokens x 2048-16 384 keys x 64/8 over the 8-bit cache (2440 MB) 397 us, 6.1; 33 requests x the newest 1024 keys x 16/4 heads of
-// 256, pages of 16 (137 MB) 34 us, 4.0: four wavefronts to a CU (a wavefront's sums, keys and values take 300 registers, a second workgroup would
+// 256, pages of 16 (137 MB) 33 us, 4.1: four wavefronts to a CU (a wavefront's sums, keys and values take 300 registers, a second workgroup would
 // not fit), five tiles each, and most chunks begin a second sequence.  One request x 1021 keys x 4/1 heads 8.7 us: 6.5 of the split, whose loads
 // hang on one another (length, page, keys and values, partial results), 2.2 of the join.
 #pragma once
