@@ -77,6 +77,8 @@ template <int n> __device__ __forceinline__ void wait_loads() {
 template <int n> using Int = std::integral_constant<int, n>;
 template <typename F, int... i> __device__ __forceinline__ void each_of(F f, std::integer_sequence<int, i...>) { (f(Int<i>{}), ...); }
 template <int n, typename F> __device__ __forceinline__ void each(F f) { each_of(f, std::make_integer_sequence<int, n>{}); }
+constexpr float kFine = 0x1p10f;                             // (log2 units: scores and references below it are off by half a step, 2^-15, at most)
+constexpr float kNone = -0x1.fffffep127f, kAlways = -0x1p126f;   // limits of scores against a reference: of a row that has none, of one that is looked at in each tile
 constexpr int kNowhere = 0x7effffc0;                         // a key that no request has (they have at most 2^30, and 2^24 tokens in front of the first)
 
 template <typename T, int D, bool kFp8>
@@ -246,16 +248,17 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), (D > 128 ? 1 : 2)) void g
       {
         const int64_t t = (int64_t)sq.q0 + tok;
         const bool ok = r < rows && t >= 0 && t < first->num_tokens;
-        const GLOBAL char* src = (const GLOBAL char*)first->q + (ok ? t : 0) * first->q_st + (int64_t)(head * p.group + (rr - tok * p.group)) * first->q_sh;
+        const GLOBAL char* src = (const GLOBAL char*)first->q + (ok ? t : 0) * first->q_st + (int64_t)(head * p.group + (rr - tok * p.group)) * first->q_sh +
+                                 here(h32) * 16;   // (here: not kept in front of the loop over the pieces)
 #pragma unroll
-        for (int s = 0; s < D / 16; s++) qf[s] = ok ? *(const GLOBAL u32x4*)(src + (s * 16 + h32 * 8) * 2) : u32x4{0u, 0u, 0u, 0u};
+        for (int s = 0; s < D / 16; s++) qf[s] = ok ? *(const GLOBAL u32x4*)(src + s * 32) : u32x4{0u, 0u, 0u, 0u};
       }
       int lo = 0;
       if (p.window > 0) {
         const int left = window_left(visible_of(tok));
         lo = sq.key_0 - (left > 0 ? left : 0);
       }
-      const float scale_log2 = first->scale_log2 * (kFp8 && first->k_scale ? ((const GLOBAL float*)first->k_scale)[head] : 1.f);
+      float scale_log2 = first->scale_log2 * (kFp8 && first->k_scale ? ((const GLOBAL float*)first->k_scale)[head] : 1.f);
       const int all_hi = sq.key_0, all_lo = p.window > 0 ? sq.len - p.window : 0, any_lo = p.window > 0 ? sq.key_0 - p.window : 0;
       int only = -1;                                         // the token that a pass is for, where the piece is done token by token
       while (true) {
@@ -270,7 +273,7 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), (D > 128 ? 1 : 2)) void g
         f32x16 acc[D / 32];
         float y[16];                                         // scores against the reference, log2 units
         u32x4 pf[2], pl[2];                                  // probabilities of 32 keys, 16 a product, in two operands
-        float sum[2] = {0.f, 0.f}, ref = 0.f, limit = -0x1.fffffep127f;  // limit: above which a score sets the row's reference anew; none set yet
+        float sum[2] = {0.f, 0.f}, ref = 0.f, limit = kNone;  // limit: above which a score sets the row's reference anew
 #pragma unroll
         for (int d = 0; d < D / 32; d++)
 #pragma unroll
@@ -331,7 +334,16 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), (D > 128 ? 1 : 2)) void g
             else wait_loads<0>();
           }
         };
-        // Where a score outgrows its row's reference it is set anew: what is summed up, and the probabilities that are not yet, by a whole power of two.
+        // Addresses in LDS of a lane's first granule of this tile's keys, and of the values of the one before it.  (A granule 2 n further: bits of n are
+        // flipped.  Worked out in front of the loop, by the lane's number hidden from the compiler: it would keep them in memory until then.)
+        uint32_t k_lane = 0, v_lane = 0;
+        auto read_k = [&](int n) { return *(LDS_PTR(const u32x4))(k_lane ^ n << 5); };   // 16 dims
+        auto read_v = [&](int n) {                           // 32 dims, 16 keys in the order of the scores: 4 h32 + 0 .. 3, then 8 further
+          const uint32_t row = (v_lane ^ n % (D / 32) << 6) + n / (D / 32) * 16 * W::row_b;
+          const u32x2 x0 = read_tr(row), x1 = read_tr(row + 8 * W::row_b);
+          return u32x4{x0[0], x0[1], x1[0], x1[1]};
+        };
+        // Where a score outgrows its row's reference the wavefront's are set anew (all of them: the next would follow soon): what is summed up, and the probabilities that are not yet, by a whole power of two.
         auto check = [&](int key, bool partial, float most) {
           if (partial) {
             const uint32_t bits = (tile_bits(tok, key) & ~bits_to(lo - key)) >> 4 * h32;
@@ -342,15 +354,37 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), (D > 128 ? 1 : 2)) void g
               most = fmaxf(most, y[e]);
             }
           }
-          if (__builtin_amdgcn_ballot_w64(most > limit)) {
+          if (__builtin_expect(__builtin_amdgcn_ballot_w64(most > limit) != 0, 0)) {
             most = fmaxf(most, __shfl_xor(most, 32, 64));
-            if (most > -INFINITY) {
-              const bool first_one = limit != Ty::kBelow + Ty::kOutgrown;
+            // Large scores: the turn's y is an unrounded score less the reference, the tile's that set the reference a rounded one's, and a reference
+            // does not move by less than its own steps: equal scores would weigh more or less by the tile that they lie in (at 2^20 by 4 %, beyond 2^25 all of it).
+            // So each tile of such a row is looked at here, and has its products again: rounded, then less the reference, which is a whole number near them.
+            const bool anew = most > -INFINITY, large = anew && (fabsf(ref) >= kFine || fabsf(ref + most) >= kFine);
+            const float before = ref;
+            if (__builtin_expect(__builtin_amdgcn_ballot_w64(large) != 0, 0)) {
+              f32x16 sc = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int n = 0; n < D / 16; n++) sc = Wd::mm(read_k(n), qf[n], sc);
+              float all = -INFINITY;
+#pragma unroll
+              for (int e = 0; e < 16; e++) {
+                const float s = here(sc[e] * scale_log2);      // (by itself, not one operation with the difference)
+                y[e] = large && y[e] != -INFINITY ? s : y[e];
+                all = fmaxf(all, y[e]);
+              }
+              all = fmaxf(all, __shfl_xor(all, 32, 64));
+              if (large) {
+                most = all;
+                ref = 0.f;
+              }
+            }
+            if (anew) {
               float raise = __builtin_ceilf(most - (fabsf(ref + most) < 0x1p20f ? Ty::kBelow : 0.f));
-              raise = !first_one && raise < 0.f ? 0.f : raise;
-              const float f = first_one ? 1.f : fast_exp2(-raise);   // (zeros so far)
-              limit = Ty::kBelow + Ty::kOutgrown;
+              // (a row that has a reference keeps it or gets a higher one)
+              raise = limit == kNone ? raise : fmaxf(raise, before - ref);
+              const float f = limit == kNone ? 1.f : fast_exp2(before - (ref + raise));   // (zeros so far)
               ref += raise;
+              limit = fabsf(ref) < kFine ? Ty::kBelow + Ty::kOutgrown : kAlways;
               sum[0] *= f;
               sum[1] *= f;
 #pragma unroll
@@ -368,15 +402,6 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), (D > 128 ? 1 : 2)) void g
                 }
             }
           }
-        };
-        // Addresses in LDS of a lane's first granule of this tile's keys, and of the values of the one before it.  (A granule 2 n further: bits of n are
-        // flipped.  Worked out in front of the loop, by the lane's number hidden from the compiler: it would keep them in memory until then.)
-        uint32_t k_lane = 0, v_lane = 0;
-        auto read_k = [&](int n) { return *(LDS_PTR(const u32x4))(k_lane ^ n << 5); };   // 16 dims
-        auto read_v = [&](int n) {                           // 32 dims, 16 keys in the order of the scores: 4 h32 + 0 .. 3, then 8 further
-          const uint32_t row = (v_lane ^ n % (D / 32) << 6) + n / (D / 32) * 16 * W::row_b;
-          const u32x2 x0 = read_tr(row), x1 = read_tr(row + 8 * W::row_b);
-          return u32x4{x0[0], x0[1], x1[0], x1[1]};
         };
         // One turn: the scores of the next 32 keys, these ones' probabilities, the products of the ones before with their values.  Products and the
         // rest take turns, in this order: the matrix cores work on the one while the wavefront issues the other.  D / 16 products for the scores, S, and
@@ -466,7 +491,8 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), (D > 128 ? 1 : 2)) void g
         ask(0);
         lds_barrier();                                       // (the words and the flag are there; nobody reads the tiles of the pass before)
         for (int n = threadIdx.x; n < W::lag * W::tile_b / 16; n += W::threads) ((u32x4*)(lds + (8 - W::lag) * W::tile_b))[n] = u32x4{0u, 0u, 0u, 0u};
-        // (the queries have arrived here: the compiler would wait for them, and so for all loads, at the loop's top)
+        // (the queries and the keys' scale have arrived here: the compiler would wait for them, and so for all loads, at the loop's top)
+        asm volatile("" : "+v"(scale_log2));
 #pragma unroll
         for (int s = 0; s < D / 16; s++) asm volatile("" : "+v"(qf[s]));
         if constexpr (kFp8) come(0);
@@ -508,7 +534,8 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), (D > 128 ? 1 : 2)) void g
         }
         if (!by_token) {
           const ParamsPtr last = reload();
-          const float vs = kFp8 && last->v_scale ? ((const GLOBAL float*)last->v_scale)[head] : 1.f;
+          // (waited for here: a wavefront that makes no use of it would take the load along, and the next piece's loop wait for it at its top)
+          const float vs = here(kFp8 && last->v_scale ? ((const GLOBAL float*)last->v_scale)[head] : 1.f);
           const int64_t t = (int64_t)sq.q0 + tok;
           // (the sum is of the probabilities in fp32: both operands of one are kWhole of it up to their rounding)
           const float total = sum[0] + sum[1] + __shfl_xor(sum[0] + sum[1], 32, 64), inv = total == 0.f ? 0.f : vs / (total * kWhole);
@@ -517,7 +544,7 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), (D > 128 ? 1 : 2)) void g
             const int qh = head * p.group + (r - tok * p.group);
             if (whole) {
               if (last->lse && h32 == 0) ((GLOBAL float*)last->lse)[t * (p.kv_heads * p.group) + qh] = lse2 * kLn2;
-              GLOBAL char* dst = (GLOBAL char*)last->out + t * last->o_st + (int64_t)qh * last->o_sh + h32 * 8;
+              GLOBAL char* dst = (GLOBAL char*)last->out + t * last->o_st + (int64_t)qh * last->o_sh + here(h32) * 8;
 #pragma unroll
               for (int d = 0; d < D / 32; d++)
 #pragma unroll
