@@ -64,7 +64,7 @@ struct Params {
   char* out; int64_t o_st, o_sh;
   float* lse;                                                // [T, heads] or null
   int32_t* seg_ids;                                          // [batch][2]: first and last partial of a sequence, or -1
-  float *part_lse, *part_acc;                                // [slot][kv head][row](, [D]); log-sum-exps in log2 units
+  f32x2* part_lse; float* part_acc;                          // [slot][kv head][row](, [D]); log-sum-exps in log2 units, each as a sum of two
   const uint64_t* visible; int64_t visible_stride; int32_t words;   // trees: [T][words], a token's bits
 };
 
@@ -142,6 +142,13 @@ __device__ __forceinline__ Seq seq_at(const Params& p, int b) {
 __device__ __forceinline__ int chunk_units(int tot, int n) {
   tot += n - 1;
   return tot < (1 << 21) ? (int)(((float)tot + 0.5f) * __builtin_amdgcn_rcpf((float)n)) : (int)((uint32_t)tot / (uint32_t)n);
+}
+
+// A piece's log-sum-exp, its reference and the sum's logarithm, as what the sum of both is rounded to and what that leaves: at 2^20 one float alone would be off
+// by 4 % of the piece's weight, and beyond 2^25 pieces of one key and of thousands would weigh the same.
+__device__ __forceinline__ f32x2 lse_of(float ref, float log_sum) {
+  const float hi = ref + log_sum, b = hi - ref, lo = (ref - (hi - b)) + (log_sum - b);
+  return f32x2{hi, fabsf(hi) < INFINITY ? lo : 0.f};
 }
 
 // A page as a buffer, and 16 bytes out of it that are read once: at the lane's offset and a scalar one.  (Host: no page takes 2^31 bytes.)
@@ -702,13 +709,13 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
         const int tk = p.max_q_len == 1 ? 0 : (int)((uint32_t)r / (uint32_t)p.group), qh = hd * p.group + (r - tk * p.group);
         const int64_t t = (int64_t)sq.q0 + tk;
         if ((only >= 0 && tk != only) || (whole && (t < 0 || t >= last->num_tokens))) return (char*)nullptr;
-        const float lse2 = total == 0.f ? -INFINITY : most + (fast_log2(total) - kWholeLog2);
+        const f32x2 lse2 = total == 0.f ? f32x2{-INFINITY, 0.f} : lse_of(most, fast_log2(total) - kWholeLog2);
         if (whole) {
-          if (last->lse && first_dims) ((GLOBAL float*)last->lse)[t * (p.kv_heads * p.group) + qh] = lse2 * kLn2;
+          if (last->lse && first_dims) ((GLOBAL float*)last->lse)[t * (p.kv_heads * p.group) + qh] = lse2[0] * kLn2;
           return last->out + t * last->o_st + (int64_t)qh * last->o_sh;
         }
         const int64_t slot = ((int64_t)(blockIdx.x + b) * p.kv_heads + hd) * (p.max_q_len * p.group) + r;
-        if (first_dims) ((GLOBAL float*)last->part_lse)[slot] = lse2;
+        if (first_dims) ((GLOBAL f32x2*)last->part_lse)[slot] = lse2;
         return (char*)(last->part_acc + slot * D);
       };
       // Four dims of a row.  Granule gi = 4 d + g'
@@ -822,7 +829,7 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
 constexpr float kFar = 24.f;
 template <bool kTree, typename T, int D, int kWaves>
 __global__ __launch_bounds__(256) void gqa_join_kernel(const Params p) {
-  __shared__ float part[4][D], stat[4][2];
+  __shared__ float part[4][D], stat[4][3];
   constexpr int kLanes = D / 4, kPer = 64 / kLanes;          // lanes of a partial; partials, or rows, of a wavefront at once
   constexpr int kApart = kWaves == 0 ? 1 : kWaves * kPer;    // between a lane's partials
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / kLanes, gi = lane % kLanes;
@@ -840,39 +847,45 @@ __global__ __launch_bounds__(256) void gqa_join_kernel(const Params p) {
   const int hd = (int)((uint32_t)item / (uint32_t)rows_max), r = item - hd * rows_max;
   const bool there = hd < p.kv_heads && r < sq.s * p.group;
   const int64_t stride = (int64_t)p.kv_heads * rows_max, base = there ? (int64_t)hd * rows_max + r : 0;
-  float most = -INFINITY, sum = 0.f;
+  f32x2 most = {-INFINITY, 0.f};
+  float sum = 0.f;
   f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  // A difference of two; the larger of each part, which neither lies above; what to weigh by.  (The differences first: beyond 2^23 a sum with kFar rounds.)
+  auto above = [](f32x2 x, f32x2 y) { return (x[0] - y[0]) + (x[1] - y[1]); };
+  auto higher = [](f32x2 x, f32x2 y) { return f32x2{fmaxf(x[0], y[0]), fmaxf(x[1], y[1])}; };
+  auto base_of = [](f32x2 x) { return f32x2{x[0] == -INFINITY ? 0.f : x[0], x[1]}; };
   for (int s0 = first + w; s0 <= last; s0 += 4 * kApart) {
-    float l[4], next = most;
+    f32x2 l[4], next = most;
     f32x4 a[4];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       const int s = s0 + k * kApart, at = s <= last ? s : last;
       l[k] = p.part_lse[at * stride + base];
       a[k] = *(const f32x4*)(p.part_acc + (at * stride + base) * D + gi * 4);
-      l[k] = s <= last ? l[k] : -INFINITY;
+      l[k] = s <= last ? l[k] : f32x2{-INFINITY, 0.f};
     }
 #pragma unroll
-    for (int k = 0; k < 4; k++) next = fmaxf(next, l[k]);
-    const float ref = next == -INFINITY ? 0.f : next, f = fast_exp2(most - ref), far = ref + kFar;   // (nothing so far: zeros)
+    for (int k = 0; k < 4; k++) next = higher(next, l[k]);
+    const f32x2 ref = base_of(next);
+    const float f = fast_exp2(above(most, ref));             // (nothing so far: zeros)
     sum *= f;
 #pragma unroll
     for (int e = 0; e < 4; e++) acc[e] *= f;
     most = next;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      const float wt = fast_exp2(l[k] - far);
+      const float wt = fast_exp2(above(l[k], ref) - kFar);
       sum += wt;
 #pragma unroll
       for (int e = 0; e < 4; e++) acc[e] += wt == 0.f ? 0.f : wt * a[k][e];
     }
   }
   // the wavefront's partials side by side, then the row's wavefronts
-  float top = most;
+  f32x2 top = most;
   if constexpr (kWaves > 0) {
 #pragma unroll
-    for (int o = kLanes; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    const float f = fast_exp2(most - (top == -INFINITY ? 0.f : top));
+    for (int o = kLanes; o < 64; o <<= 1) top = higher(top, f32x2{__shfl_xor(top[0], o, 64), __shfl_xor(top[1], o, 64)});
+    const float f = fast_exp2(above(most, base_of(top)));
     sum *= f;
 #pragma unroll
     for (int e = 0; e < 4; e++) acc[e] *= f;
@@ -886,21 +899,21 @@ __global__ __launch_bounds__(256) void gqa_join_kernel(const Params p) {
   if constexpr (kWaves > 1) {
     if (sub == 0) {
       *(f32x4*)&part[wave][gi * 4] = acc;
-      if (gi == 0) { stat[wave][0] = top; stat[wave][1] = sum; }
+      if (gi == 0) { stat[wave][0] = top[0]; stat[wave][1] = top[1]; stat[wave][2] = sum; }
     }
     __syncthreads();
     if (wave != 0) return;
-    float all = -INFINITY;
+    f32x2 all = {-INFINITY, 0.f};
 #pragma unroll
-    for (int k = 0; k < kWaves; k++) all = fmaxf(all, stat[k][0]);
-    const float ref = all == -INFINITY ? 0.f : all;
+    for (int k = 0; k < kWaves; k++) all = higher(all, f32x2{stat[k][0], stat[k][1]});
+    const f32x2 ref = base_of(all);
     sum = 0.f;
     acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < kWaves; k++) {
-      const float wt = fast_exp2(stat[k][0] - ref);
+      const float wt = fast_exp2(above(f32x2{stat[k][0], stat[k][1]}, ref));
       const f32x4 a = *(const f32x4*)&part[k][gi * 4];
-      sum += wt * stat[k][1];
+      sum += wt * stat[k][2];
 #pragma unroll
       for (int e = 0; e < 4; e++) acc[e] += wt * a[e];
     }
@@ -915,7 +928,7 @@ __global__ __launch_bounds__(256) void gqa_join_kernel(const Params p) {
 #pragma unroll
   for (int e = 0; e < 4; e++) y[e] = (T)(sum == 0.f ? 0.f : acc[e] / sum);
   *(typename Types<T>::v4*)(p.out + t * p.o_st + (int64_t)qh * p.o_sh + gi * 8) = y;
-  if (p.lse && gi == 0) p.lse[t * (p.kv_heads * p.group) + qh] = sum == 0.f ? -INFINITY : (top + (fast_log2(sum) + kFar)) * kLn2;
+  if (p.lse && gi == 0) p.lse[t * (p.kv_heads * p.group) + qh] = sum == 0.f ? -INFINITY : (top[0] + (top[1] + fast_log2(sum) + kFar)) * kLn2;
 }
 
 template <bool kTree, typename T, int D>
@@ -960,7 +973,7 @@ inline int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 inline size_t workspace_need(int32_t batch, int32_t max_q_len, int32_t q_heads, int32_t dim, int32_t num_chunks) {
   if (batch <= 0 || max_q_len <= 0 || q_heads <= 0 || dim <= 0 || num_chunks <= 0) return 0;
   const int64_t n = slots(batch, num_chunks) * max_q_len * q_heads;
-  return (size_t)(align256((int64_t)batch * 8) + align256(n * 4) + n * dim * 4);
+  return (size_t)(align256((int64_t)batch * 8) + align256(n * 8) + n * dim * 4);
 }
 
 // gqa_wide.hip: 128 rows to a workgroup.
@@ -1042,8 +1055,8 @@ int run(const char* me, const void* q, int64_t q_stride_t, int64_t q_stride_h, i
     char* ws = (char*)workspace;
     const int64_t n = slots(batch, num_chunks) * max_q_len * q_heads;
     p.seg_ids = (int32_t*)ws;
-    p.part_lse = (float*)(ws + align256((int64_t)batch * 8));
-    p.part_acc = (float*)((char*)p.part_lse + align256(n * 4));
+    p.part_lse = (f32x2*)(ws + align256((int64_t)batch * 8));
+    p.part_acc = (float*)((char*)p.part_lse + align256(n * 8));
   }
   if (wide) return launch_wide_rows(me, p, dtype, dim, cache_dtype == 3, x, stream);
   return dtype == 0 ? pick<kTree, __bf16>(me, p, dim, cache_dtype == 3, mt, row_groups, x, stream)

@@ -539,11 +539,11 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), (D > 128 ? 1 : 2)) void g
           const int64_t t = (int64_t)sq.q0 + tok;
           // (the sum is of the probabilities in fp32: both operands of one are kWhole of it up to their rounding)
           const float total = sum[0] + sum[1] + __shfl_xor(sum[0] + sum[1], 32, 64), inv = total == 0.f ? 0.f : vs / (total * kWhole);
-          const float lse2 = total == 0.f ? -INFINITY : ref + fast_log2(total);
+          const f32x2 lse2 = total == 0.f ? f32x2{-INFINITY, 0.f} : lse_of(ref, fast_log2(total));
           if (r < rows && (only < 0 || tok == only) && (!whole || (t >= 0 && t < last->num_tokens))) {
             const int qh = head * p.group + (r - tok * p.group);
             if (whole) {
-              if (last->lse && h32 == 0) ((GLOBAL float*)last->lse)[t * (p.kv_heads * p.group) + qh] = lse2 * kLn2;
+              if (last->lse && h32 == 0) ((GLOBAL float*)last->lse)[t * (p.kv_heads * p.group) + qh] = lse2[0] * kLn2;
               GLOBAL char* dst = (GLOBAL char*)last->out + t * last->o_st + (int64_t)qh * last->o_sh + here(h32) * 8;
 #pragma unroll
               for (int d = 0; d < D / 32; d++)
@@ -556,7 +556,7 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), (D > 128 ? 1 : 2)) void g
                 }
             } else {
               const int64_t slot = ((int64_t)(chunk + b) * p.kv_heads + head) * (p.max_q_len * p.group) + r;
-              if (h32 == 0) ((GLOBAL float*)last->part_lse)[slot] = lse2;
+              if (h32 == 0) ((GLOBAL f32x2*)last->part_lse)[slot] = lse2;
               GLOBAL float* dst = (GLOBAL float*)last->part_acc + slot * D + h32 * 4;
 #pragma unroll
               for (int d = 0; d < D / 32; d++)
