@@ -821,27 +821,22 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
 
 // The partials of a sequence's chunks into its rows, by the weights exp2(lse_k - max lse): lanes of 4 dims, kWaves wavefronts for a row, each with
 // several partials at once; or (0) the lanes of several rows in a wavefront, each of which goes through its partials, four at once.  Both go by their
-// own partials' largest log-sum-exp, so that all that is read of them is asked for together.
+// own partials' largest log-sum-exp, so that all that is read of them is asked for together.  Rows side by side are few workgroups, and a request that has most
+// of a batch's keys has most of its partials: those of kMany and more get a wavefront for each row behind the others, by what each request has.
 // They are kept in log2 units: behind a product the compiler would subtract from the unrounded one, which is far off beyond 2^32.
 // Bound by the launch and two dependent reads: 2.2 us for 4 rows of 32 partials by four wavefronts; 64 requests x 256 rows of 128 dims of 2 partials 5.8,
 // 8 x 3840 of 3 10 (47 MB), where a wavefront for a row took 8.8 and 13; still ahead of it with 8 partials to a request, 194.8 / 195.2 with the
-// attention.  A weight is at most 2^-24 (kFar), so that sums over results of any size stay finite.
+// attention.  With the attention, all rows side by side / a wavefront to each of those of many: one request of 131 072 keys and 63 of 100, 32/8 heads of 64,
+// 86.7 / 65.1, of 128, 124.1 / 116.6; batches of equal lengths pay up to 1 us for looking.  A weight is at most 2^-24 (kFar), so that sums over results of any size stay finite.
 constexpr float kFar = 24.f;
+constexpr int kMany = 16;
 template <bool kTree, typename T, int D, int kWaves>
-__global__ __launch_bounds__(256) void gqa_join_kernel(const Params p) {
+__device__ __forceinline__ void join_rows(const Params& p, int b, int first, int last, int item, int w) {
   __shared__ float part[4][D], stat[4][3];
   constexpr int kLanes = D / 4, kPer = 64 / kLanes;          // lanes of a partial; partials, or rows, of a wavefront at once
   constexpr int kApart = kWaves == 0 ? 1 : kWaves * kPer;    // between a lane's partials
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / kLanes, gi = lane % kLanes;
-  const int b = blockIdx.y, rows_max = p.max_q_len * p.group;
-  int item, w = 0;
-  if constexpr (kWaves == 0) {
-    item = (blockIdx.x * 4 + wave) * kPer + sub;
-  } else {
-    item = blockIdx.x * (4 / kWaves) + wave / kWaves;
-    w = wave % kWaves * kPer + sub;
-  }
-  const int first = ((ConstPtr)p.seg_ids)[2 * b], last = ((ConstPtr)p.seg_ids)[2 * b + 1];
+  const int rows_max = p.max_q_len * p.group;
   const Seq sq = seq_at<kTree>(p, b);
   if (first < 0) return;
   const int hd = (int)((uint32_t)item / (uint32_t)rows_max), r = item - hd * rows_max;
@@ -931,12 +926,52 @@ __global__ __launch_bounds__(256) void gqa_join_kernel(const Params p) {
   if (p.lse && gi == 0) p.lse[t * (p.kv_heads * p.group) + qh] = sum == 0.f ? -INFINITY : (top[0] + (top[1] + fast_log2(sum) + kFar)) * kLn2;
 }
 
+template <bool kTree, typename T, int D, int kWaves>
+__global__ __launch_bounds__(256) void gqa_join_kernel(const Params p, int many) {
+  constexpr int kPer = 256 / D;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), sub = lane / (D / 4);
+  const ConstPtr ids = (ConstPtr)p.seg_ids;
+  if constexpr (kWaves > 0) {
+    const int b = blockIdx.y;
+    join_rows<kTree, T, D, kWaves>(p, b, ids[2 * b], ids[2 * b + 1], blockIdx.x * (4 / kWaves) + wave / kWaves, wave % kWaves * kPer + sub);
+  } else if ((int)blockIdx.y < p.batch) {
+    const int b = blockIdx.y, first = ids[2 * b], last = ids[2 * b + 1];
+    if (first < 0 || last - first < many) join_rows<kTree, T, D, 0>(p, b, first, last, (blockIdx.x * 4 + wave) * kPer + sub, 0);
+  } else {
+    // a wavefront for a row of the which-th request of many partials, if there is one
+    const int at = ((int)blockIdx.y - p.batch) * (int)gridDim.x + (int)blockIdx.x, groups = (p.kv_heads * p.max_q_len * p.group + 3) / 4;
+    int which = at / groups;
+    const int item = (at - which * groups) * 4 + wave;
+    typedef int32_t i32x2 __attribute__((ext_vector_type(2)));
+    for (int base = 0; base < p.batch; base += 64) {
+      const i32x2 x = ((const GLOBAL i32x2*)p.seg_ids)[base + lane < p.batch ? base + lane : p.batch - 1];
+      uint64_t found = __builtin_amdgcn_ballot_w64(base + lane < p.batch && x[0] >= 0 && x[1] - x[0] >= many);
+      const int n = __builtin_popcountll(found);
+      if (which >= n) {
+        which -= n;
+        continue;
+      }
+      for (; which > 0; which--) found &= found - 1;
+      const int l = __builtin_ctzll(found);
+      join_rows<kTree, T, D, 1>(p, base + l, __builtin_amdgcn_readlane(x[0], l), __builtin_amdgcn_readlane(x[1], l), item, sub);
+      return;
+    }
+  }
+}
+
 template <bool kTree, typename T, int D>
 int launch_join(const char* me, const Params& p, hipStream_t st) {
   // the rows of a wavefront side by side where the chunks leave a few partials to a request, four wavefronts to a row where they leave many
   const int items = p.kv_heads * p.max_q_len * p.group;
-  if (p.num_chunks > 8 * p.batch) hipLaunchKernelGGL((gqa_join_kernel<kTree, T, D, 4>), dim3((unsigned)items, (unsigned)p.batch), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL((gqa_join_kernel<kTree, T, D, 0>), dim3((unsigned)((items + 1024 / D - 1) / (1024 / D)), (unsigned)p.batch), dim3(256), 0, st, p);
+  if (p.num_chunks > 8 * p.batch) {
+    hipLaunchKernelGGL((gqa_join_kernel<kTree, T, D, 4>), dim3((unsigned)items, (unsigned)p.batch), dim3(256), 0, st, p, 0);
+  } else {
+    // (each of a request's partials but its first begins a chunk: there are so many of kMany)
+    const int64_t x = (items + 1024 / D - 1) / (1024 / D), more = ((p.num_chunks - 1) / kMany * (int64_t)((items + 3) / 4) + x - 1) / x;
+    const bool fits = D < 256 && p.batch + more <= 65535;    // (heads of 256: a wavefront has one row either way)
+    hipLaunchKernelGGL((gqa_join_kernel<kTree, T, D, 0>), dim3((unsigned)x, (unsigned)(p.batch + (fits ? more : 0))), dim3(256), 0, st, p,
+                       fits ? kMany : 0x7fffffff);
+  }
   return check_launch(me);
 }
 template <bool kTree, typename T, int D, bool kFp8, int MT>
