@@ -198,6 +198,9 @@ __device__ __forceinline__ Sums scan(int a, int b, int2* parts) {
 
 // Pages: every request's, by one workgroup, kThreads of them at a time; a thread's own stays in registers where that is all there are.
 struct Room { int2 parts[kThreads / 64]; int upto[kThreads], end[kThreads]; };
+// A page or a few to a request are its thread's.  More: a page to a thread, which finds the request by its sum.  us, one request that ends with 512 pages by
+// its thread / by all 50-59 / 4.5, with 8192 815 / 6.4, 64 with 512 98 / 25, 64 with three 4.4 / 5.0.
+constexpr int kOwn = 2, kOwnBack = 4;
 __device__ void pages(const Params& p, Room& room, int32_t* ctx, int32_t* len) {
   const int tid = threadIdx.x;
   const int there = *p.num_free;
@@ -224,6 +227,19 @@ __device__ void pages(const Params& p, Room& room, int32_t* ctx, int32_t* len) {
   int free = there < 0 ? 0 : there < p.capacity ? there : p.capacity;
   // pages that go back: how many in all, then each to its place
   int back = 0, before = 0;
+  // page k of a request's that end at room.upto: f(the request's row, the page's entry in it)
+  auto spread = [&](int base, int all, auto fits, auto f) {
+    const int rows = p.batch - base < kThreads ? p.batch - base : kThreads;
+    for (int k = tid; k < all; k += kThreads) {
+      int lo = 0, hi = rows - 1;
+      while (lo < hi) {                                      // the first whose sum is above k
+        const int mid = (lo + hi) >> 1;
+        if (room.upto[mid] > k) hi = mid;
+        else lo = mid + 1;
+      }
+      if (fits(room.upto[lo])) f(k, p.table + (base + lo) * p.table_stride + room.end[lo] - (room.upto[lo] - k));
+    }
+  };
   each([&](int) { back += s.all_a; });
   if (free + back > p.capacity) {
     back = 0;
@@ -235,11 +251,24 @@ __device__ void pages(const Params& p, Room& room, int32_t* ctx, int32_t* len) {
   }
   if (back > 0) {
     each([&](int base) {
-      if (m.give > 0 && before + s.a + free <= p.capacity) {
-        const int32_t* row = p.table + (base + tid) * p.table_stride + m.t;
-        const int first = free + back - 1 - (before + s.a - m.give);
-        for (int k = 0; k < m.give; k++) p.free_pages[first - k] = row[k];
-        p.held[base + tid] = m.t;
+      const bool goes = m.give > 0 && before + s.a + free <= p.capacity;
+      if (goes) p.held[base + tid] = m.t;
+      if (s.all_a > 0) {
+        room.upto[tid] = s.a;
+        room.end[tid] = m.h;
+        const int top = free + back - 1 - before;
+        if (__syncthreads_or(m.give > kOwnBack)) {
+          spread(base, s.all_a, [&](int upto) { return before + upto + free <= p.capacity; }, [&](int k, const int32_t* at) { p.free_pages[top - k] = *at; });
+          __syncthreads();
+        } else if (goes) {
+          const int32_t* row = p.table + (base + tid) * p.table_stride + m.t;
+          int32_t mine[kOwnBack];
+#pragma unroll
+          for (int k = 0; k < kOwnBack; k++) mine[k] = row[k < m.give ? k : 0];
+#pragma unroll
+          for (int k = 0; k < kOwnBack; k++)
+            if (k < m.give) p.free_pages[top - (s.a - m.give) - k] = mine[k];
+        }
       }
       before += s.all_a;
     });
@@ -261,23 +290,11 @@ __device__ void pages(const Params& p, Room& room, int32_t* ctx, int32_t* len) {
       if (m.need > 0 && got) p.held[base + tid] = m.t;
     }
     if (s.all_b > 0) {
-      // A page or a few to a request: by its thread.  More: a page to a thread, which finds the request by its sum.
-      constexpr int kOwn = 2;
       room.upto[tid] = s.b;
       room.end[tid] = m.t;
       const int all = s.all_b;
       if (__syncthreads_or(m.need > kOwn)) {
-        const int rows = p.batch - base < kThreads ? p.batch - base : kThreads;
-        for (int k = tid; k < all; k += kThreads) {
-          int lo = 0, hi = rows - 1;
-          while (lo < hi) {                                  // the first whose sum is above k
-            const int mid = (lo + hi) >> 1;
-            if (room.upto[mid] > k) hi = mid;
-            else lo = mid + 1;
-          }
-          if (before + room.upto[lo] <= free)
-            p.table[(base + lo) * p.table_stride + room.end[lo] - (room.upto[lo] - k)] = p.free_pages[free - 1 - before - k];
-        }
+        spread(base, all, [&](int upto) { return before + upto <= free; }, [&](int k, int32_t* at) { *at = p.free_pages[free - 1 - before - k]; });
       } else if (got) {
 #pragma unroll
         for (int k = 0; k < kOwn; k++)
