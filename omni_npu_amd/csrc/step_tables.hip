@@ -225,7 +225,8 @@ __device__ void pages(const Params& p, Room& room, int32_t* ctx, int32_t* len) {
   };
   if (p.batch <= kThreads) look(0);
   int free = there < 0 ? 0 : there < p.capacity ? there : p.capacity;
-  // pages that go back: how many in all, then each to its place
+  // pages that go back: how many in all, then each to its place (all sums of pages are below 2^31, as tables have fewer, with those of the list they need not be)
+  const int left = p.capacity - free;
   int back = 0, before = 0;
   // page k of a request's that end at room.upto: f(the request's row, the page's entry in it)
   auto spread = [&](int base, int all, auto fits, auto f) {
@@ -241,24 +242,24 @@ __device__ void pages(const Params& p, Room& room, int32_t* ctx, int32_t* len) {
     }
   };
   each([&](int) { back += s.all_a; });
-  if (free + back > p.capacity) {
+  if (back > left) {
     back = 0;
     each([&](int) {
-      back += scan(before + s.a + free <= p.capacity ? m.give : 0, 0, room.parts).all_a;
+      back += scan(before + s.a <= left ? m.give : 0, 0, room.parts).all_a;
       before += s.all_a;
     });
     before = 0;
   }
   if (back > 0) {
     each([&](int base) {
-      const bool goes = m.give > 0 && before + s.a + free <= p.capacity;
+      const bool goes = m.give > 0 && before + s.a <= left;
       if (goes) p.held[base + tid] = m.t;
       if (s.all_a > 0) {
         room.upto[tid] = s.a;
         room.end[tid] = m.h;
         const int top = free + back - 1 - before;
         if (__syncthreads_or(m.give > kOwnBack)) {
-          spread(base, s.all_a, [&](int upto) { return before + upto + free <= p.capacity; }, [&](int k, const int32_t* at) { p.free_pages[top - k] = *at; });
+          spread(base, s.all_a, [&](int upto) { return before + upto <= left; }, [&](int k, const int32_t* at) { p.free_pages[top - k] = *at; });
           __syncthreads();
         } else if (goes) {
           const int32_t* row = p.table + (base + tid) * p.table_stride + m.t;

@@ -73,3 +73,27 @@ def test_giving_back_takes_as_long_as_taking(dev):
 
     take, give = us(n * page - 1, 0, n), us(-1, n, 0)
     assert give < 2 * take + 20, (take, give)
+
+
+@pytest.mark.parametrize("left", [0, 2, 9, 10, 4000])
+def test_a_list_of_two_thousand_million_pages(dev, left):
+    """Pages on the list and pages that go back are more than 2^31 together: from the first request that they do not fit for on, none go back."""
+    from omni_npu_amd import kernels as K
+    most = 2 ** 31 - 1
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)
+    free = torch.empty(most, dtype=torch.int32, device=dev)
+    free[-5000:] = 7
+    held, table = [4, 6, 4001], torch.arange(3 * 4001, dtype=torch.int32, device=dev).view(3, 4001)
+    num_blocks, num_free, seq = i32(*held), i32(most - left), i32(5, 5, 5)
+    rows = lambda: torch.zeros(3, dtype=torch.int64, device=dev)
+    K.step_tables(i32(-1, -1, -1), table, 16, seq, rows(), rows(), num_blocks=num_blocks, free_pages=free, num_free=num_free)
+    back, given = [], 0
+    for b, h in enumerate(held):
+        given += h
+        if given <= left:
+            back += table[b, :h].tolist()
+            held[b] = 0
+    want = [7] * 5000
+    want[5000 - left:5000 - left + len(back)] = back[::-1]
+    assert num_blocks.tolist() == held and num_free.tolist() == [most - left + len(back)] and seq.tolist() == [0, 0, 0]
+    assert free[-5000:].tolist() == want
