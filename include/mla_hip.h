@@ -654,8 +654,8 @@ int mlahip_copy_pages(const mlahip_page_cache* caches, int32_t num_caches, const
  * accepted_stride apart), and kept_lens[b] = context_lens[b] + their number.  A path is numbers of the request's new tokens, each larger than the one before:
  * it ends at its first entry that is not, that is no token of the request (context_lens[b] + it >= seq_lens[b]) or whose page, or the place's that it would
  * go to, is not in the table or the cache.  Idle places (negative context) keep their length.  All but ``caches`` on the device; kept_lens shares
- * no memory with what is read.  Requests must not share the pages that their new tokens lie in, nor caches memory (the same one twice is refused).  Rows of
- * at most 2 MB. */
+ * no memory with what is read.  Requests must not share the pages that their new tokens lie in.  Caches that share memory are refused, and so are those that lie in one another with
+ * pages (or, of one page, rows) differently far apart.  Rows of at most 2 MB. */
 int mlahip_keep_rows(const mlahip_page_cache* caches, int32_t num_caches, int64_t num_pages, int32_t page_size, const int32_t* block_table,
                      int64_t bt_stride, int32_t max_blocks, const int32_t* context_lens, const int32_t* seq_lens, int32_t batch,
                      const int32_t* accepted, int64_t accepted_stride, int32_t max_accepted, const int32_t* num_accepted, int32_t* kept_lens,

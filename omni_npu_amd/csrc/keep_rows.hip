@@ -13,7 +13,8 @@
 // (one takes up what another waits for); pieces of a row in neighbouring wavefronts 5.3 and 59.
 #include "mla_common.hpp"
 #include "../../include/mla_hip.h"
-#include <string.h>
+#include <algorithm>
+#include <new>
 
 namespace mlahip {
 namespace keep {
@@ -104,6 +105,98 @@ __global__ __launch_bounds__(256) void keep_rows_kernel(const Params p) {
   if (p.kept && blockIdx.y == 0 && blockIdx.z == 0 && lane == 0) p.kept[b] = ctx < 0 ? ctx : ctx + kept;
 }
 
+// ---- caches that share memory (on the host): two moves of the same bytes would take each other's results for what they read ----
+// A cache as blocks that lie ``outer`` apart, each of rows ``inner`` apart: pages of rows, or, where these lie inside rows, rows of pages.
+struct Layout {
+  int64_t begin, end;                                        // of all of it
+  int64_t outer, inner, row;
+  int32_t blocks, rows;
+  int64_t block() const { return (rows - 1) * inner + row; }
+};
+bool layout_of(const mlahip_page_cache& c, int32_t pages, int32_t page_size, Layout* x) {
+  const int64_t begin = (int64_t)(uintptr_t)c.base;
+  if (pages == 1) *x = {begin, 0, c.row_stride_bytes, 0, c.row_bytes, page_size, 1};
+  else if (page_size == 1) *x = {begin, 0, c.page_stride_bytes, 0, c.row_bytes, pages, 1};
+  else if (c.page_stride_bytes >= c.row_stride_bytes) *x = {begin, 0, c.page_stride_bytes, c.row_stride_bytes, c.row_bytes, pages, page_size};
+  else *x = {begin, 0, c.row_stride_bytes, c.page_stride_bytes, c.row_bytes, page_size, pages};
+  int64_t size;
+  return !__builtin_mul_overflow((int64_t)(x->blocks - 1), x->outer, &size) && !__builtin_add_overflow(size, x->block(), &size) &&
+         !__builtin_add_overflow(begin, size, &x->end);
+}
+int64_t floor_div(int64_t a, int64_t b) { return a / b - (a % b < 0); }
+// A block of a and one of b, which begins ``apart`` behind it.
+bool blocks_meet(const Layout& a, const Layout& b, int64_t apart) {
+  if (apart >= a.block() || apart + b.block() <= 0) return false;
+  const auto last_in_front_of = [&](int64_t end, int32_t rows) {   // b's last row that begins in front of ``end``, of so many
+    if (rows == 1) return (int64_t)(apart < end ? 0 : -1);
+    const int64_t r = floor_div(end - 1 - apart, b.inner);
+    return r < rows - 1 ? r : (int64_t)rows - 1;
+  };
+  if (a.inner == b.inner && a.rows == b.rows) {              // by how many rows b's lie further: -rows < k < rows
+    if (a.rows == 1) return true;                            // (two rows that overlap, as said above)
+    const int64_t k = floor_div(a.row - 1 - apart, a.inner), most = k < a.rows - 1 ? k : a.rows - 1;
+    return most > -(int64_t)a.rows && apart + most * a.inner + b.row > 0;
+  }
+  for (int64_t i = 0; i < a.rows; i++) {
+    const int64_t at = i * a.inner, r = last_in_front_of(at + a.row, b.rows);
+    if (r >= 0 && apart + r * b.inner + b.row > at) return true;
+  }
+  return false;
+}
+// Blocks that lie differently far apart are not looked through: they are taken to share memory where one cache begins in the other.
+bool caches_meet(const Layout& a, const Layout& b) {
+  if (a.end <= b.begin || b.end <= a.begin) return false;
+  if (a.outer != b.outer || a.blocks != b.blocks) return true;
+  if (a.blocks == 1) return blocks_meet(a, b, b.begin - a.begin);
+  const int64_t n = floor_div(b.begin - a.begin, a.outer), apart = b.begin - a.begin - n * a.outer;
+  const auto some = [&](int64_t by) { return by > -(int64_t)a.blocks && by < a.blocks; };
+  return (some(n) && blocks_meet(a, b, apart)) || (some(n + 1) && blocks_meet(a, b, apart - a.outer));
+}
+// Two of them that share memory; false: none do.  In order of their beginnings, and those that lie in one another (of one storage) as pieces of a block, or of a
+// row, where they are such pieces, so that each is held against the next one alone: 128 caches of one storage take 2 us; each against
+// each, as where rows of two strides lie between each other, 64 take 66.
+struct Place { int64_t at; int32_t of; };
+void in_order(Place* x, int32_t n) {
+  const auto less = [](const Place& a, const Place& b) { return a.at < b.at; };
+  if (!std::is_sorted(x, x + n, less)) std::sort(x, x + n, less);
+}
+bool any_meet(const Layout* all, Place* places, int32_t n, int32_t* one, int32_t* other) {
+  for (int32_t i = 0; i < n; i++) places[i] = {all[i].begin, i};
+  in_order(places, n);
+  for (int32_t i = 0, next; i < n; i = next) {
+    const Layout& first = all[places[i].of];
+    int64_t end = first.end;
+    bool alike = true, rows = true;
+    for (next = i + 1; next < n && places[next].at < end; next++) {
+      const Layout& x = all[places[next].of];
+      end = x.end > end ? x.end : end;
+      alike = alike && x.outer == first.outer;
+      rows = rows && x.inner == first.inner && x.rows == first.rows;
+    }
+    const int32_t m = next - i;
+    Place* x = places + i;
+    if (m == 1) continue;
+    // places modulo a stride, each with what it takes there: apart from the next one, and the last from the first
+    const auto apart = [&](int64_t stride, auto size) {
+      for (int32_t k = 0; k < m; k++) x[k].at = (all[x[k].of].begin - first.begin) % stride;
+      in_order(x, m);
+      for (int32_t k = 0; k < m; k++)
+        if (x[k].at + size(all[x[k].of]) > (k + 1 < m ? x[k + 1].at : x[0].at + stride)) return false;
+      return true;
+    };
+    if (alike && apart(first.outer, [](const Layout& y) { return y.block(); })) continue;
+    if (alike && rows && first.rows > 1 && first.outer % first.inner == 0 && apart(first.inner, [](const Layout& y) { return y.row; })) continue;
+    for (int32_t k = 0; k < m; k++)
+      for (int32_t l = k + 1; l < m; l++)
+        if (caches_meet(all[x[k].of], all[x[l].of])) {
+          *one = x[k].of < x[l].of ? x[k].of : x[l].of;
+          *other = x[k].of < x[l].of ? x[l].of : x[k].of;
+          return true;
+        }
+  }
+  return false;
+}
+
 }  // namespace keep
 }  // namespace mlahip
 using namespace mlahip;
@@ -132,14 +225,29 @@ extern "C" int mlahip_keep_rows(const mlahip_page_cache* caches, int32_t num_cac
                 MLA_ERR_SHAPE, "%s: cache %d: pages that share memory: rows of %lld bytes, %lld apart, %d to a page, pages %lld apart", me, i,
                 (long long)c.row_bytes, (long long)c.row_stride_bytes, page_size, (long long)c.page_stride_bytes);
   }
-  // Two moves of the same rows would take each other's results for what they read.  (A bit for an address: looked at again where two have one.)
-  uint64_t bits[64] = {};
-  for (int32_t i = 0; i < num_caches; i++) {
-    const uint32_t at = (uint32_t)((uint64_t)(uintptr_t)caches[i].base * 0x9e3779b97f4a7c15ull >> 52);
-    const bool met = bits[at >> 6] >> (at & 63) & 1;
-    for (int32_t k = 0; met && k < i; k++)
-      MLA_REQUIRE(caches[k].base != caches[i].base, MLA_ERR_UNSUPPORTED, "%s: caches %d and %d are the same", me, k, i);
-    bits[at >> 6] |= 1ull << (at & 63);
+  {
+    constexpr int32_t kFew = 256;
+    keep::Layout few[kFew], *layouts = few;
+    keep::Place few_places[kFew], *places = few_places;
+    if (num_caches > kFew) {
+      layouts = new (std::nothrow) keep::Layout[num_caches];
+      places = new (std::nothrow) keep::Place[num_caches];
+    }
+    int32_t one = 0, other = 0, past = -1;
+    bool meet = false;
+    const bool room = layouts && places;
+    if (room) {
+      for (int32_t i = 0; i < num_caches && past < 0; i++)
+        if (!keep::layout_of(caches[i], (int32_t)num_pages, page_size, layouts + i)) past = i;
+      meet = past < 0 && keep::any_meet(layouts, places, num_caches, &one, &other);
+    }
+    if (num_caches > kFew) {
+      delete[] layouts;
+      delete[] places;
+    }
+    MLA_REQUIRE(room, MLA_ERR_UNSUPPORTED, "%s: no memory to look through %d caches", me, num_caches);
+    MLA_REQUIRE(past < 0, MLA_ERR_SHAPE, "%s: cache %d: pages %lld apart end past all addresses", me, past, (long long)caches[past < 0 ? 0 : past].page_stride_bytes);
+    MLA_REQUIRE(!meet, MLA_ERR_UNSUPPORTED, "%s: caches %d and %d share memory", me, one, other);
   }
   if (batch == 0) return MLA_OK;
   const char *out = (const char*)kept_lens, *out_end = out + batch * 4ll;

@@ -1825,8 +1825,8 @@ def keep_rows(caches, block_table: torch.Tensor, context_lens: torch.Tensor, seq
     All of it lies on the device: ``block_table`` int32 [>= B, blocks], ``context_lens`` and ``seq_lens`` int32 [B] as step_tables has them, ``accepted``
     int32 [B,A] (numbers of a request's new tokens, each larger than the one before, as a path down a tree is), ``num_accepted`` and ``kept_lens``
     int32 [B].  A path ends at its first entry that is not larger, that is no token of its request, or whose rows are not in the table or the
-    caches.  Idle places keep their negative length.  Requests must not share the pages that their new tokens lie in, nor caches memory (the same
-    one twice is refused)."""
+    caches.  Idle places keep their negative length.  Requests must not share the pages that their new tokens lie in.  Caches that share memory
+    are refused, and so are those that lie in one another with their pages differently far apart."""
     what = "keep_rows"
     native = _host.load().keep_rows
     if native(caches, block_table, context_lens, seq_lens, accepted, num_accepted, kept_lens):     # (a list of tensors)
