@@ -622,7 +622,10 @@ int mlahip_gqa_tree_decode(const void* q, int64_t q_stride_t, int64_t q_stride_h
  * fit fewer; an idle place needs none) go back behind the list's end, the last one named first, so that they would be taken again in the order in which they
  * were held; then pages are taken from the list's end, in the order of the requests.  A request whose table has no room, or for whom and those
  * in front of it the list is too short, gets no page: its length stays context_lens[b] and its tokens get no slots.  A list without room for what
- * comes back takes none of it from that request on.  Entries behind a request's pages are left as they were.
+ * comes back takes none of it from that request on.  Entries behind a request's pages are left as they were.  All of a request's num_blocks pages go
+ * back when it ends, so each is in one table only, and once: a page that two tables share (a fork by mlahip_copy_pages with rows) would be handed out
+ * while the other one still reads it, and pages that are moved (its block_table) have to change places with the list's.  A request without pages, a context
+ * and no new tokens is given pages for its context: those of a fork, whole, to copy into.
  * seq_lens [batch]: context + n (idle: 0).  positions, slot_mapping [num_tokens] int64: token i's position context + i, and the cache row of place
  * context + i by the block table, -1 where the table ends or names no page; rows behind the last request and an idle place's get 0 and -1.
  * With parents [num_tokens] (a token's parent among its request's tokens, in front of it; anything else: it follows the context) positions are context +

@@ -1705,7 +1705,10 @@ def step_tables(context_lens: torch.Tensor, block_table: torch.Tensor, page_size
     With ``num_blocks`` int32 [B], ``free_pages`` int32 [pages] and ``num_free`` int32 [1] the block table is kept as well: pages that a request
     needs are taken from the end of free_pages[:num_free], in the order of the requests, those that it needs no more go back there first, so that they
     would come out again in their order.  A request that the table or the list has too few pages for keeps the length of its context and gets no slots, and
-    so does every one behind it that needs pages, where the list is short.
+    so does every one behind it that needs pages, where the list is short.  Its rows of the step are to be thrown away (seq_lens[b] == context_lens[b]
+    with tokens in the step): attention over them works something out, and it is not theirs.  A page that is kept so is in one table only: a request
+    that ends gives back all of its pages, those too that a fork shares (copy_pages with ``rows``).  A fork gets pages of its own by a step with its context and no
+    tokens, into which copy_pages copies all of the other's; pages that copy_pages moves have to change places with the list's.
     With ``parents`` int32 [T], a token's parent among its request's tokens (in front of it; anything else: the token follows the context),
     positions go by the depth, and ``visible`` int64 [T,W] gets the bits of the token and its ancestors, for gqa_tree_decode."""
     what = "step_tables"
