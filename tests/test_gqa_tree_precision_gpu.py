@@ -160,6 +160,37 @@ def test_equal_scores_of_any_size_weigh_the_same(dev, dtype, scale, sign, behind
     assert torch.allclose(lse.double(), l, rtol=2.0 ** -21)
 
 
+@pytest.mark.parametrize("d", [64, 128, 256])
+@BOTH
+@pytest.mark.parametrize("fp8", [False, True], ids=["same", "e4m3"])
+@pytest.mark.parametrize("scale", [2.0 ** -11, 1.0, 64.0, 2.0 ** 14])
+@pytest.mark.parametrize("chunks", [0, 9])
+@ROWS
+def test_equal_scores_of_any_head_and_cache(dev, d, dtype, fp8, scale, chunks, rows):
+    """The same with scales of the cache's heads, in pieces (their log-sum-exps' sums off by a few times 2^-20), and a value that is no number where some tokens
+    do not see it, so that those are done by themselves."""
+    s = 9
+    c = tree(make(dev, [300, 75], q_len=s, hq=8, hk=2, d=d, dtype=dtype, fp8=fp8, page=16, seed=2), seed=2)
+    c["scale"] = scale
+    c["q"].zero_()
+    c["q"][..., 0] = 32768.0
+    for name, at, x in (("k", (Ellipsis, 0), 96.0), ("v", (c["table"][0, (300 - s + 3) // 16].long(), (300 - s + 3) % 16), float("nan"))):
+        y = c[name].float()
+        y[at] = x
+        c[name] = y.to(c[name].dtype)
+    if fp8:
+        c["k_scale"] = torch.tensor([0.5, 4.0])
+    rows_of = ~torch.cat((seen(c, 0, s)[:, 300 - s + 3], torch.zeros(s, dtype=torch.bool)))
+    assert 0 < rows_of.sum() < 2 * s
+    out, lse = call(dev, c, s, num_chunks=chunks, **own_rows(rows, d))
+    o, l, weight, reach = exact(c)
+    clean = dict(c, v=c["v"].float().nan_to_num(0.0))
+    tol = tolerance(clean, o, weight, torch.zeros_like(reach), l) + 2.0 ** -18 * (weight + o.abs())
+    err = (out.double() - o).abs()
+    assert (err[rows_of] <= tol[rows_of]).all(), f"worst {(err / tol)[rows_of].max():.3g} of the tolerance"
+    assert torch.isnan(out[~rows_of].float()).all() and torch.allclose(lse.double(), l, rtol=2.0 ** -21)
+
+
 @BOTH
 @pytest.mark.parametrize("lens,chunks", [([6, 7, 40, 700], 0), ([6, 7, 40, 700], 9), ([5000], 1), ([5000], 40), ([5000, 3000, 20], 30)])
 @pytest.mark.parametrize("d", [64, 256])
