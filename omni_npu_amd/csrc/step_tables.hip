@@ -13,8 +13,9 @@
 // A few KB: what takes time is what waits for something else.  A launch of this takes 3.3 us when it does nothing for tokens, of which one is the first
 // loads' way; so all of a request's numbers are asked for at once, one scan adds up what is given back and what is needed (the others only where a
 // list is too short), what tokens look up lies in LDS, parents too (a tree ten deep is ten loads behind each other), and a token's page is under way
-// meanwhile.  us: one token 4.1, 67 requests of 26 tokens as trees 6.2, 500 of up to 64 8.4 (pages 3.3, tokens 5), 16 000 tokens of prompts 6.3; loads
-// where they are used: 4.5, 9.0, 9.3, 6.9.
+// meanwhile.  us, where no page moves: one token 4.1, 67 requests of 26 tokens as trees 6.2, 500 of up to 64 8.4 (pages 3.3, tokens 5), 16 000 tokens of
+// prompts 6.3; loads where they are used: 4.5, 9.0, 9.3, 6.9.  Kernels alone, none / the steps' pages taken: trees of 67 6.0 / 8.4 (104 pages, and 6 back), the
+// pages' launch of 500 requests 3.4 / 4.0, of nine prompts 3.2 / 4.2 (128 pages).
 #include "mla_common.hpp"
 #include "../../include/mla_hip.h"
 
