@@ -827,7 +827,8 @@ __global__ __launch_bounds__((Shape<T, D, kFp8, MT>::waves * 64)) void gqa_split
 // Bound by the launch and two dependent reads: 2.2 us for 4 rows of 32 partials by four wavefronts; 64 requests x 256 rows of 128 dims of 2 partials 5.8,
 // 8 x 3840 of 3 10 (47 MB), where a wavefront for a row took 8.8 and 13; still ahead of it with 8 partials to a request, 194.8 / 195.2 with the
 // attention.  With the attention, all rows side by side / a wavefront to each of those of many: one request of 131 072 keys and 63 of 100, 32/8 heads of 64,
-// 86.7 / 65.1, of 128, 124.1 / 116.6; batches of equal lengths pay up to 1 us for looking.  A weight is at most 2^-24 (kFar), so that sums over results of any size stay finite.
+// 86.7 / 65.1, of 128, 124.1 / 116.6; batches of equal lengths pay up to 1 us for looking.  A weight is at most 2^-24 (kFar), so that sums over results of
+// any size stay finite.
 constexpr float kFar = 24.f;
 constexpr int kMany = 16;
 template <bool kTree, typename T, int D, int kWaves>

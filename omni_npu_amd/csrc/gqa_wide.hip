@@ -343,7 +343,8 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), (D > 128 ? 1 : 2)) void g
           const u32x2 x0 = read_tr(row), x1 = read_tr(row + 8 * W::row_b);
           return u32x4{x0[0], x0[1], x1[0], x1[1]};
         };
-        // Where a score outgrows its row's reference the wavefront's are set anew (all of them: the next would follow soon): what is summed up, and the probabilities that are not yet, by a whole power of two.
+        // Where a score outgrows its row's reference the wavefront's are set anew (all of them, the next would follow soon: fp16 6 % faster than one by one):
+        // what is summed up, and the probabilities that are not yet, by a whole power of two.
         auto check = [&](int key, bool partial, float most) {
           if (partial) {
             const uint32_t bits = (tile_bits(tok, key) & ~bits_to(lo - key)) >> 4 * h32;
@@ -359,6 +360,7 @@ __global__ __launch_bounds__((Wide<D, kFp8>::threads), (D > 128 ? 1 : 2)) void g
             // Large scores: the turn's y is an unrounded score less the reference, the tile's that set the reference a rounded one's, and a reference
             // does not move by less than its own steps: equal scores would weigh more or less by the tile that they lie in (at 2^20 by 4 %, beyond 2^25 all of it).
             // So each tile of such a row is looked at here, and has its products again: rounded, then less the reference, which is a whole number near them.
+            // (8 requests of 480 rows, 2000-16 000 keys 269 us, all rows such 428; every row's products rounded in the turn instead 2.5 % more for all.)
             const bool anew = most > -INFINITY, large = anew && (fabsf(ref) >= kFine || fabsf(ref + most) >= kFine);
             const float before = ref;
             if (__builtin_expect(__builtin_amdgcn_ballot_w64(large) != 0, 0)) {
